@@ -10,10 +10,11 @@ from .codebook import Codebook, validate_image_path
 from .engine import HipEngine
 from .gray import GrayCodebook
 from .pipeline import EncodePipeline
+from .cache import train_cache_codebooks
 from .lbg import train_lbg, lbg_iteration, initial_centroid, final_codebook_size, LBGResult
 from ._lib import VQ_MODE_EXACT, VQ_MODE_FAST, VQ_PAD_EDGE, VQ_PAD_ZERO
 
 __all__ = [
-    "Codebook", "GrayCodebook", "validate_image_path", "HipEngine", "EncodePipeline", "train_lbg", "lbg_iteration", "initial_centroid",
+    "Codebook", "GrayCodebook", "validate_image_path", "HipEngine", "EncodePipeline", "train_cache_codebooks", "train_lbg", "lbg_iteration", "initial_centroid",
     "final_codebook_size", "LBGResult", "VQ_MODE_EXACT", "VQ_MODE_FAST", "VQ_PAD_EDGE", "VQ_PAD_ZERO",
 ]

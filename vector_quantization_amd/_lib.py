@@ -1,4 +1,4 @@
-"""ctypes binding of libvqhip.so (the C ABI declared in include/vq_hip.h).
+"""ctypes binding of libvqhip.so (the C ABI declared in include/vq_hip.h and include/vq_cache.h).
 
 The library is the only compute backend of this package: if it cannot be loaded the import
 fails loudly -- there is no CPU fallback.
@@ -19,6 +19,10 @@ VQ_MODE_FAST = 1
 
 VQ_PAD_EDGE = 0
 VQ_PAD_ZERO = 1
+
+VQ_F32 = 0
+VQ_BF16 = 1
+VQ_F16 = 2
 
 ABI_VERSION = 8
 
@@ -68,6 +72,18 @@ SIGNATURES = {
     "vq_unpack_labels": (_i, [_vp, _i64, _i, _vp, _vp]),
 }
 
+# the same for include/vq_cache.h
+CACHE_SIGNATURES = {
+    "vq_cache_write": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _i64, _i, _vp]),
+    "vq_cache_read": (_i, [_vp, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _i64, _i, _vp, _vp, _vp]),
+    "vq_cache_attention_ws_bytes": (_sz, [_i64, _i, _i, _i, _i, _i, _i, _i64, _i64]),
+    "vq_cache_attention": (_i, [_vp, _i64, _i64, _i64, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _i64, _i, _vp, _i, _i, _vp, _vp,
+                                _i64, _i64, _dbl, _vp, _vp, _vp, _sz, _vp]),
+    "vq_cache_lbg_ws_bytes": (_sz, [_i64, _i, _i, _i, _i]),
+    "vq_cache_lbg_accum": (_i, [_vp, _i64, _i64, _i64, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vq_cache_lbg_finish": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp]),
+}
+
 
 def library_path():
     """Path of libvqhip.so: $VQ_HIP_LIB if set, else the in-tree build."""
@@ -92,7 +108,7 @@ def _load():
         lib = ctypes.CDLL(path)
     except OSError as exc:  # pragma: no cover - depends on the machine
         raise VQLibraryError(f"cannot load {path}: {exc}") from exc
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in (*SIGNATURES.items(), *CACHE_SIGNATURES.items()):
         try:
             fn = getattr(lib, name)
         except AttributeError as exc:

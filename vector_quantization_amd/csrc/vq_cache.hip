@@ -1,0 +1,453 @@
+// vq_cache.hip -- HIP kernels (gfx950 / CDNA4) and C ABI of the vector-quantised key-value cache (vq_cache.h).
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "vq_cache.h"
+#include "vq_hip.h"
+
+__attribute__((visibility("hidden"))) int vq_internal_fail(int code, const char *message);
+__attribute__((visibility("hidden"))) int vq_internal_device(int *cus);
+
+namespace {
+
+int fail(int code, const char *fmt, ...) {
+    char text[400];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(text, sizeof(text), fmt, ap);
+    va_end(ap);
+    return vq_internal_fail(code, text);
+}
+
+#define LAUNCH_CHECK(name)                                                                         \
+    do {                                                                                           \
+        hipError_t e_ = hipGetLastError();                                                         \
+        if (e_ != hipSuccess) return fail(VQ_E_HIP, "launch of %s failed: %s", name, hipGetErrorString(e_)); \
+    } while (0)
+
+// ------------------------------------------------------------------------------------------------
+// kernels
+// ------------------------------------------------------------------------------------------------
+
+// Number of the codeword nearest to the sub-vector x, by the definition: squared distance summed left to right in
+// fp64, strictly less wins.  cb points at codeword 0's sub-vector, codewords are `row` elements apart.
+template <typename T, typename C>
+__device__ int nearest_f64(const T *x, const C *cb, int row, int sub, int K, double *least) {
+    double best = INFINITY;
+    int code = 0;
+    for (int k = 0; k < K; ++k) {
+        double d = 0.0;
+        for (int e = 0; e < sub; ++e) {
+            const double t = (double)(float)x[e] - (double)(float)cb[(int64_t)k * row + e];
+            d += t * t;
+        }
+        if (d < best) {
+            best = d;
+            code = k;
+        }
+    }
+    *least = best;
+    return code;
+}
+
+struct WriteArgs {
+    const void *x[2];
+    int64_t token_stride[2], head_stride[2];
+    const void *cb[2];
+    const int64_t *slots;
+    int64_t tokens, pages;
+    int cb_heads, heads, dim, sub, K, page;
+    uint8_t *k_codes, *v_codes;
+};
+
+// Where the code of one sub-vector lies.
+__device__ inline int64_t code_at(int which, int64_t slot, int h, int m, int heads, int parts, int page) {
+    const int64_t p = slot / page;
+    const int o = (int)(slot % page);
+    return which == 0 ? ((p * heads + h) * page + o) * parts + m : ((p * heads + h) * parts + m) * page + o;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_cache_write(const WriteArgs a) {
+    const int parts = a.dim / a.sub;
+    const int64_t n = a.tokens * a.heads * parts;
+    const int which = blockIdx.y;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int m = (int)(i % parts), h = (int)(i / parts % a.heads);
+        const int64_t t = i / parts / a.heads, slot = a.slots[t];
+        if (slot < 0 || slot >= a.pages * a.page) continue;
+        const T *x = static_cast<const T *>(a.x[which]) + t * a.token_stride[which] + h * a.head_stride[which] + m * a.sub;
+        const T *cb = static_cast<const T *>(a.cb[which]) + (a.cb_heads == 1 ? 0 : (int64_t)h * a.K * a.dim) + m * a.sub;
+        double least;
+        const int code = nearest_f64(x, cb, a.dim, a.sub, a.K, &least);
+        (which == 0 ? a.k_codes : a.v_codes)[code_at(which, slot, h, m, a.heads, parts, a.page)] = (uint8_t)code;
+    }
+}
+
+struct ReadArgs {
+    const int64_t *slots;
+    int64_t tokens, pages;
+    const void *cb[2];
+    int cb_heads, heads, dim, sub, K, page;
+    const uint8_t *codes[2];
+    void *out[2];
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_cache_read(const ReadArgs a) {
+    const int parts = a.dim / a.sub;
+    const int64_t n = a.tokens * a.heads * parts;
+    const int which = blockIdx.y;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int m = (int)(i % parts), h = (int)(i / parts % a.heads);
+        const int64_t slot = a.slots[i / parts / a.heads];
+        const bool there = slot >= 0 && slot < a.pages * a.page;
+        int code = there ? a.codes[which][code_at(which, slot, h, m, a.heads, parts, a.page)] : 0;
+        code = code < a.K ? code : a.K - 1;
+        const T *cb = static_cast<const T *>(a.cb[which]) + ((a.cb_heads == 1 ? 0 : (int64_t)h * a.K) + code) * a.dim + m * a.sub;
+        T *out = static_cast<T *>(a.out[which]) + i * a.sub;
+        for (int e = 0; e < a.sub; ++e) out[e] = there ? cb[e] : (T)0.0f;
+    }
+}
+
+struct AttendArgs {
+    const void *q;
+    int64_t q_token_stride, q_head_stride, rows;
+    int q_heads;
+    const void *cb[2];
+    int cb_heads, heads, dim, sub, K;
+    const uint8_t *codes[2];
+    int64_t pages;
+    int page;
+    const int32_t *table;
+    int seqs, width;
+    const int32_t *kv_lens, *starts;
+    float scale;
+    void *out;
+    float *lse;
+};
+
+// The rows and the length of sequence b, kept inside the tensors whatever the device arrays hold.
+__device__ inline void sequence(const AttendArgs &a, int b, int64_t &first, int &n_q, int &n_kv) {
+    int64_t s = a.starts[b], e = a.starts[b + 1];
+    s = s < 0 ? 0 : (s > a.rows ? a.rows : s);
+    e = e < s ? s : (e > a.rows ? a.rows : e);
+    const int64_t most = (int64_t)a.width * a.page;
+    const int n = a.kv_lens[b];
+    first = s;
+    n_q = (int)(e - s);
+    n_kv = n < 0 ? 0 : (n > most ? (int)most : n);
+}
+
+// One wave for each row and head, 64 tokens at a time.
+template <typename T>
+__global__ __launch_bounds__(64) void k_cache_attend(const AttendArgs a) {
+    __shared__ float s_q[256], s_p[64];
+    __shared__ int64_t s_page[64];
+    const int lane = threadIdx.x, parts = a.dim / a.sub;
+    const int head = blockIdx.y, b = blockIdx.z, h = head / (a.q_heads / a.heads);
+    int64_t first;
+    int n_q, n_kv;
+    sequence(a, b, first, n_q, n_kv);
+    const int64_t cb0 = a.cb_heads == 1 ? 0 : (int64_t)h * a.K * a.dim;
+    const T *k_cb = static_cast<const T *>(a.cb[0]) + cb0, *v_cb = static_cast<const T *>(a.cb[1]) + cb0;
+    for (int i = blockIdx.x; i < n_q; i += gridDim.x) {
+        const int64_t row = first + i;
+        const T *q = static_cast<const T *>(a.q) + row * a.q_token_stride + head * a.q_head_stride;
+        __syncthreads();
+        for (int e = lane; e < a.dim; e += 64) s_q[e] = (float)q[e];
+        float top = -INFINITY, total = 0.0f, acc[4] = {0, 0, 0, 0};
+        const int64_t end = (int64_t)n_kv - n_q + i + 1;
+        for (int64_t t0 = 0; t0 < end; t0 += 64) {
+            const int64_t t = t0 + lane;
+            int64_t pg = t < end ? a.table[(int64_t)b * a.width + t / a.page] : -1;
+            if (pg >= a.pages) pg = -1;
+            float s = -INFINITY;
+            __syncthreads();
+            if (pg >= 0) {
+                const uint8_t *kc = a.codes[0] + ((pg * a.heads + h) * a.page + t % a.page) * parts;
+                float sum = 0.0f;
+                for (int m = 0; m < parts; ++m) {
+                    const int code = kc[m] < a.K ? kc[m] : a.K - 1;
+                    for (int e = 0; e < a.sub; ++e) sum += s_q[m * a.sub + e] * (float)k_cb[(int64_t)code * a.dim + m * a.sub + e];
+                }
+                s = sum * a.scale;
+            }
+            float best = s;
+            for (int o = 32; o; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
+            const float now = fmaxf(top, best);
+            const float keep = now == -INFINITY ? 1.0f : expf(top - now);
+            const float p = pg < 0 ? 0.0f : expf(s - now);
+            float sum = p;
+            for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+            total = total * keep + sum;
+            top = now;
+            s_p[lane] = p;
+            s_page[lane] = pg;
+            __syncthreads();
+            for (int u = 0; u < 4; ++u) {
+                const int e = lane + 64 * u;
+                if (e >= a.dim) break;
+                acc[u] *= keep;
+                for (int j = 0; j < 64; ++j) {
+                    if (s_page[j] < 0) continue;
+                    int code = a.codes[1][((s_page[j] * a.heads + h) * parts + e / a.sub) * a.page + (t0 + j) % a.page];
+                    code = code < a.K ? code : a.K - 1;
+                    acc[u] += s_p[j] * (float)v_cb[(int64_t)code * a.dim + e];
+                }
+            }
+        }
+        for (int u = 0; u < 4; ++u) {
+            const int e = lane + 64 * u;
+            if (e < a.dim)
+                static_cast<T *>(a.out)[(row * a.q_heads + head) * a.dim + e] = (T)(total > 0.0f ? acc[u] / total : 0.0f);
+        }
+        if (a.lse && lane == 0) a.lse[row * a.q_heads + head] = total > 0.0f ? top + logf(total) : -INFINITY;
+    }
+}
+
+// One thread for each sub-vector: its codeword (-1 where a number is not finite) and least distance.
+template <typename T>
+__global__ __launch_bounds__(256) void k_lbg_assign(const T *x, int64_t token_stride, int64_t head_stride, int64_t tokens,
+                                                    const float *cb, int heads, int dim, int sub, int K, int16_t *labels,
+                                                    double *least) {
+    const int parts = dim / sub;
+    const int64_t n = tokens * heads * parts;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int m = (int)(i % parts), h = (int)(i / parts % heads);
+        const int64_t t = i / parts / heads;
+        const T *p = x + t * token_stride + h * head_stride + m * sub;
+        bool fine = true;
+        for (int e = 0; e < sub; ++e) fine = fine && fabsf((float)p[e]) < INFINITY;
+        double d = 0.0;
+        const int code = fine ? nearest_f64(p, cb + (int64_t)h * K * dim + m * sub, dim, sub, K, &d) : -1;
+        labels[(int64_t)(h * parts + m) * tokens + t] = (int16_t)code;
+        least[(int64_t)(h * parts + m) * tokens + t] = d;
+    }
+}
+
+// One workgroup for each head and part, a thread for each codeword.
+template <typename T>
+__global__ __launch_bounds__(256) void k_lbg_sum(const T *x, int64_t token_stride, int64_t head_stride, int64_t tokens,
+                                                 int heads, int dim, int sub, int K, const int16_t *labels, const double *least,
+                                                 double *sums, int64_t *counts, double *dist) {
+    __shared__ double s_d[256];
+    const int parts = dim / sub, h = blockIdx.x / parts, m = blockIdx.x % parts, k = threadIdx.x;
+    const int16_t *lab = labels + (int64_t)blockIdx.x * tokens;
+    const double *d = least + (int64_t)blockIdx.x * tokens;
+    double sum[8] = {0, 0, 0, 0, 0, 0, 0, 0}, far = 0.0;
+    int64_t count = 0;
+    for (int64_t t = 0; t < tokens; ++t) {
+        if (lab[t] == k) {
+            const T *p = x + t * token_stride + h * head_stride + m * sub;
+            for (int e = 0; e < sub; ++e) sum[e] += (double)(float)p[e];
+            ++count;
+        }
+        if (t % 256 == k && lab[t] >= 0) far += d[t];
+    }
+    s_d[k] = far;
+    __syncthreads();
+    for (int o = 128; o; o >>= 1) {
+        if (k < o) s_d[k] += s_d[k + o];
+        __syncthreads();
+    }
+    if (k == 0) dist[blockIdx.x] = s_d[0];
+    if (k >= K) return;
+    counts[(int64_t)blockIdx.x * K + k] = count;
+    for (int e = 0; e < sub; ++e) sums[((int64_t)h * K + k) * dim + m * sub + e] = sum[e];
+}
+
+__global__ __launch_bounds__(256) void k_lbg_close(const double *sums, const int64_t *counts, const double *dist, const float *cb_old,
+                                                   int heads, int dim, int sub, int K, float *cb_new, double *mean_dist) {
+    const int parts = dim / sub;
+    const int64_t n = (int64_t)heads * K * dim;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int e = (int)(i % dim), k = (int)(i / dim % K), h = (int)(i / dim / K);
+        const int64_t c = counts[((int64_t)h * parts + e / sub) * K + k];
+        cb_new[i] = c > 0 ? (float)(sums[i] / (double)c) : cb_old[i];
+    }
+    for (int g = blockIdx.x * 256 + threadIdx.x; g < heads * parts; g += gridDim.x * 256) {
+        int64_t c = 0;
+        for (int k = 0; k < K; ++k) c += counts[(int64_t)g * K + k];
+        mean_dist[g] = c > 0 ? dist[g] / (double)c : 0.0;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+int check_shape(int heads, int dim, int sub, int K) {
+    if (heads <= 0) return fail(VQ_E_INVALID, "need heads > 0 (got %d)", heads);
+    if (heads > 1024) return fail(VQ_E_UNSUPPORTED, "heads=%d: at most 1024", heads);
+    if (dim != 32 && dim != 64 && dim != 96 && dim != 128 && dim != 192 && dim != 256)
+        return fail(VQ_E_UNSUPPORTED, "dim=%d: 32, 64, 96, 128, 192 or 256", dim);
+    if (sub != 2 && sub != 4 && sub != 8) return fail(VQ_E_UNSUPPORTED, "sub=%d: 2, 4 or 8", sub);
+    if (K < 1 || K > 256) return fail(VQ_E_UNSUPPORTED, "K=%d: a code is one byte, 1 to 256 codewords", K);
+    return VQ_OK;
+}
+
+int check_cache(const void *k_codes, const void *v_codes, const void *k_cb, const void *v_cb, int cb_heads, int heads,
+                int64_t pages, int page, int dtype) {
+    if (!k_codes || !v_codes || !k_cb || !v_cb) return fail(VQ_E_INVALID, "null pointer");
+    if (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_cb | (uintptr_t)v_cb) & 15)
+        return fail(VQ_E_INVALID, "codes and codebooks must start at multiples of 16 bytes");
+    if (cb_heads != 1 && cb_heads != heads) return fail(VQ_E_INVALID, "cb_heads=%d: 1 or heads (%d)", cb_heads, heads);
+    if (pages <= 0 || pages > 0x7fffffff) return fail(VQ_E_INVALID, "need 0 < pages < 2^31");
+    if (page <= 0 || page > (1 << 20)) return fail(VQ_E_INVALID, "need 0 < page <= 2^20 (got %d)", page);
+    if (page % 16) return fail(VQ_E_UNSUPPORTED, "page=%d: a multiple of 16", page);
+    if (dtype != VQ_BF16 && dtype != VQ_F16) return fail(VQ_E_UNSUPPORTED, "cache vectors are VQ_BF16 or VQ_F16");
+    return VQ_OK;
+}
+
+// Vectors are read 16 bytes at a time: both strides have to keep that alignment.
+int check_vectors(const char *name, const void *p, int64_t token_stride, int64_t head_stride, int64_t size) {
+    if (!p) return fail(VQ_E_INVALID, "null pointer");
+    if (((uintptr_t)p & 15) || (token_stride * size) % 16 || (head_stride * size) % 16)
+        return fail(VQ_E_INVALID, "the vectors of %s must start at multiples of 16 bytes", name);
+    return VQ_OK;
+}
+
+int grid_for(int64_t items, int64_t most) {
+    const int64_t g = (items + 255) / 256;
+    return (int)(g < 1 ? 1 : (g > most ? most : g));
+}
+
+}  // namespace
+
+extern "C" {
+
+int vq_cache_write(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                   int64_t v_head_stride, const int64_t *slots, int64_t tokens, const void *k_cb, const void *v_cb, int cb_heads,
+                   int heads, int dim, int sub, int K, int dtype, uint8_t *k_codes, uint8_t *v_codes, int64_t pages, int page,
+                   void *stream) {
+    int rc = check_shape(heads, dim, sub, K);
+    if (rc) return rc;
+    if ((rc = check_cache(k_codes, v_codes, k_cb, v_cb, cb_heads, heads, pages, page, dtype))) return rc;
+    if (tokens < 0) return fail(VQ_E_INVALID, "need tokens >= 0");
+    if (tokens == 0) return VQ_OK;
+    if (!slots) return fail(VQ_E_INVALID, "null pointer");
+    if ((rc = check_vectors("k", k, k_token_stride, k_head_stride, 2))) return rc;
+    if ((rc = check_vectors("v", v, v_token_stride, v_head_stride, 2))) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    WriteArgs a = {{k, v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, {k_cb, v_cb}, slots, tokens, pages,
+                   cb_heads, heads, dim, sub, K, page, k_codes, v_codes};
+    const dim3 grid(grid_for(tokens * heads * (dim / sub), 1 << 20), 2);
+    if (dtype == VQ_BF16) hipLaunchKernelGGL(k_cache_write<__bf16>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_cache_write<_Float16>, grid, dim3(256), 0, st, a);
+    LAUNCH_CHECK("k_cache_write");
+    return VQ_OK;
+}
+
+int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const void *v_cb, int cb_heads, int heads, int dim,
+                  int sub, int K, int dtype, const uint8_t *k_codes, const uint8_t *v_codes, int64_t pages, int page, void *k_out,
+                  void *v_out, void *stream) {
+    int rc = check_shape(heads, dim, sub, K);
+    if (rc) return rc;
+    if ((rc = check_cache(k_codes, v_codes, k_cb, v_cb, cb_heads, heads, pages, page, dtype))) return rc;
+    if (tokens < 0) return fail(VQ_E_INVALID, "need tokens >= 0");
+    if (tokens == 0) return VQ_OK;
+    if (!slots) return fail(VQ_E_INVALID, "null pointer");
+    if ((rc = check_vectors("k_out", k_out, dim, dim, 2))) return rc;
+    if ((rc = check_vectors("v_out", v_out, dim, dim, 2))) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    ReadArgs a = {slots, tokens, pages, {k_cb, v_cb}, cb_heads, heads, dim, sub, K, page, {k_codes, v_codes}, {k_out, v_out}};
+    const dim3 grid(grid_for(tokens * heads * (dim / sub), 1 << 20), 2);
+    if (dtype == VQ_BF16) hipLaunchKernelGGL(k_cache_read<__bf16>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_cache_read<_Float16>, grid, dim3(256), 0, st, a);
+    LAUNCH_CHECK("k_cache_read");
+    return VQ_OK;
+}
+
+size_t vq_cache_attention_ws_bytes(int64_t rows, int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q,
+                                   int64_t max_kv) {
+    (void)rows, (void)q_heads, (void)heads, (void)dim, (void)sub, (void)K, (void)seqs, (void)max_q, (void)max_kv;
+    return 0;
+}
+
+int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t rows, int q_heads, const void *k_cb,
+                       const void *v_cb, int cb_heads, int heads, int dim, int sub, int K, int dtype, const uint8_t *k_codes,
+                       const uint8_t *v_codes, int64_t pages, int page, const int32_t *table, int seqs, int width,
+                       const int32_t *kv_lens, const int32_t *starts, int64_t max_q, int64_t max_kv, double scale, void *out,
+                       float *lse, void *ws, size_t ws_bytes, void *stream) {
+    int rc = check_shape(heads, dim, sub, K);
+    if (rc) return rc;
+    if ((rc = check_cache(k_codes, v_codes, k_cb, v_cb, cb_heads, heads, pages, page, dtype))) return rc;
+    if (q_heads <= 0 || q_heads % heads) return fail(VQ_E_INVALID, "q_heads=%d: a positive multiple of heads (%d)", q_heads, heads);
+    if (q_heads > 4096) return fail(VQ_E_UNSUPPORTED, "q_heads=%d: at most 4096", q_heads);
+    if (rows < 0 || seqs < 0 || width < 0) return fail(VQ_E_INVALID, "need rows, seqs and width >= 0");
+    if (rows > 0x7fffffff || (int64_t)width * page > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "rows and width * page below 2^31");
+    if (max_q < 1 || max_kv < 1) return fail(VQ_E_INVALID, "need max_q and max_kv >= 1");
+    if (!(scale > -INFINITY && scale < INFINITY)) return fail(VQ_E_INVALID, "scale must be finite");
+    if (rows == 0 || seqs == 0) return VQ_OK;
+    if (seqs > 65535) return fail(VQ_E_UNSUPPORTED, "seqs=%d: at most 65535", seqs);
+    if ((!table && width > 0) || !kv_lens || !starts) return fail(VQ_E_INVALID, "null pointer");
+    if ((rc = check_vectors("q", q, q_token_stride, q_head_stride, 2))) return rc;
+    if ((rc = check_vectors("out", out, dim, dim, 2))) return rc;
+    const size_t need = vq_cache_attention_ws_bytes(rows, q_heads, heads, dim, sub, K, seqs, max_q, max_kv);
+    if (need > 0 && (!ws || ws_bytes < need)) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, need);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    AttendArgs a = {q, q_token_stride, q_head_stride, rows, q_heads, {k_cb, v_cb}, cb_heads, heads, dim, sub, K,
+                    {k_codes, v_codes}, pages, page, table, seqs, width, kv_lens, starts, (float)scale, out, lse};
+    const dim3 grid((unsigned)(max_q > 65535 ? 65535 : max_q), q_heads, seqs);
+    if (dtype == VQ_BF16) hipLaunchKernelGGL(k_cache_attend<__bf16>, grid, dim3(64), 0, st, a);
+    else hipLaunchKernelGGL(k_cache_attend<_Float16>, grid, dim3(64), 0, st, a);
+    LAUNCH_CHECK("k_cache_attend");
+    return VQ_OK;
+}
+
+size_t vq_cache_lbg_ws_bytes(int64_t tokens, int heads, int dim, int sub, int K) {
+    if (tokens <= 0 || heads <= 0 || sub <= 0 || dim <= 0 || K <= 0) return 0;
+    return (size_t)tokens * heads * (dim / sub) * 10;
+}
+
+int vq_cache_lbg_accum(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens, const float *cb, int heads, int dim,
+                       int sub, int K, int dtype, double *sums, int64_t *counts, double *dist, void *ws, size_t ws_bytes,
+                       void *stream) {
+    int rc = check_shape(heads, dim, sub, K);
+    if (rc) return rc;
+    if (dtype != VQ_F32 && dtype != VQ_BF16 && dtype != VQ_F16) return fail(VQ_E_UNSUPPORTED, "dtype=%d", dtype);
+    if (tokens < 1) return fail(VQ_E_INVALID, "need tokens >= 1");
+    if (tokens > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "tokens below 2^31");
+    if (!cb || !sums || !counts || !dist) return fail(VQ_E_INVALID, "null pointer");
+    if ((uintptr_t)cb & 15) return fail(VQ_E_INVALID, "the codebook must start at a multiple of 16 bytes");
+    if ((rc = check_vectors("x", x, token_stride, head_stride, dtype == VQ_F32 ? 4 : 2))) return rc;
+    const size_t need = vq_cache_lbg_ws_bytes(tokens, heads, dim, sub, K);
+    if (!ws || ws_bytes < need) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, need);
+    if ((uintptr_t)ws & 15) return fail(VQ_E_INVALID, "the workspace must start at a multiple of 16 bytes");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int64_t n = tokens * heads * (dim / sub);
+    double *least = static_cast<double *>(ws);
+    int16_t *labels = reinterpret_cast<int16_t *>(least + n);
+    const dim3 grid(grid_for(n, 1 << 20));
+#define VQ_LBG(T)                                                                                                          \
+    do {                                                                                                                   \
+        const T *p = static_cast<const T *>(x);                                                                            \
+        hipLaunchKernelGGL(k_lbg_assign<T>, grid, dim3(256), 0, st, p, token_stride, head_stride, tokens, cb, heads, dim,  \
+                           sub, K, labels, least);                                                                         \
+        LAUNCH_CHECK("k_lbg_assign");                                                                                      \
+        hipLaunchKernelGGL(k_lbg_sum<T>, dim3(heads * (dim / sub)), dim3(256), 0, st, p, token_stride, head_stride, tokens, \
+                           heads, dim, sub, K, labels, least, sums, counts, dist);                                         \
+        LAUNCH_CHECK("k_lbg_sum");                                                                                         \
+    } while (0)
+    if (dtype == VQ_F32) VQ_LBG(float);
+    else if (dtype == VQ_BF16) VQ_LBG(__bf16);
+    else VQ_LBG(_Float16);
+#undef VQ_LBG
+    return VQ_OK;
+}
+
+int vq_cache_lbg_finish(const double *sums, const int64_t *counts, const double *dist, const float *cb_old, int heads, int dim,
+                        int sub, int K, float *cb_new, double *mean_dist, void *stream) {
+    int rc = check_shape(heads, dim, sub, K);
+    if (rc) return rc;
+    if (!sums || !counts || !dist || !cb_old || !cb_new || !mean_dist) return fail(VQ_E_INVALID, "null pointer");
+    hipLaunchKernelGGL(k_lbg_close, dim3(grid_for((int64_t)heads * K * dim, 4096)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       sums, counts, dist, cb_old, heads, dim, sub, K, cb_new, mean_dist);
+    LAUNCH_CHECK("k_lbg_close");
+    return VQ_OK;
+}
+
+}  // extern "C"

@@ -10,6 +10,7 @@ import torch
 
 from . import _lib
 from ._lib import lib, check, VQ_MODE_EXACT, VQ_MODE_FAST, VQ_PAD_EDGE, VQ_PAD_ZERO  # noqa: F401
+from .cache import CacheOps
 
 
 def _ptr(t):
@@ -20,9 +21,10 @@ def _nbytes(t):
     return t.numel() * t.element_size() if t is not None else 0
 
 
-class HipEngine:
+class HipEngine(CacheOps):
     """Launches the HIP kernels on one device.  Not thread-safe per instance (it caches its
-    workspace); use one engine per host thread, or one per GPU in a multi-process job."""
+    workspace); use one engine per host thread, or one per GPU in a multi-process job.
+    The cache_* methods (vector-quantised key-value cache) come from CacheOps."""
 
     def __init__(self, device=None, mode="fast"):
         if not torch.cuda.is_available():
