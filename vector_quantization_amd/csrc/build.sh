@@ -10,8 +10,14 @@ FLAGS=(-O3 -std=c++17 --offload-arch=gfx950 -fPIC -ffp-contract=off -Xclang -tar
 # objects of this run only, so that two builds at once do not mix
 OBJ="$(mktemp -d)"
 trap 'rm -rf "$OBJ"' EXIT
-/opt/rocm/bin/hipcc "${FLAGS[@]}" -c "$HERE/vq_hip.hip" -o "$OBJ/vq_hip.o" &
-FIRST=$!
-/opt/rocm/bin/hipcc "${FLAGS[@]}" -c "$HERE/vq_cache.hip" -o "$OBJ/vq_cache.o"
-wait $FIRST
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC "$OBJ/vq_hip.o" "$OBJ/vq_cache.o" -o "$LIB/libvqhip.so"
+PIDS=()
+compile() {  # source, object, further flags
+    /opt/rocm/bin/hipcc "${FLAGS[@]}" "${@:3}" -c "$HERE/$1" -o "$OBJ/$2" &
+    PIDS+=($!)
+}
+compile vq_hip.hip vq_hip.o
+compile vq_cache.hip vq_cache.o
+compile vq_cache_attend.hip vq_cache_attend_bf16.o -DVQ_CACHE_TYPE=__bf16 -DVQ_CACHE_ATTEND=vq_internal_attend_bf16
+compile vq_cache_attend.hip vq_cache_attend_f16.o -DVQ_CACHE_TYPE=_Float16 -DVQ_CACHE_ATTEND=vq_internal_attend_f16
+for pid in "${PIDS[@]}"; do wait "$pid"; done
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC "$OBJ"/*.o -o "$LIB/libvqhip.so"

@@ -1,15 +1,13 @@
 // vq_cache.hip -- HIP kernels (gfx950 / CDNA4) and C ABI of the vector-quantised key-value cache (vq_cache.h).
-#include <hip/hip_runtime.h>
-#include <math.h>
 #include <stdarg.h>
-#include <stdint.h>
 #include <stdio.h>
 
-#include "vq_cache.h"
-#include "vq_hip.h"
+#include "vq_cache_internal.h"
 
-__attribute__((visibility("hidden"))) int vq_internal_fail(int code, const char *message);
-__attribute__((visibility("hidden"))) int vq_internal_device(int *cus);
+#ifndef VQ_RB
+#define VQ_RB 4
+#define VQ_NW 4
+#endif
 
 namespace {
 
@@ -110,102 +108,6 @@ __global__ __launch_bounds__(256) void k_cache_read(const ReadArgs a) {
         const T *cb = static_cast<const T *>(a.cb[which]) + ((a.cb_heads == 1 ? 0 : (int64_t)h * a.K) + code) * a.dim + m * a.sub;
         T *out = static_cast<T *>(a.out[which]) + i * a.sub;
         for (int e = 0; e < a.sub; ++e) out[e] = there ? cb[e] : (T)0.0f;
-    }
-}
-
-struct AttendArgs {
-    const void *q;
-    int64_t q_token_stride, q_head_stride, rows;
-    int q_heads;
-    const void *cb[2];
-    int cb_heads, heads, dim, sub, K;
-    const uint8_t *codes[2];
-    int64_t pages;
-    int page;
-    const int32_t *table;
-    int seqs, width;
-    const int32_t *kv_lens, *starts;
-    float scale;
-    void *out;
-    float *lse;
-};
-
-// The rows and the length of sequence b, kept inside the tensors whatever the device arrays hold.
-__device__ inline void sequence(const AttendArgs &a, int b, int64_t &first, int &n_q, int &n_kv) {
-    int64_t s = a.starts[b], e = a.starts[b + 1];
-    s = s < 0 ? 0 : (s > a.rows ? a.rows : s);
-    e = e < s ? s : (e > a.rows ? a.rows : e);
-    const int64_t most = (int64_t)a.width * a.page;
-    const int n = a.kv_lens[b];
-    first = s;
-    n_q = (int)(e - s);
-    n_kv = n < 0 ? 0 : (n > most ? (int)most : n);
-}
-
-// One wave for each row and head, 64 tokens at a time.
-template <typename T>
-__global__ __launch_bounds__(64) void k_cache_attend(const AttendArgs a) {
-    __shared__ float s_q[256], s_p[64];
-    __shared__ int64_t s_page[64];
-    const int lane = threadIdx.x, parts = a.dim / a.sub;
-    const int head = blockIdx.y, b = blockIdx.z, h = head / (a.q_heads / a.heads);
-    int64_t first;
-    int n_q, n_kv;
-    sequence(a, b, first, n_q, n_kv);
-    const int64_t cb0 = a.cb_heads == 1 ? 0 : (int64_t)h * a.K * a.dim;
-    const T *k_cb = static_cast<const T *>(a.cb[0]) + cb0, *v_cb = static_cast<const T *>(a.cb[1]) + cb0;
-    for (int i = blockIdx.x; i < n_q; i += gridDim.x) {
-        const int64_t row = first + i;
-        const T *q = static_cast<const T *>(a.q) + row * a.q_token_stride + head * a.q_head_stride;
-        __syncthreads();
-        for (int e = lane; e < a.dim; e += 64) s_q[e] = (float)q[e];
-        float top = -INFINITY, total = 0.0f, acc[4] = {0, 0, 0, 0};
-        const int64_t end = (int64_t)n_kv - n_q + i + 1;
-        for (int64_t t0 = 0; t0 < end; t0 += 64) {
-            const int64_t t = t0 + lane;
-            int64_t pg = t < end ? a.table[(int64_t)b * a.width + t / a.page] : -1;
-            if (pg >= a.pages) pg = -1;
-            float s = -INFINITY;
-            __syncthreads();
-            if (pg >= 0) {
-                const uint8_t *kc = a.codes[0] + ((pg * a.heads + h) * a.page + t % a.page) * parts;
-                float sum = 0.0f;
-                for (int m = 0; m < parts; ++m) {
-                    const int code = kc[m] < a.K ? kc[m] : a.K - 1;
-                    for (int e = 0; e < a.sub; ++e) sum += s_q[m * a.sub + e] * (float)k_cb[(int64_t)code * a.dim + m * a.sub + e];
-                }
-                s = sum * a.scale;
-            }
-            float best = s;
-            for (int o = 32; o; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
-            const float now = fmaxf(top, best);
-            const float keep = now == -INFINITY ? 1.0f : expf(top - now);
-            const float p = pg < 0 ? 0.0f : expf(s - now);
-            float sum = p;
-            for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-            total = total * keep + sum;
-            top = now;
-            s_p[lane] = p;
-            s_page[lane] = pg;
-            __syncthreads();
-            for (int u = 0; u < 4; ++u) {
-                const int e = lane + 64 * u;
-                if (e >= a.dim) break;
-                acc[u] *= keep;
-                for (int j = 0; j < 64; ++j) {
-                    if (s_page[j] < 0) continue;
-                    int code = a.codes[1][((s_page[j] * a.heads + h) * parts + e / a.sub) * a.page + (t0 + j) % a.page];
-                    code = code < a.K ? code : a.K - 1;
-                    acc[u] += s_p[j] * (float)v_cb[(int64_t)code * a.dim + e];
-                }
-            }
-        }
-        for (int u = 0; u < 4; ++u) {
-            const int e = lane + 64 * u;
-            if (e < a.dim)
-                static_cast<T *>(a.out)[(row * a.q_heads + head) * a.dim + e] = (T)(total > 0.0f ? acc[u] / total : 0.0f);
-        }
-        if (a.lse && lane == 0) a.lse[row * a.q_heads + head] = total > 0.0f ? top + logf(total) : -INFINITY;
     }
 }
 
@@ -315,6 +217,38 @@ int grid_for(int64_t items, int64_t most) {
     return (int)(g < 1 ? 1 : (g > most ? most : g));
 }
 
+int64_t clamp_hint(int64_t n) { return n > 0x7fffffff ? 0x7fffffff : n; }
+
+// How many rows a workgroup takes, and into how many pieces the context is cut.  Host arithmetic on sizes alone.
+struct Attention {
+    AttendPlan p;
+    int64_t row_tiles;
+    int splits, split_tiles;
+    size_t ws;
+};
+
+Attention plan_attention(int64_t rows, int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q, int64_t max_kv) {
+    constexpr int CUS = 256;
+    Attention r;
+    const int Kp = rows_padded(K), group = q_heads / heads;
+    const int64_t per_seq = max_q * group;
+    r.p.rb = per_seq <= 16 ? 1 : dim >= 192 ? 2 : VQ_RB;
+    r.p.nw = r.p.rb == 1 ? 8 : dim >= 192 ? 4 : VQ_NW;
+    r.p.values_in_lds = values_in_lds(Kp, dim, sub);
+    const size_t tables = key_bytes(Kp, dim, sub) + (r.p.values_in_lds ? (size_t)Kp * dim * 2 : 0), join = join_bytes(r.p.nw, r.p.rb, dim);
+    r.p.lds = tables > join ? tables : join;
+    r.row_tiles = (per_seq + r.p.rb * 16 - 1) / (r.p.rb * 16);
+    const int64_t base = r.row_tiles * heads * seqs, tiles = (max_kv + TILE - 1) / TILE;
+    int64_t splits = (2 * CUS + base - 1) / base;
+    const int64_t most = (tiles + 2 * r.p.nw - 1) / (2 * r.p.nw);
+    splits = splits < most ? splits : most;
+    splits = splits < 1 ? 1 : splits > 256 ? 256 : splits;
+    r.split_tiles = (int)((tiles + splits - 1) / splits);
+    r.splits = (int)((tiles + r.split_tiles - 1) / r.split_tiles);
+    r.ws = r.splits > 1 ? (size_t)r.splits * rows * q_heads * (dim * 4 + 8) : 0;
+    return r;
+}
+
 }  // namespace
 
 extern "C" {
@@ -363,8 +297,10 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
 
 size_t vq_cache_attention_ws_bytes(int64_t rows, int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q,
                                    int64_t max_kv) {
-    (void)rows, (void)q_heads, (void)heads, (void)dim, (void)sub, (void)K, (void)seqs, (void)max_q, (void)max_kv;
-    return 0;
+    if (rows <= 0 || q_heads <= 0 || q_heads > 4096 || seqs <= 0 || max_q < 1 || max_kv < 1 || check_shape(heads, dim, sub, K) ||
+        q_heads % heads || rows > 0x7fffffff)
+        return 0;
+    return plan_attention(rows, q_heads, heads, dim, sub, K, seqs, clamp_hint(max_q), clamp_hint(max_kv)).ws;
 }
 
 int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t rows, int q_heads, const void *k_cb,
@@ -380,21 +316,26 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
     if (rows < 0 || seqs < 0 || width < 0) return fail(VQ_E_INVALID, "need rows, seqs and width >= 0");
     if (rows > 0x7fffffff || (int64_t)width * page > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "rows and width * page below 2^31");
     if (max_q < 1 || max_kv < 1) return fail(VQ_E_INVALID, "need max_q and max_kv >= 1");
-    if (!(scale > -INFINITY && scale < INFINITY)) return fail(VQ_E_INVALID, "scale must be finite");
+    if (!(fabs(scale) < 1e38)) return fail(VQ_E_INVALID, "scale must be finite and below 1e38 in size");
     if (rows == 0 || seqs == 0) return VQ_OK;
     if (seqs > 65535) return fail(VQ_E_UNSUPPORTED, "seqs=%d: at most 65535", seqs);
     if ((!table && width > 0) || !kv_lens || !starts) return fail(VQ_E_INVALID, "null pointer");
     if ((rc = check_vectors("q", q, q_token_stride, q_head_stride, 2))) return rc;
     if ((rc = check_vectors("out", out, dim, dim, 2))) return rc;
-    const size_t need = vq_cache_attention_ws_bytes(rows, q_heads, heads, dim, sub, K, seqs, max_q, max_kv);
-    if (need > 0 && (!ws || ws_bytes < need)) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, need);
+    max_q = clamp_hint(max_q);
+    max_kv = clamp_hint(max_kv);
+    const Attention r = plan_attention(rows, q_heads, heads, dim, sub, K, seqs, max_q, max_kv);
+    if (r.ws > 0 && (!ws || ws_bytes < r.ws)) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, r.ws);
+    if (r.ws > 0 && ((uintptr_t)ws & 15)) return fail(VQ_E_INVALID, "the workspace must start at a multiple of 16 bytes");
+    float *part_o = static_cast<float *>(ws);
+    AttendArgs a = {q, q_token_stride, q_head_stride, rows, q_heads, {k_cb, v_cb}, cb_heads, heads, K, rows_padded(K), {k_codes, v_codes}, pages,
+                    page, table, seqs, width, kv_lens, starts, (float)(scale * 1.4426950408889634), out, lse, r.splits, r.split_tiles, part_o,
+                    reinterpret_cast<float2 *>(part_o + (int64_t)r.splits * rows * q_heads * dim)};
+    const int64_t items = r.row_tiles * r.splits;
+    const dim3 grid(heads, (unsigned)(items > 65535 ? 65535 : items), seqs);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    AttendArgs a = {q, q_token_stride, q_head_stride, rows, q_heads, {k_cb, v_cb}, cb_heads, heads, dim, sub, K,
-                    {k_codes, v_codes}, pages, page, table, seqs, width, kv_lens, starts, (float)scale, out, lse};
-    const dim3 grid((unsigned)(max_q > 65535 ? 65535 : max_q), q_heads, seqs);
-    if (dtype == VQ_BF16) hipLaunchKernelGGL(k_cache_attend<__bf16>, grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL(k_cache_attend<_Float16>, grid, dim3(64), 0, st, a);
-    LAUNCH_CHECK("k_cache_attend");
+    const hipError_t e = (dtype == VQ_BF16 ? vq_internal_attend_bf16 : vq_internal_attend_f16)(a, r.p, dim, sub, grid, st);
+    if (e != hipSuccess) return fail(VQ_E_HIP, "launch of k_cache_attend failed: %s", hipGetErrorString(e));
     return VQ_OK;
 }
 

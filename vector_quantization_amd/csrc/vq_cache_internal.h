@@ -1,0 +1,77 @@
+// vq_cache_internal.h -- what the source files of the vector-quantised cache share.
+#ifndef VQ_CACHE_INTERNAL_H
+#define VQ_CACHE_INTERNAL_H
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "vq_cache.h"
+#include "vq_hip.h"
+
+#define VQ_HIDDEN __attribute__((visibility("hidden")))
+
+VQ_HIDDEN int vq_internal_fail(int code, const char *message);
+VQ_HIDDEN int vq_internal_device(int *cus);
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
+struct AttendArgs {
+    const void *q;
+    int64_t q_token_stride, q_head_stride, rows;
+    int q_heads;
+    const void *cb[2];
+    int cb_heads, heads, K, Kp;
+    const uint8_t *codes[2];
+    int64_t pages;
+    int page;
+    const int32_t *table;
+    int seqs, width;
+    const int32_t *kv_lens, *starts;
+    float scale2;                      // scale * log2(e)
+    void *out;
+    float *lse;
+    int splits, split_tiles;           // the context is cut into pieces of split_tiles tiles; the last takes what is left
+    float *part_o;                     // (splits, rows * q_heads, D), against part_ml's maximum
+    float2 *part_ml;                   // (splits, rows * q_heads): maximum (base 2) and sum
+};
+
+// How an attention call is laid out: RB * 16 rows to a workgroup of NW waves.
+struct AttendPlan {
+    int rb, nw;
+    bool values_in_lds;
+    size_t lds;
+};
+
+// Launches k_cache_attend and, for several splits, the kernel that joins them; one for each element type.
+VQ_HIDDEN hipError_t vq_internal_attend_bf16(const AttendArgs &a, const AttendPlan &p, int dim, int sub, dim3 grid, hipStream_t stream);
+VQ_HIDDEN hipError_t vq_internal_attend_f16(const AttendArgs &a, const AttendPlan &p, int dim, int sub, dim3 grid, hipStream_t stream);
+
+constexpr int LDS_MOST = 160 * 1024;
+constexpr int TILE = 32;              // tokens a wave takes at a time: two groups of 16, each inside one page
+
+constexpr int value_chunk(int D, int SUB) {
+    int e = SUB;
+    while (D % (16 * e)) e /= 2;
+    return e;
+}
+// Key table: part m starts at m * key_stride bytes; the pad keeps the writes of a codebook row's parts in different banks.
+__host__ __device__ inline int rows_padded(int K) {
+    int p = 1;
+    while (p < K) p *= 2;
+    return p;
+}
+__host__ __device__ inline int key_stride(int Kp, int SUB) { return (Kp + 1) * SUB * 2; }
+inline size_t key_bytes(int Kp, int D, int SUB) { return ((size_t)(D / SUB) * key_stride(Kp, SUB) + 15) / 16 * 16; }
+inline size_t join_bytes(int NW, int RB, int D) { return (size_t)NW * RB * 16 * (D + 4) * 4 + (size_t)NW * RB * 16 * 8; }
+inline bool values_in_lds(int Kp, int D, int SUB) { return key_bytes(Kp, D, SUB) + (size_t)Kp * D * 2 <= LDS_MOST; }
+
+
+#endif
