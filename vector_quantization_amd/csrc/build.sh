@@ -17,6 +17,7 @@ compile() {  # source, object, further flags
 }
 compile vq_hip.hip vq_hip.o
 compile vq_cache.hip vq_cache.o
+compile vq_cache_search.hip vq_cache_search.o
 compile vq_cache_attend.hip vq_cache_attend_bf16.o -DVQ_CACHE_TYPE=__bf16 -DVQ_CACHE_ATTEND=vq_internal_attend_bf16
 compile vq_cache_attend.hip vq_cache_attend_f16.o -DVQ_CACHE_TYPE=_Float16 -DVQ_CACHE_ATTEND=vq_internal_attend_f16
 for pid in "${PIDS[@]}"; do wait "$pid"; done

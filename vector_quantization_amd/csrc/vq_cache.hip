@@ -30,59 +30,11 @@ int fail(int code, const char *fmt, ...) {
 // kernels
 // ------------------------------------------------------------------------------------------------
 
-// Number of the codeword nearest to the sub-vector x, by the definition: squared distance summed left to right in
-// fp64, strictly less wins.  cb points at codeword 0's sub-vector, codewords are `row` elements apart.
-template <typename T, typename C>
-__device__ int nearest_f64(const T *x, const C *cb, int row, int sub, int K, double *least) {
-    double best = INFINITY;
-    int code = 0;
-    for (int k = 0; k < K; ++k) {
-        double d = 0.0;
-        for (int e = 0; e < sub; ++e) {
-            const double t = (double)(float)x[e] - (double)(float)cb[(int64_t)k * row + e];
-            d += t * t;
-        }
-        if (d < best) {
-            best = d;
-            code = k;
-        }
-    }
-    *least = best;
-    return code;
-}
-
-struct WriteArgs {
-    const void *x[2];
-    int64_t token_stride[2], head_stride[2];
-    const void *cb[2];
-    const int64_t *slots;
-    int64_t tokens, pages;
-    int cb_heads, heads, dim, sub, K, page;
-    uint8_t *k_codes, *v_codes;
-};
-
 // Where the code of one sub-vector lies.
 __device__ inline int64_t code_at(int which, int64_t slot, int h, int m, int heads, int parts, int page) {
     const int64_t p = slot / page;
     const int o = (int)(slot % page);
     return which == 0 ? ((p * heads + h) * page + o) * parts + m : ((p * heads + h) * parts + m) * page + o;
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_cache_write(const WriteArgs a) {
-    const int parts = a.dim / a.sub;
-    const int64_t n = a.tokens * a.heads * parts;
-    const int which = blockIdx.y;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int m = (int)(i % parts), h = (int)(i / parts % a.heads);
-        const int64_t t = i / parts / a.heads, slot = a.slots[t];
-        if (slot < 0 || slot >= a.pages * a.page) continue;
-        const T *x = static_cast<const T *>(a.x[which]) + t * a.token_stride[which] + h * a.head_stride[which] + m * a.sub;
-        const T *cb = static_cast<const T *>(a.cb[which]) + (a.cb_heads == 1 ? 0 : (int64_t)h * a.K * a.dim) + m * a.sub;
-        double least;
-        const int code = nearest_f64(x, cb, a.dim, a.sub, a.K, &least);
-        (which == 0 ? a.k_codes : a.v_codes)[code_at(which, slot, h, m, a.heads, parts, a.page)] = (uint8_t)code;
-    }
 }
 
 struct ReadArgs {
@@ -109,57 +61,6 @@ __global__ __launch_bounds__(256) void k_cache_read(const ReadArgs a) {
         T *out = static_cast<T *>(a.out[which]) + i * a.sub;
         for (int e = 0; e < a.sub; ++e) out[e] = there ? cb[e] : (T)0.0f;
     }
-}
-
-// One thread for each sub-vector: its codeword (-1 where a number is not finite) and least distance.
-template <typename T>
-__global__ __launch_bounds__(256) void k_lbg_assign(const T *x, int64_t token_stride, int64_t head_stride, int64_t tokens,
-                                                    const float *cb, int heads, int dim, int sub, int K, int16_t *labels,
-                                                    double *least) {
-    const int parts = dim / sub;
-    const int64_t n = tokens * heads * parts;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int m = (int)(i % parts), h = (int)(i / parts % heads);
-        const int64_t t = i / parts / heads;
-        const T *p = x + t * token_stride + h * head_stride + m * sub;
-        bool fine = true;
-        for (int e = 0; e < sub; ++e) fine = fine && fabsf((float)p[e]) < INFINITY;
-        double d = 0.0;
-        const int code = fine ? nearest_f64(p, cb + (int64_t)h * K * dim + m * sub, dim, sub, K, &d) : -1;
-        labels[(int64_t)(h * parts + m) * tokens + t] = (int16_t)code;
-        least[(int64_t)(h * parts + m) * tokens + t] = d;
-    }
-}
-
-// One workgroup for each head and part, a thread for each codeword.
-template <typename T>
-__global__ __launch_bounds__(256) void k_lbg_sum(const T *x, int64_t token_stride, int64_t head_stride, int64_t tokens,
-                                                 int heads, int dim, int sub, int K, const int16_t *labels, const double *least,
-                                                 double *sums, int64_t *counts, double *dist) {
-    __shared__ double s_d[256];
-    const int parts = dim / sub, h = blockIdx.x / parts, m = blockIdx.x % parts, k = threadIdx.x;
-    const int16_t *lab = labels + (int64_t)blockIdx.x * tokens;
-    const double *d = least + (int64_t)blockIdx.x * tokens;
-    double sum[8] = {0, 0, 0, 0, 0, 0, 0, 0}, far = 0.0;
-    int64_t count = 0;
-    for (int64_t t = 0; t < tokens; ++t) {
-        if (lab[t] == k) {
-            const T *p = x + t * token_stride + h * head_stride + m * sub;
-            for (int e = 0; e < sub; ++e) sum[e] += (double)(float)p[e];
-            ++count;
-        }
-        if (t % 256 == k && lab[t] >= 0) far += d[t];
-    }
-    s_d[k] = far;
-    __syncthreads();
-    for (int o = 128; o; o >>= 1) {
-        if (k < o) s_d[k] += s_d[k + o];
-        __syncthreads();
-    }
-    if (k == 0) dist[blockIdx.x] = s_d[0];
-    if (k >= K) return;
-    counts[(int64_t)blockIdx.x * K + k] = count;
-    for (int e = 0; e < sub; ++e) sums[((int64_t)h * K + k) * dim + m * sub + e] = sum[e];
 }
 
 __global__ __launch_bounds__(256) void k_lbg_close(const double *sums, const int64_t *counts, const double *dist, const float *cb_old,
@@ -261,17 +162,17 @@ int vq_cache_write(const void *k, int64_t k_token_stride, int64_t k_head_stride,
     if (rc) return rc;
     if ((rc = check_cache(k_codes, v_codes, k_cb, v_cb, cb_heads, heads, pages, page, dtype))) return rc;
     if (tokens < 0) return fail(VQ_E_INVALID, "need tokens >= 0");
+    if (tokens > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "tokens below 2^31");
     if (tokens == 0) return VQ_OK;
     if (!slots) return fail(VQ_E_INVALID, "null pointer");
     if ((rc = check_vectors("k", k, k_token_stride, k_head_stride, 2))) return rc;
     if ((rc = check_vectors("v", v, v_token_stride, v_head_stride, 2))) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    WriteArgs a = {{k, v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, {k_cb, v_cb}, slots, tokens, pages,
-                   cb_heads, heads, dim, sub, K, page, k_codes, v_codes};
-    const dim3 grid(grid_for(tokens * heads * (dim / sub), 1 << 20), 2);
-    if (dtype == VQ_BF16) hipLaunchKernelGGL(k_cache_write<__bf16>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_cache_write<_Float16>, grid, dim3(256), 0, st, a);
-    LAUNCH_CHECK("k_cache_write");
+    const SearchPlan p = vq_internal_search_plan(tokens, heads, dim, sub, 2);
+    const SearchArgs a = {{k, v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, {k_cb, v_cb}, tokens, cb_heads, heads, dim, K,
+                          p.pw, p.chunk, slots, pages, page, page & (page - 1) ? -1 : __builtin_ctz(page), k_codes, v_codes, nullptr, nullptr};
+    const hipError_t e = vq_internal_search(a, sub, dtype, false, p.blocks, st);
+    if (e != hipSuccess) return fail(VQ_E_HIP, "launch of k_cache_search failed: %s", hipGetErrorString(e));
     return VQ_OK;
 }
 
@@ -282,6 +183,7 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
     if (rc) return rc;
     if ((rc = check_cache(k_codes, v_codes, k_cb, v_cb, cb_heads, heads, pages, page, dtype))) return rc;
     if (tokens < 0) return fail(VQ_E_INVALID, "need tokens >= 0");
+    if (tokens > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "tokens below 2^31");
     if (tokens == 0) return VQ_OK;
     if (!slots) return fail(VQ_E_INVALID, "null pointer");
     if ((rc = check_vectors("k_out", k_out, dim, dim, 2))) return rc;
@@ -340,8 +242,9 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
 }
 
 size_t vq_cache_lbg_ws_bytes(int64_t tokens, int heads, int dim, int sub, int K) {
-    if (tokens <= 0 || heads <= 0 || sub <= 0 || dim <= 0 || K <= 0) return 0;
-    return (size_t)tokens * heads * (dim / sub) * 10;
+    if (tokens <= 0 || tokens > 0x7fffffff || check_shape(heads, dim, sub, K)) return 0;
+    const SearchPlan p = vq_internal_search_plan(tokens, heads, dim, sub, 1);
+    return (size_t)p.chunks * heads * (dim / sub) * ((sub + 1) * 256 * 4 + 8);
 }
 
 int vq_cache_lbg_accum(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens, const float *cb, int heads, int dim,
@@ -359,24 +262,14 @@ int vq_cache_lbg_accum(const void *x, int64_t token_stride, int64_t head_stride,
     if (!ws || ws_bytes < need) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, need);
     if ((uintptr_t)ws & 15) return fail(VQ_E_INVALID, "the workspace must start at a multiple of 16 bytes");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int64_t n = tokens * heads * (dim / sub);
-    double *least = static_cast<double *>(ws);
-    int16_t *labels = reinterpret_cast<int16_t *>(least + n);
-    const dim3 grid(grid_for(n, 1 << 20));
-#define VQ_LBG(T)                                                                                                          \
-    do {                                                                                                                   \
-        const T *p = static_cast<const T *>(x);                                                                            \
-        hipLaunchKernelGGL(k_lbg_assign<T>, grid, dim3(256), 0, st, p, token_stride, head_stride, tokens, cb, heads, dim,  \
-                           sub, K, labels, least);                                                                         \
-        LAUNCH_CHECK("k_lbg_assign");                                                                                      \
-        hipLaunchKernelGGL(k_lbg_sum<T>, dim3(heads * (dim / sub)), dim3(256), 0, st, p, token_stride, head_stride, tokens, \
-                           heads, dim, sub, K, labels, least, sums, counts, dist);                                         \
-        LAUNCH_CHECK("k_lbg_sum");                                                                                         \
-    } while (0)
-    if (dtype == VQ_F32) VQ_LBG(float);
-    else if (dtype == VQ_BF16) VQ_LBG(__bf16);
-    else VQ_LBG(_Float16);
-#undef VQ_LBG
+    const SearchPlan p = vq_internal_search_plan(tokens, heads, dim, sub, 1);
+    double *part_dist = static_cast<double *>(ws);
+    float *part_sums = reinterpret_cast<float *>(part_dist + (int64_t)p.chunks * heads * (dim / sub));
+    const SearchArgs a = {{x, x}, {token_stride, token_stride}, {head_stride, head_stride}, {cb, cb}, tokens, heads, heads, dim, K, p.pw, p.chunk,
+                          nullptr, 0, 0, 0, nullptr, nullptr, part_sums, part_dist};
+    hipError_t e = vq_internal_search(a, sub, dtype, true, p.blocks, st);
+    if (e == hipSuccess) e = vq_internal_lbg_gather(a, sub, p.chunks, sums, counts, dist, st);
+    if (e != hipSuccess) return fail(VQ_E_HIP, "launch of k_cache_search failed: %s", hipGetErrorString(e));
     return VQ_OK;
 }
 

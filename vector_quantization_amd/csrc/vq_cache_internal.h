@@ -43,6 +43,29 @@ struct AttendArgs {
     float2 *part_ml;                   // (splits, rows * q_heads): maximum (base 2) and sum
 };
 
+struct SearchArgs {
+    const void *x[2];
+    int64_t token_stride[2], head_stride[2];
+    const void *cb[2];
+    int64_t tokens;
+    int cb_heads, heads, dim, K;
+    int pw, chunk;                     // parts a workgroup takes, tokens a wave takes
+    const int64_t *slots;              // writing
+    int64_t pages;
+    int page, page_shift;              // page = 1 << page_shift, or page_shift < 0
+    uint8_t *k_codes, *v_codes;
+    float *part_sums;                  // training: (chunks, heads * parts, sub + 1, 256), the last plane the counts
+    double *part_dist;                 // (chunks, heads * parts)
+};
+
+struct SearchPlan {
+    int pw, chunk, blocks, chunks;
+};
+// both: 2 where keys and values are searched by one launch
+VQ_HIDDEN SearchPlan vq_internal_search_plan(int64_t tokens, int heads, int dim, int sub, int both);
+VQ_HIDDEN hipError_t vq_internal_search(const SearchArgs &a, int sub, int dtype, bool train, int blocks, hipStream_t stream);
+VQ_HIDDEN hipError_t vq_internal_lbg_gather(const SearchArgs &a, int sub, int chunks, double *sums, int64_t *counts, double *dist, hipStream_t stream);
+
 // How an attention call is laid out: RB * 16 rows to a workgroup of NW waves.
 struct AttendPlan {
     int rb, nw;

@@ -1,0 +1,392 @@
+// vq_cache_search.hip -- nearest codewords of float sub-vectors: vq_cache_write, and the search and sums of vq_cache_lbg_accum (vq_cache.h).
+//
+// A code is the argmin of a squared distance summed in fp64, the lowest codeword of equal ones.  It is found in three steps, each of
+// which hands on what it cannot decide:
+//   1. Scores 1/2 |c|^2 - x.c of 32 vectors against 32 codewords at a time, v_mfma 32x32x16 bf16.  Numbers of wider types go in as two or three
+//      bf16 pieces each, and 1/2 |c|^2 as three further terms against ones, so a score comes out of the matrix unit whole.  A lane keeps the two
+//      least of the minima over groups of 8 codewords, the group's number in the low bits.  With B = 1/2 max |c|^2 + |x| max |c|, every
+//      score is off by at most 2^-18 B (up to 64 additions in fp32, dropped pieces, the group number), so a second-best group more
+//      than 2^-16 B behind holds no nearest codeword.
+//   2. The 8 codewords of the best group by direct differences in fp32, each sum off by less than 2^-19 of itself.
+//   3. Vectors that either step leaves open (close calls, ties, values beyond fp32's range, what is not finite) are searched by the whole wave
+//      in fp64, by the definition: about one in a hundred.
+//
+// A wave keeps its part's 256 codewords in registers as the operand of step 1 and streams its tokens past them.
+#include "vq_cache_internal.h"
+
+namespace {
+
+template <typename V> constexpr int PIECES = 3;
+template <> constexpr int PIECES<_Float16> = 2;
+template <> constexpr int PIECES<__bf16> = 1;
+
+// The products of pieces that step 1 takes: (vector's piece, codeword's piece), those below 2^-24 of the whole left out.
+struct Terms {
+    int n, x[6], c[6];
+};
+constexpr Terms terms_of(int xp, int cp) {
+    Terms t = {0, {}, {}};
+    for (int i = 0; i < xp; ++i)
+        for (int j = 0; j < cp; ++j)
+            if (i + j < 3) t.x[t.n] = i, t.c[t.n] = j, ++t.n;
+    return t;
+}
+
+constexpr int SEARCH_WAVES = 8;
+constexpr float FAR_SCORE = 1e38f, FAR_NUMBER = 1e18f, BOUND_MOST = 1e30f;
+constexpr float SUM_SCALE = 16777216.0f;       // lifts fp32's smallest numbers into bf16's normal range
+
+__device__ inline uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+
+// v = sum of P bf16 pieces (to 2^-8P of itself; exact for a type of 8P bits).
+template <int P> __device__ inline void split(float v, uint32_t (&piece)[P]) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        piece[i] = bf16_bits(v);
+        v -= __builtin_bit_cast(float, piece[i] << 16);
+    }
+}
+
+template <typename V, int N> struct alignas(N * sizeof(V) < 16 ? N * sizeof(V) : 16) Numbers {
+    V v[N];
+};
+
+__device__ inline void halves(float v, float &lo, float &hi) {      // the value of lane l and of lane l + 32, in both
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    const uint32_t first = r[0], second = r[1];
+    lo = __builtin_bit_cast(float, first);
+    hi = __builtin_bit_cast(float, second);
+}
+
+// The lesser of two finite scores, without the canonicalisation that fminf of unknown bits brings.
+__device__ inline float least(float a, float b) { return __builtin_amdgcn_fmed3f(-FAR_SCORE * 3.0f, a, b); }
+
+// T: the vectors' type, C: the codebook's; NT: groups of 32 codewords.
+template <typename T, typename C, int SUB, int NT, bool TRAIN>
+__global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const SearchArgs a) {
+    constexpr int XP = PIECES<T>, CP = PIECES<C>, H2 = SUB / 2;
+    constexpr Terms TM = terms_of(XP, CP);
+    constexpr int PAIRS = TM.n * H2 + 2, NM = (PAIRS * 2 + 15) / 16;     // slots in pairs; the last two hold the norm
+    __shared__ float s_tab[SEARCH_WAVES][NT * 32 * SUB];
+    __shared__ int16_t s_lab[TRAIN ? SEARCH_WAVES : 1][32];
+    __shared__ __align__(16) uint32_t s_x[TRAIN ? SEARCH_WAVES : 1][XP][32][H2];
+    const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int which = blockIdx.z, parts = a.dim / SUB, per = parts / a.pw;
+    const int h = blockIdx.x / per, m = blockIdx.x % per * a.pw + wave % a.pw;
+    const int chunk = blockIdx.y * (SEARCH_WAVES / a.pw) + wave / a.pw;
+    const int64_t begin = (int64_t)chunk * a.chunk;
+    const int64_t end = begin + a.chunk < a.tokens ? begin + a.chunk : a.tokens;
+    if (begin >= end && !TRAIN) return;
+    float *tab = s_tab[wave];
+    const C *cb = static_cast<const C *>(a.cb[which]) + (a.cb_heads == 1 ? 0 : (int64_t)h * a.K * a.dim) + m * SUB;
+    const T *x0 = static_cast<const T *>(a.x[which]) + h * a.head_stride[which] + m * SUB;
+
+    // the codewords: operand of step 1, and in fp32 for steps 2 and 3; rows past K lie far away
+    u32x4 A[NT][NM];
+    float reach = 0.0f;                                                   // max |c|^2, infinite if any codeword is not finite
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int k = t * 32 + col;
+        Numbers<C, SUB> raw;
+        if (k < a.K) raw = *reinterpret_cast<const Numbers<C, SUB> *>(cb + (int64_t)k * a.dim);
+        float c[SUB], norm = 0.0f;
+        uint32_t cp[CP][H2];
+#pragma unroll
+        for (int e = 0; e < SUB; ++e) {
+            c[e] = k < a.K ? (float)raw.v[e] : 0.0f;
+            norm += c[e] * c[e];
+        }
+        reach = fmaxf(reach, norm < INFINITY ? norm : INFINITY);
+#pragma unroll
+        for (int i = 0; i < H2; ++i) {
+            uint32_t p0[CP], p1[CP];
+            split<CP>(-c[2 * i], p0);
+            split<CP>(-c[2 * i + 1], p1);
+#pragma unroll
+            for (int p = 0; p < CP; ++p) cp[p][i] = p0[p] | p1[p] << 16;
+        }
+        uint32_t np[3];
+        split<3>(k < a.K ? 0.5f * norm : FAR_SCORE, np);
+        auto pair = [&](int s) -> uint32_t {
+            return s < TM.n * H2 ? cp[TM.c[s / H2]][s % H2] : s == TM.n * H2 ? np[0] | np[1] << 16 : s == TM.n * H2 + 1 ? np[2] : 0u;
+        };
+#pragma unroll
+        for (int n = 0; n < NM; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) A[t][n][j] = hh ? pair(8 * n + 4 + j) : pair(8 * n + j);
+        if (hh == 0)
+#pragma unroll
+            for (int e = 0; e < SUB; ++e) tab[k * SUB + e] = k < a.K ? c[e] : FAR_NUMBER;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) reach = fmaxf(reach, __shfl_xor(reach, o));
+    const float far = __builtin_amdgcn_sqrtf(reach);
+
+    f32x4 sum[TRAIN ? SUB + 1 : 1];
+    double away = 0.0;
+    if constexpr (TRAIN)
+#pragma unroll
+        for (int e = 0; e <= SUB; ++e) sum[e] = (f32x4){0, 0, 0, 0};
+
+    auto fetch = [&](int64_t t) -> Numbers<T, SUB> {                      // past the end: the last token again
+        t = t < end ? t : end - 1;
+        return *reinterpret_cast<const Numbers<T, SUB> *>(x0 + t * a.token_stride[which]);
+    };
+    Numbers<T, SUB> next;
+    if (begin < end) next = fetch(begin + col);
+    for (int64_t t0 = begin; t0 < end; t0 += 32) {
+        const Numbers<T, SUB> raw = next;
+        if (t0 + 32 < end) next = fetch(t0 + 32 + col);
+        const int64_t token = t0 + col;
+        float x[SUB], size = 0.0f;
+        uint32_t xp[XP][H2];
+#pragma unroll
+        for (int e = 0; e < SUB; ++e) {
+            x[e] = (float)raw.v[e];
+            size += x[e] * x[e];
+        }
+#pragma unroll
+        for (int i = 0; i < H2; ++i) {
+            uint32_t p0[XP], p1[XP];
+            split<XP>(x[2 * i], p0);
+            split<XP>(x[2 * i + 1], p1);
+#pragma unroll
+            for (int p = 0; p < XP; ++p) xp[p][i] = p0[p] | p1[p] << 16;
+        }
+        auto pair = [&](int s) -> uint32_t {
+            return s < TM.n * H2 ? xp[TM.x[s / H2]][s % H2] : s == TM.n * H2 ? 0x3f803f80u : s == TM.n * H2 + 1 ? 0x3f80u : 0u;
+        };
+        u32x4 B[NM];
+#pragma unroll
+        for (int n = 0; n < NM; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) B[n][j] = hh ? pair(8 * n + 4 + j) : pair(8 * n + j);
+
+        // step 1
+        float m1 = FAR_SCORE * 3.0f, m2 = FAR_SCORE * 3.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            f32x16 s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < NM; ++n)
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, A[t][n]), __builtin_bit_cast(bf16x8, B[n]), s, 0, 0, 0);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float v = FAR_SCORE * 3.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) v = fminf(fminf(v, s[8 * q + i]), s[8 * q + i + 1]);
+                const float key = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) & ~15u) | (uint32_t)(2 * t + q));
+                m2 = __builtin_amdgcn_fmed3f(m1, m2, key);
+                m1 = least(m1, key);
+            }
+        }
+        float l1, h1, l2, h2;
+        halves(m1, l1, h1);
+        halves(m2, l2, h2);
+        const bool upper = h1 < l1;
+        const float best = upper ? h1 : l1, second = least(upper ? l1 : h1, least(l2, h2));
+        const float bound = 0.5f * reach + __builtin_amdgcn_sqrtf(size) * far;
+        bool open = !(second - best > bound * 1.52587890625e-5f + 1e-36f) || !(bound < BOUND_MOST);
+        const int group = __builtin_bit_cast(uint32_t, best) & 15;
+
+        // step 2: the two halves of a wave take four codewords each
+        const int k0 = group * 16 + 4 * (int)upper;
+        uint32_t d1 = 0x7f800000u, d2 = 0x7f800000u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float d = 0.0f;
+#pragma unroll
+            for (int e = 0; e < SUB; ++e) {
+                const float v = x[e] - tab[(k0 + 8 * hh + j) * SUB + e];
+                d = __builtin_fmaf(v, v, d);
+            }
+            const uint32_t key = (__builtin_bit_cast(uint32_t, d) & ~3u) | j;
+            d2 = max(min(d1, d2), min(max(d1, d2), key));
+            d1 = min(d1, key);
+        }
+        const auto r1 = __builtin_amdgcn_permlane32_swap(d1, d1, false, false);
+        const auto r2 = __builtin_amdgcn_permlane32_swap(d2, d2, false, false);
+        const bool right = r1[1] < r1[0];
+        const uint32_t near = right ? r1[1] : r1[0], other = min(right ? r1[0] : r1[1], min(r2[0], r2[1]));
+        open = open || !(__builtin_bit_cast(float, other) > __builtin_bit_cast(float, near) * 1.00000763f + 1e-36f);
+        int code = k0 + (right ? 8 : 0) + (int)(near & 3u);
+
+        // step 3
+        uint64_t todo = __ballot(open && token < end) & 0xffffffffu;
+        while (todo) {
+            const int v = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            double y[SUB];
+#pragma unroll
+            for (int e = 0; e < SUB; ++e) y[e] = (double)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x[e]), v));
+            double d = INFINITY;
+            int k_best = 256;
+            for (int k = lane; k < a.K; k += 64) {
+                double f = 0.0;
+#pragma unroll
+                for (int e = 0; e < SUB; ++e) {
+                    const double w = y[e] - (double)tab[k * SUB + e];
+                    f += w * w;
+                }
+                if (f < d) d = f, k_best = k;
+            }
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const double d_o = __shfl_xor(d, o);
+                const int k_o = __shfl_xor(k_best, o);
+                if (d_o < d || (d_o == d && k_o < k_best)) d = d_o, k_best = k_o;
+            }
+            if (col == v) code = k_best < 256 ? k_best : 0;
+        }
+
+        if constexpr (!TRAIN) {
+            const int64_t slot = hh == 0 && token < end ? a.slots[token] : -1;
+            if (slot >= 0 && slot < a.pages * a.page) {
+                const int64_t p = a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page;
+                const int o = (int)(slot - p * a.page);
+                if (which == 0) a.k_codes[((p * a.heads + h) * a.page + o) * parts + m] = (uint8_t)code;
+                else a.v_codes[((p * a.heads + h) * parts + m) * a.page + o] = (uint8_t)code;
+            }
+        } else {
+            bool fine = token < end;
+#pragma unroll
+            for (int e = 0; e < SUB; ++e) fine = fine && fabsf(x[e]) < INFINITY;
+            // sums by products with the one-hot numbers of the codewords: number = 16 hi + lo, and
+            // sum[hi][lo] = sum over vectors of (x where its hi is this row) * (1 where its lo is this column)
+            if (hh == 0) {
+                if (fine) {
+                    double f = 0.0;
+#pragma unroll
+                    for (int e = 0; e < SUB; ++e) {
+                        const double w = (double)x[e] - (double)tab[code * SUB + e];
+                        f += w * w;
+                    }
+                    away += f <= INFINITY ? f : INFINITY;
+                }
+                s_lab[wave][col] = fine ? (int16_t)code : (int16_t)-1;
+#pragma unroll
+                for (int i = 0; i < H2; ++i) {
+                    uint32_t p0[XP], p1[XP];
+                    split<XP>(x[2 * i] * SUM_SCALE, p0);
+                    split<XP>(x[2 * i + 1] * SUM_SCALE, p1);
+#pragma unroll
+                    for (int p = 0; p < XP; ++p) s_x[wave][p][col][i] = p0[p] | p1[p] << 16;
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int row = lane & 15, g = lane >> 4;
+            u32x4 member, lows;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int la = s_lab[wave][8 * g + 2 * j], lb = s_lab[wave][8 * g + 2 * j + 1];
+                member[j] = ((la >> 4) == row ? 0xffffu : 0u) | ((lb >> 4) == row ? 0xffff0000u : 0u);
+                lows[j] = ((la & 15) == row ? 0x3f80u : 0u) | ((lb & 15) == row ? 0x3f800000u : 0u);
+            }
+            const bf16x8 lo8 = __builtin_bit_cast(bf16x8, lows);
+#pragma unroll
+            for (int p = 0; p < XP; ++p)
+#pragma unroll
+                for (int i = 0; i < H2; ++i) {
+                    u32x4 e0, e1;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t va = s_x[wave][p][8 * g + 2 * j][i], vb = s_x[wave][p][8 * g + 2 * j + 1][i];
+                        e0[j] = __builtin_amdgcn_perm(vb, va, 0x05040100u) & member[j];
+                        e1[j] = __builtin_amdgcn_perm(vb, va, 0x07060302u) & member[j];
+                    }
+                    sum[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e0), lo8, sum[2 * i], 0, 0, 0);
+                    sum[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e1), lo8, sum[2 * i + 1], 0, 0, 0);
+                }
+            u32x4 ones;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ones[j] = member[j] & 0x3f803f80u;
+            sum[SUB] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), lo8, sum[SUB], 0, 0, 0);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    if constexpr (TRAIN) {
+        const int64_t place = (int64_t)chunk * a.heads * parts + h * parts + m;
+#pragma unroll
+        for (int e = 0; e <= SUB; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a.part_sums[(place * (SUB + 1) + e) * 256 + (4 * (lane >> 4) + i) * 16 + (lane & 15)] = sum[e][i];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) away += __shfl_xor(away, o);
+        if (lane == 0) a.part_dist[place] = away;
+    }
+}
+
+// Adds the chunks' sums, in fp64 and in their order: a workgroup for each head and part, a thread for each codeword.
+__global__ __launch_bounds__(256) void k_lbg_gather(const float *part_sums, const double *part_dist, int chunks, int heads, int dim, int sub, int K,
+                                                    double *sums, int64_t *counts, double *dist) {
+    const int parts = dim / sub, h = blockIdx.x / parts, m = blockIdx.x % parts, k = threadIdx.x;
+    const int64_t groups = (int64_t)heads * parts;
+    for (int e = 0; e <= sub; ++e) {
+        double s = 0.0;
+        for (int c = 0; c < chunks; ++c) s += (double)part_sums[((c * groups + blockIdx.x) * (sub + 1) + e) * 256 + k];
+        if (k >= K) continue;
+        if (e < sub) sums[((int64_t)h * K + k) * dim + m * sub + e] = s / (double)SUM_SCALE;
+        else counts[(int64_t)blockIdx.x * K + k] = (int64_t)s;
+    }
+    if (k == 0) {
+        double d = 0.0;
+        for (int c = 0; c < chunks; ++c) d += part_dist[c * groups + blockIdx.x];
+        dist[blockIdx.x] = d;
+    }
+}
+
+template <typename T, typename C, int SUB, bool TRAIN>
+void launch_sub(const SearchArgs &a, dim3 grid, hipStream_t stream) {
+    const dim3 block(SEARCH_WAVES * 64);
+    if (a.K <= 64) hipLaunchKernelGGL((k_cache_search<T, C, SUB, 2, TRAIN>), grid, block, 0, stream, a);
+    else if (a.K <= 128) hipLaunchKernelGGL((k_cache_search<T, C, SUB, 4, TRAIN>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_cache_search<T, C, SUB, 8, TRAIN>), grid, block, 0, stream, a);
+}
+
+template <typename T, typename C, bool TRAIN>
+void launch(const SearchArgs &a, int sub, dim3 grid, hipStream_t stream) {
+    if (sub == 2) launch_sub<T, C, 2, TRAIN>(a, grid, stream);
+    else if (sub == 4) launch_sub<T, C, 4, TRAIN>(a, grid, stream);
+    else launch_sub<T, C, 8, TRAIN>(a, grid, stream);
+}
+
+}  // namespace
+
+SearchPlan vq_internal_search_plan(int64_t tokens, int heads, int dim, int sub, int both) {
+    constexpr int CUS = 256;
+    SearchPlan p;
+    const int parts = dim / sub;
+    p.pw = parts % 8 ? 4 : 8;
+    const int64_t side = SEARCH_WAVES / p.pw;                             // token ranges side by side in one workgroup
+    const int64_t base = (int64_t)heads * (parts / p.pw) * both;
+    const int64_t most = (tokens + 32 * side - 1) / (32 * side), least = (tokens + 4096 * side - 1) / (4096 * side);
+    int64_t n = (2 * CUS + base - 1) / base;
+    n = n < most ? n : most;
+    n = n > least ? n : least;
+    p.chunk = (int)(((tokens + n * side - 1) / (n * side) + 31) / 32 * 32);
+    p.blocks = (int)((tokens + p.chunk * side - 1) / (p.chunk * side));
+    p.chunks = (int)(p.blocks * side);
+    return p;
+}
+
+hipError_t vq_internal_search(const SearchArgs &a, int sub, int dtype, bool train, int blocks, hipStream_t stream) {
+    const dim3 grid(a.heads * (a.dim / sub / a.pw), blocks, train ? 1 : 2);
+    if (train) {
+        if (dtype == VQ_F32) launch<float, float, true>(a, sub, grid, stream);
+        else if (dtype == VQ_BF16) launch<__bf16, float, true>(a, sub, grid, stream);
+        else launch<_Float16, float, true>(a, sub, grid, stream);
+    } else {
+        if (dtype == VQ_BF16) launch<__bf16, __bf16, false>(a, sub, grid, stream);
+        else launch<_Float16, _Float16, false>(a, sub, grid, stream);
+    }
+    return hipGetLastError();
+}
+
+hipError_t vq_internal_lbg_gather(const SearchArgs &a, int sub, int chunks, double *sums, int64_t *counts, double *dist, hipStream_t stream) {
+    hipLaunchKernelGGL(k_lbg_gather, dim3(a.heads * (a.dim / sub)), dim3(256), 0, stream, a.part_sums, a.part_dist, chunks, a.heads, a.dim, sub, a.K,
+                       sums, counts, dist);
+    return hipGetLastError();
+}
