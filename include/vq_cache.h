@@ -76,11 +76,17 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
  * the sum of the least squared distances.  A vector of numbers that are not all finite is left out of all three.
  * sums (heads, K, dim) fp64, counts (heads, parts, K) int64, dist (heads, parts) fp64 are overwritten; the result
  * does not depend on timing.  cb is (heads, K, dim) fp32; x is of any of the three types, its finite numbers below
- * 2^100 in size.  Adding several calls' sums, counts and dist gives those of their tokens together. */
+ * 2^90 in size.  Adding several calls' sums, counts and dist gives those of their tokens together. */
 size_t vq_cache_lbg_ws_bytes(int64_t tokens, int heads, int dim, int sub, int K);
 int vq_cache_lbg_accum(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens,
                        const float *cb, int heads, int dim, int sub, int K, int dtype,
                        double *sums, int64_t *counts, double *dist, void *ws, size_t ws_bytes, void *stream);
+
+/* Both halves in one: the new codebook, the members' numbers (heads, parts, K) and the mean squared distance to the old codewords
+ * (heads, parts).  cb_new may be cb. */
+int vq_cache_lbg_iterate(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens,
+                         const float *cb, int heads, int dim, int sub, int K, int dtype,
+                         float *cb_new, int64_t *counts, double *mean_dist, void *ws, size_t ws_bytes, void *stream);
 
 /* The closing half: cb_new = sums / counts, a codeword without members staying as it is in cb_old, and
  * mean_dist (heads, parts) = dist / the number of vectors (0 where there is none).  cb_new may be cb_old. */

@@ -81,6 +81,7 @@ CACHE_SIGNATURES = {
                                 _i64, _i64, _dbl, _vp, _vp, _vp, _sz, _vp]),
     "vq_cache_lbg_ws_bytes": (_sz, [_i64, _i, _i, _i, _i]),
     "vq_cache_lbg_accum": (_i, [_vp, _i64, _i64, _i64, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vq_cache_lbg_iterate": (_i, [_vp, _i64, _i64, _i64, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "vq_cache_lbg_finish": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp]),
 }
 

@@ -16,7 +16,6 @@ The methods launch on the engine's device and its current stream, allocate what 
 from torch's allocator and wait for nothing, so they may be captured into a graph.  None of them is differentiable:
 they refuse tensors that require a gradient.
 """
-import ctypes
 import math
 
 import torch
@@ -26,13 +25,12 @@ from ._lib import lib, check, VQ_BF16, VQ_F16, VQ_F32
 _DTYPES = {torch.float32: VQ_F32, torch.bfloat16: VQ_BF16, torch.float16: VQ_F16}
 
 
-def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
-
-
-# ---- checks of arguments: shapes, types and devices only, nothing is read from the GPU ------------------------------
+# ---- checks of arguments: shapes, types and devices only, nothing is read from the GPU.  They run on every call, so what
+# is right passes in one expression and only what is not is looked at again for its message. ------------------------------
 
 def _tensor(name, t, device, dtypes, dims):
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dims and t.device == device and not t.requires_grad:
+        return t
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.device != device:
@@ -41,7 +39,7 @@ def _tensor(name, t, device, dtypes, dims):
         raise ValueError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
     if t.dim() != dims:
         raise ValueError(f"{name} must have {dims} dimensions, got shape {tuple(t.shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the cache operators are not differentiable")
     return t
 
@@ -54,47 +52,53 @@ def _whole(name, t):
 
 def _vectors(t):
     """t as the kernels read it: each vector's numbers side by side from a multiple of 16 bytes.  Anything else is copied."""
-    size = t.element_size()
-    if t.numel() == 0 or (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * size % 16 == 0 and t.stride(1) * size % 16 == 0):
+    token, head, one = t.stride()
+    if one == 1 and (token | head) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _books(t, multiple=16):
-    return t if t.is_contiguous() and t.data_ptr() % multiple == 0 else t.clone(memory_format=torch.contiguous_format)
+def _books(t):
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+_HALVES = (torch.bfloat16, torch.float16)
+_BYTES = (torch.uint8,)
+_INT32 = (torch.int32,)
+_INT64 = (torch.int64,)
+_FLOATS = tuple(_DTYPES)
+_F32 = (torch.float32,)
+_F64 = (torch.float64,)
 
 
 def cache_shape(k_cb, v_cb, k_codes, v_codes, device):
     """Checks codebooks and code buffers against each other; returns (heads, dim, sub, K, pages, page)."""
-    _tensor("k_cb", k_cb, device, (torch.bfloat16, torch.float16), 3)
+    _tensor("k_cb", k_cb, device, _HALVES, 3)
     _tensor("v_cb", v_cb, device, (k_cb.dtype,), 3)
-    _whole("k_codes", _tensor("k_codes", k_codes, device, (torch.uint8,), 4))
-    _whole("v_codes", _tensor("v_codes", v_codes, device, (torch.uint8,), 4))
+    _whole("k_codes", _tensor("k_codes", k_codes, device, _BYTES, 4))
+    _whole("v_codes", _tensor("v_codes", v_codes, device, _BYTES, 4))
     pages, heads, page, parts = k_codes.shape
-    if 0 in k_codes.shape:
+    books, K, dim = k_cb.shape
+    if not (pages and heads and page and parts):
         raise ValueError(f"k_codes must not be empty, got shape {tuple(k_codes.shape)}")
-    if tuple(v_codes.shape) != (pages, heads, parts, page):
+    if v_codes.shape != (pages, heads, parts, page):
         raise ValueError(f"v_codes must have shape {(pages, heads, parts, page)} (k_codes: {tuple(k_codes.shape)}), got {tuple(v_codes.shape)}")
-    if k_cb.shape != v_cb.shape or k_cb.shape[0] not in (1, heads) or 0 in k_cb.shape:
+    if k_cb.shape != v_cb.shape or books not in (1, heads) or not (K and dim):
         raise ValueError(f"codebooks must be (1 or {heads}, K, dim) of one shape, got {tuple(k_cb.shape)} and {tuple(v_cb.shape)}")
-    K, dim = k_cb.shape[1:]
     if dim % parts:
         raise ValueError(f"vectors of {dim} numbers cannot be cut into the {parts} codes of a cache entry")
     return heads, dim, dim // parts, K, pages, page
 
 
-def check_vectors(name, t, tokens, heads, dim, dtype, device):
-    _tensor(name, t, device, (dtype,), 3)
-    if tokens is not None and t.shape[0] != tokens or t.shape[1] != heads or t.shape[2] != dim:
-        raise ValueError(f"{name} must have shape {('tokens' if tokens is None else tokens, heads, dim)}, got {tuple(t.shape)}")
-    return _vectors(t)
-
-
-def check_ints(name, t, dtype, shape, device):
-    _tensor(name, t, device, (dtype,), len(shape))
-    if any(s is not None and s != n for s, n in zip(shape, t.shape)):
-        raise ValueError(f"{name} must have shape {tuple('any' if s is None else s for s in shape)}, got {tuple(t.shape)}")
+def _ints(name, t, dtypes, dims, device):
+    _tensor(name, t, device, dtypes, dims)
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _sized(name, t, shape):
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    return t
 
 
 class CacheOps:
@@ -109,34 +113,45 @@ class CacheOps:
         return (torch.zeros((pages, heads, page, parts), dtype=torch.uint8, device=self.device),
                 torch.zeros((pages, heads, parts, page), dtype=torch.uint8, device=self.device))
 
+    def _launch(self, name, *args):
+        """Calls the library on the engine's device and its current stream."""
+        stream = self._stream()
+        if torch.cuda.current_device() == self.device.index:
+            check(getattr(lib, name)(*args, stream), name)
+        else:
+            with torch.cuda.device(self.device):
+                check(getattr(lib, name)(*args, stream), name)
+
     def cache_write(self, k, v, slots, k_cb, v_cb, k_codes, v_codes):
         """Quantises k and v (tokens, heads, dim) and stores the codes at slots (tokens, int64); a slot outside the cache
         (-1, say) stores nothing.  Slots should be distinct: of two tokens with one slot, each code is that of either."""
-        heads, dim, sub, K, pages, page = cache_shape(k_cb, v_cb, k_codes, v_codes, self.device)
-        slots = check_ints("slots", slots, torch.int64, (None,), self.device)
+        device = self.device
+        heads, dim, sub, K, pages, page = cache_shape(k_cb, v_cb, k_codes, v_codes, device)
+        slots = _ints("slots", slots, _INT64, 1, device)
         tokens = slots.shape[0]
-        k = check_vectors("k", k, tokens, heads, dim, k_cb.dtype, self.device)
-        v = check_vectors("v", v, tokens, heads, dim, k_cb.dtype, self.device)
+        dtypes, shape = (k_cb.dtype,), (tokens, heads, dim)
+        _sized("k", _tensor("k", k, device, dtypes, 3), shape)
+        _sized("v", _tensor("v", v, device, dtypes, 3), shape)
         if tokens == 0:
             return
-        k_cb, v_cb = _books(k_cb), _books(v_cb)
-        with torch.cuda.device(self.device):
-            check(lib.vq_cache_write(_ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), _ptr(slots), tokens,
-                                     _ptr(k_cb), _ptr(v_cb), k_cb.shape[0], heads, dim, sub, K, _DTYPES[k_cb.dtype], _ptr(k_codes),
-                                     _ptr(v_codes), pages, page, self._stream()), "vq_cache_write")
+        k, v, k_cb, v_cb = _vectors(k), _vectors(v), _books(k_cb), _books(v_cb)
+        self._launch("vq_cache_write", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(),
+                     tokens, k_cb.data_ptr(), v_cb.data_ptr(), k_cb.shape[0], heads, dim, sub, K, _DTYPES[k_cb.dtype], k_codes.data_ptr(),
+                     v_codes.data_ptr(), pages, page)
 
     def cache_read(self, slots, k_cb, v_cb, k_codes, v_codes):
         """The keys and values that the codes at slots stand for: two tensors (tokens, heads, dim) of the codebooks'
         dtype.  A slot outside the cache reads as zeros."""
-        heads, dim, sub, K, pages, page = cache_shape(k_cb, v_cb, k_codes, v_codes, self.device)
-        slots = check_ints("slots", slots, torch.int64, (None,), self.device)
+        device = self.device
+        heads, dim, sub, K, pages, page = cache_shape(k_cb, v_cb, k_codes, v_codes, device)
+        slots = _ints("slots", slots, _INT64, 1, device)
         tokens = slots.shape[0]
         k_cb, v_cb = _books(k_cb), _books(v_cb)
-        k, v = (torch.empty((tokens, heads, dim), dtype=k_cb.dtype, device=self.device) for _ in range(2))
+        k = torch.empty((tokens, heads, dim), dtype=k_cb.dtype, device=device)
+        v = torch.empty((tokens, heads, dim), dtype=k_cb.dtype, device=device)
         if tokens:
-            with torch.cuda.device(self.device):
-                check(lib.vq_cache_read(_ptr(slots), tokens, _ptr(k_cb), _ptr(v_cb), k_cb.shape[0], heads, dim, sub, K, _DTYPES[k_cb.dtype],
-                                        _ptr(k_codes), _ptr(v_codes), pages, page, _ptr(k), _ptr(v), self._stream()), "vq_cache_read")
+            self._launch("vq_cache_read", slots.data_ptr(), tokens, k_cb.data_ptr(), v_cb.data_ptr(), k_cb.shape[0], heads, dim, sub, K,
+                         _DTYPES[k_cb.dtype], k_codes.data_ptr(), v_codes.data_ptr(), pages, page, k.data_ptr(), v.data_ptr())
         return k, v
 
     def cache_attention(self, q, k_cb, v_cb, k_codes, v_codes, table, kv_lens, starts, max_q, max_kv=None, scale=None, out=None,
@@ -152,86 +167,104 @@ class CacheOps:
         (max_kv None: what the table can hold).  scale: 1 / sqrt(dim) if None.
         Returns out (rows, q_heads, dim), with want_lse also the natural logarithm of each row's sum of exponentials
         (rows, q_heads) float32, by which results over parts of a context are joined."""
-        heads, dim, sub, K, pages, page = cache_shape(k_cb, v_cb, k_codes, v_codes, self.device)
-        _tensor("q", q, self.device, (k_cb.dtype,), 3)
-        rows, q_heads = q.shape[:2]
-        if q.shape[2] != dim or q_heads == 0 or q_heads % heads:
+        device = self.device
+        heads, dim, sub, K, pages, page = cache_shape(k_cb, v_cb, k_codes, v_codes, device)
+        dtype = k_cb.dtype
+        _tensor("q", q, device, (dtype,), 3)
+        rows, q_heads, q_dim = q.shape
+        if q_dim != dim or q_heads == 0 or q_heads % heads:
             raise ValueError(f"q must have shape (rows, a multiple of {heads}, {dim}), got {tuple(q.shape)}")
-        kv_lens = check_ints("kv_lens", kv_lens, torch.int32, (None,), self.device)
+        kv_lens = _ints("kv_lens", kv_lens, _INT32, 1, device)
         seqs = kv_lens.shape[0]
-        starts = check_ints("starts", starts, torch.int32, (seqs + 1,), self.device)
-        table = check_ints("table", table, torch.int32, (seqs, None), self.device)
+        starts = _sized("starts", _ints("starts", starts, _INT32, 1, device), (seqs + 1,))
+        table = _ints("table", table, _INT32, 2, device)
         width = table.shape[1]
+        _sized("table", table, (seqs, width))
         if out is None:
-            out = torch.empty((rows, q_heads, dim), dtype=q.dtype, device=self.device)
+            out = torch.empty((rows, q_heads, dim), dtype=dtype, device=device)
         else:
-            _whole("out", _tensor("out", out, self.device, (q.dtype,), 3))
-            if out.shape != q.shape:
-                raise ValueError(f"out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
-        lse = torch.empty((rows, q_heads), dtype=torch.float32, device=self.device) if want_lse else None
+            _sized("out", _whole("out", _tensor("out", out, device, (dtype,), 3)), (rows, q_heads, dim))
+        lse = torch.empty((rows, q_heads), dtype=torch.float32, device=device) if want_lse else None
         if rows and seqs:
             q, k_cb, v_cb = _vectors(q), _books(k_cb), _books(v_cb)
             scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
             max_q = int(max_q)
             max_kv = max(1, width * page) if max_kv is None else int(max_kv)
             need = lib.vq_cache_attention_ws_bytes(rows, q_heads, heads, dim, sub, K, seqs, max_q, max_kv)
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            with torch.cuda.device(self.device):
-                check(lib.vq_cache_attention(_ptr(q), q.stride(0), q.stride(1), rows, q_heads, _ptr(k_cb), _ptr(v_cb), k_cb.shape[0], heads,
-                                             dim, sub, K, _DTYPES[q.dtype], _ptr(k_codes), _ptr(v_codes), pages, page, _ptr(table), seqs,
-                                             width, _ptr(kv_lens), _ptr(starts), max_q, max_kv, scale, _ptr(out), _ptr(lse), _ptr(ws), need,
-                                             self._stream()), "vq_cache_attention")
+            ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+            self._launch("vq_cache_attention", q.data_ptr(), q.stride(0), q.stride(1), rows, q_heads, k_cb.data_ptr(), v_cb.data_ptr(),
+                         k_cb.shape[0], heads, dim, sub, K, _DTYPES[dtype], k_codes.data_ptr(), v_codes.data_ptr(), pages, page,
+                         table.data_ptr(), seqs, width, kv_lens.data_ptr(), starts.data_ptr(), max_q, max_kv, scale, out.data_ptr(),
+                         lse.data_ptr() if want_lse else None, ws.data_ptr() if need else None, need)
         return (out, lse) if want_lse else out
+
+    def _lbg_arguments(self, x, cb, sub):
+        device = self.device
+        _tensor("cb", cb, device, _F32, 3)
+        _tensor("x", x, device, _FLOATS, 3)
+        heads, K, dim = cb.shape
+        tokens = x.shape[0]
+        _sized("x", x, (tokens, heads, dim))
+        if not (heads and K and dim) or sub < 1 or dim % sub:
+            raise ValueError(f"codebook of shape {tuple(cb.shape)} cannot be cut into sub-vectors of {sub}")
+        return tokens, heads, K, dim, dim // sub
 
     def cache_lbg_accum(self, x, cb, sub):
         """The accumulating half of an LBG iteration of float codebooks cb (heads, K, dim) float32 over the vectors
         x (tokens, heads, dim): for each codeword the sum (heads, K, dim) float64 and number (heads, parts, K) int64 of the
         sub-vectors nearest to it, and the sum of their squared distances (heads, parts) float64.  A sub-vector of numbers
         that are not all finite is left out.  Shards' results are added."""
-        _tensor("cb", cb, self.device, (torch.float32,), 3)
-        _tensor("x", x, self.device, tuple(_DTYPES), 3)
-        heads, K, dim = cb.shape
-        check_vectors("x", x, None, heads, dim, x.dtype, self.device)
-        if 0 in cb.shape or sub < 1 or dim % sub:
-            raise ValueError(f"codebook of shape {tuple(cb.shape)} cannot be cut into sub-vectors of {sub}")
-        tokens, parts = x.shape[0], dim // sub
+        device = self.device
+        tokens, heads, K, dim, parts = self._lbg_arguments(x, cb, sub)
         make = torch.empty if tokens else torch.zeros
-        sums = make((heads, K, dim), dtype=torch.float64, device=self.device)
-        counts = make((heads, parts, K), dtype=torch.int64, device=self.device)
-        dist = make((heads, parts), dtype=torch.float64, device=self.device)
+        sums = make((heads, K, dim), dtype=torch.float64, device=device)
+        counts = make((heads, parts, K), dtype=torch.int64, device=device)
+        dist = make((heads, parts), dtype=torch.float64, device=device)
         if tokens:
             x, cb = _vectors(x), _books(cb)
             need = lib.vq_cache_lbg_ws_bytes(tokens, heads, dim, sub, K)
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-            with torch.cuda.device(self.device):
-                check(lib.vq_cache_lbg_accum(_ptr(x), x.stride(0), x.stride(1), tokens, _ptr(cb), heads, dim, sub, K, _DTYPES[x.dtype],
-                                             _ptr(sums), _ptr(counts), _ptr(dist), _ptr(ws), need, self._stream()), "vq_cache_lbg_accum")
+            ws = torch.empty(need, dtype=torch.uint8, device=device)
+            self._launch("vq_cache_lbg_accum", x.data_ptr(), x.stride(0), x.stride(1), tokens, cb.data_ptr(), heads, dim, sub, K, _DTYPES[x.dtype],
+                         sums.data_ptr(), counts.data_ptr(), dist.data_ptr(), ws.data_ptr(), need)
         return sums, counts, dist
 
     def cache_lbg_finish(self, sums, counts, dist, cb):
         """The closing half: (new codebook, mean squared distance (heads, parts)); a codeword without members stays."""
-        _tensor("cb", cb, self.device, (torch.float32,), 3)
+        device = self.device
+        _tensor("cb", cb, device, _F32, 3)
         heads, K, dim = cb.shape
-        _tensor("dist", dist, self.device, (torch.float64,), 2)
+        _tensor("dist", dist, device, _F64, 2)
         parts = dist.shape[1]
-        _tensor("sums", sums, self.device, (torch.float64,), 3)
-        _tensor("counts", counts, self.device, (torch.int64,), 3)
-        if 0 in cb.shape or parts < 1 or dim % parts or dist.shape[0] != heads or sums.shape != cb.shape or \
-                tuple(counts.shape) != (heads, parts, K):
+        _tensor("sums", sums, device, _F64, 3)
+        _tensor("counts", counts, device, _INT64, 3)
+        if not (heads and K and dim) or parts < 1 or dim % parts or dist.shape[0] != heads or sums.shape != cb.shape or \
+                counts.shape != (heads, parts, K):
             raise ValueError(f"shapes do not belong together: sums {tuple(sums.shape)}, counts {tuple(counts.shape)}, dist {tuple(dist.shape)}, "
                              f"cb {tuple(cb.shape)}")
         sums, counts, dist, cb = (t.contiguous() for t in (sums, counts, dist, cb))
         new, mean = torch.empty_like(cb), torch.empty_like(dist)
-        with torch.cuda.device(self.device):
-            check(lib.vq_cache_lbg_finish(_ptr(sums), _ptr(counts), _ptr(dist), _ptr(cb), heads, dim, dim // parts, K, _ptr(new), _ptr(mean),
-                                          self._stream()), "vq_cache_lbg_finish")
+        self._launch("vq_cache_lbg_finish", sums.data_ptr(), counts.data_ptr(), dist.data_ptr(), cb.data_ptr(), heads, dim, dim // parts, K,
+                     new.data_ptr(), mean.data_ptr())
         return new, mean
 
     def cache_lbg_iterate(self, x, cb, sub):
-        """One LBG iteration of the float codebooks cb (heads, K, dim) over the vectors x (tokens, heads, dim): returns (new
-        codebook, members (heads, parts, K), mean squared distance to the old codewords (heads, parts))."""
-        sums, counts, dist = self.cache_lbg_accum(x, cb, sub)
-        new, mean = self.cache_lbg_finish(sums, counts, dist, cb)
+        """One LBG iteration of the float codebooks cb (heads, K, dim) float32 over the vectors x (tokens, heads, dim): both
+        halves in one.  Returns (new codebook, members (heads, parts, K), mean squared distance to the old codewords
+        (heads, parts))."""
+        device = self.device
+        tokens, heads, K, dim, parts = self._lbg_arguments(x, cb, sub)
+        if tokens == 0:
+            sums, counts, dist = self.cache_lbg_accum(x, cb, sub)
+            new, mean = self.cache_lbg_finish(sums, counts, dist, cb)
+            return new, counts, mean
+        x, cb = _vectors(x), _books(cb)
+        new = torch.empty((heads, K, dim), dtype=torch.float32, device=device)
+        counts = torch.empty((heads, parts, K), dtype=torch.int64, device=device)
+        mean = torch.empty((heads, parts), dtype=torch.float64, device=device)
+        need = lib.vq_cache_lbg_ws_bytes(tokens, heads, dim, sub, K)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        self._launch("vq_cache_lbg_iterate", x.data_ptr(), x.stride(0), x.stride(1), tokens, cb.data_ptr(), heads, dim, sub, K, _DTYPES[x.dtype],
+                     new.data_ptr(), counts.data_ptr(), mean.data_ptr(), ws.data_ptr(), need)
         return new, counts, mean
 
 

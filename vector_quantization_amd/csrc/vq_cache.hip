@@ -30,53 +30,96 @@ int fail(int code, const char *fmt, ...) {
 // kernels
 // ------------------------------------------------------------------------------------------------
 
-// Where the code of one sub-vector lies.
-__device__ inline int64_t code_at(int which, int64_t slot, int h, int m, int heads, int parts, int page) {
-    const int64_t p = slot / page;
-    const int o = (int)(slot % page);
-    return which == 0 ? ((p * heads + h) * page + o) * parts + m : ((p * heads + h) * parts + m) * page + o;
-}
-
 struct ReadArgs {
     const int64_t *slots;
     int64_t tokens, pages;
     const void *cb[2];
-    int cb_heads, heads, dim, sub, K, page;
+    int cb_heads, heads, K;
+    int page, page_shift;              // page = 1 << page_shift, or page_shift < 0
+    int chunk;                         // tokens a workgroup takes
     const uint8_t *codes[2];
     void *out[2];
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_cache_read(const ReadArgs a) {
-    const int parts = a.dim / a.sub;
-    const int64_t n = a.tokens * a.heads * parts;
-    const int which = blockIdx.y;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int m = (int)(i % parts), h = (int)(i / parts % a.heads);
-        const int64_t slot = a.slots[i / parts / a.heads];
-        const bool there = slot >= 0 && slot < a.pages * a.page;
-        int code = there ? a.codes[which][code_at(which, slot, h, m, a.heads, parts, a.page)] : 0;
-        code = code < a.K ? code : a.K - 1;
-        const T *cb = static_cast<const T *>(a.cb[which]) + ((a.cb_heads == 1 ? 0 : (int64_t)h * a.K) + code) * a.dim + m * a.sub;
-        T *out = static_cast<T *>(a.out[which]) + i * a.sub;
-        for (int e = 0; e < a.sub; ++e) out[e] = there ? cb[e] : (T)0.0f;
+// Codes -> vectors.  A workgroup holds one head's codebook in LDS (both cache types have 2 bytes a number) and expands `chunk` tokens; a
+// thread writes 16 bytes, 8 numbers of 8 / SUB codewords.  Neighbouring threads read neighbouring parts, so the look-ups
+// never clash in the banks.  Bound by the writes.
+template <int D, int SUB, bool LDS>
+__global__ __launch_bounds__(512) void k_cache_read(const ReadArgs a) {
+    constexpr int M = D / SUB, CH = D / 8, N = 8 / SUB;
+    extern __shared__ __align__(16) uint8_t s_book[];
+    const int h = blockIdx.x, which = blockIdx.z;
+    const uint8_t *book = static_cast<const uint8_t *>(a.cb[which]) + (a.cb_heads == 1 ? 0 : (int64_t)h * a.K * D * 2);
+    if constexpr (LDS) {
+        for (int i = threadIdx.x; i < a.K * CH; i += 512)
+            reinterpret_cast<u32x4 *>(s_book)[i] = reinterpret_cast<const u32x4 *>(book)[i];
+        __syncthreads();
+    }
+    const int64_t begin = (int64_t)blockIdx.y * a.chunk, end = begin + a.chunk < a.tokens ? begin + a.chunk : a.tokens;
+    const int64_t slots = a.pages * a.page;
+    const uint8_t *codes = a.codes[which] + (int64_t)h * a.page * M;
+    uint8_t *out = static_cast<uint8_t *>(a.out[which]);
+    for (int64_t i = begin * CH + threadIdx.x; i < end * CH; i += 512) {
+        const int64_t t = i / CH;
+        const int c = (int)(i % CH);
+        const int64_t slot = a.slots[t];
+        u32x4 v = {0, 0, 0, 0};
+        if (slot >= 0 && slot < slots) {
+            const int64_t p = a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page;
+            const int o = (int)(slot - p * a.page);
+            const uint8_t *q = codes + p * a.heads * a.page * M + (which == 0 ? (int64_t)o * M + c * N : (int64_t)c * N * a.page + o);
+            const int step = which == 0 ? 1 : a.page;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                int code = q[(int64_t)j * step];
+                code = code < a.K ? code : a.K - 1;
+                const uint8_t *w = (LDS ? s_book : book) + code * (D * 2) + c * 16 + j * (SUB * 2);
+                if constexpr (SUB == 8) v = *reinterpret_cast<const u32x4 *>(w);
+                else if constexpr (SUB == 4) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(w);
+                    v[2 * j] = x.x, v[2 * j + 1] = x.y;
+                } else v[j] = *reinterpret_cast<const uint32_t *>(w);
+            }
+        }
+        *reinterpret_cast<u32x4 *>(out + (t * a.heads + h) * (D * 2) + c * 16) = v;
     }
 }
 
-__global__ __launch_bounds__(256) void k_lbg_close(const double *sums, const int64_t *counts, const double *dist, const float *cb_old,
-                                                   int heads, int dim, int sub, int K, float *cb_new, double *mean_dist) {
-    const int parts = dim / sub;
-    const int64_t n = (int64_t)heads * K * dim;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int e = (int)(i % dim), k = (int)(i / dim % K), h = (int)(i / dim / K);
-        const int64_t c = counts[((int64_t)h * parts + e / sub) * K + k];
-        cb_new[i] = c > 0 ? (float)(sums[i] / (double)c) : cb_old[i];
+template <int D, int SUB> hipError_t launch_read(const ReadArgs &a, hipStream_t stream) {
+    // A codebook that a workgroup's tokens outweigh goes to LDS; for a few tokens the look-ups go to the caches instead.
+    const size_t book = (size_t)a.K * D * 2;
+    const dim3 grid(a.heads, (unsigned)((a.tokens + a.chunk - 1) / a.chunk), 2);
+    if (a.chunk >= a.K) {
+        if (book > 48 * 1024) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_cache_read<D, SUB, true>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)book);
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL((k_cache_read<D, SUB, true>), grid, dim3(512), book, stream, a);
+    } else hipLaunchKernelGGL((k_cache_read<D, SUB, false>), grid, dim3(512), 0, stream, a);
+    return hipGetLastError();
+}
+
+template <int D> hipError_t launch_read(const ReadArgs &a, int sub, hipStream_t stream) {
+    return sub == 2 ? launch_read<D, 2>(a, stream) : sub == 4 ? launch_read<D, 4>(a, stream) : launch_read<D, 8>(a, stream);
+}
+
+// The closing half by itself: a workgroup for each head and part, a thread for each codeword.
+__global__ __launch_bounds__(256) void k_lbg_close(const double *sums, const int64_t *counts, const double *dist, const float *cb_old, int dim,
+                                                   int sub, int K, float *cb_new, double *mean_dist) {
+    __shared__ int64_t s_n[256];
+    const int parts = dim / sub, h = blockIdx.x / parts, m = blockIdx.x % parts, k = threadIdx.x;
+    const int64_t n = k < K ? counts[(int64_t)blockIdx.x * K + k] : 0;
+    s_n[k] = n;
+    __syncthreads();
+    for (int o = 128; o; o >>= 1) {
+        if (k < o) s_n[k] += s_n[k + o];
+        __syncthreads();
     }
-    for (int g = blockIdx.x * 256 + threadIdx.x; g < heads * parts; g += gridDim.x * 256) {
-        int64_t c = 0;
-        for (int k = 0; k < K; ++k) c += counts[(int64_t)g * K + k];
-        mean_dist[g] = c > 0 ? dist[g] / (double)c : 0.0;
-    }
+    if (k == 0) mean_dist[blockIdx.x] = s_n[0] > 0 ? dist[blockIdx.x] / (double)s_n[0] : 0.0;
+    if (k >= K) return;
+    const int64_t at = ((int64_t)h * K + k) * dim + m * sub;
+    for (int e = 0; e < sub; ++e) cb_new[at + e] = n > 0 ? (float)(sums[at + e] / (double)n) : cb_old[at + e];
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -150,6 +193,32 @@ Attention plan_attention(int64_t rows, int q_heads, int heads, int dim, int sub,
     return r;
 }
 
+int lbg(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens, const float *cb, int sub, int dtype, const LbgOut &out,
+        void *ws, size_t ws_bytes, void *stream) {
+    const int heads = out.heads, dim = out.dim, K = out.K;
+    int rc = check_shape(heads, dim, sub, K);
+    if (rc) return rc;
+    if (dtype != VQ_F32 && dtype != VQ_BF16 && dtype != VQ_F16) return fail(VQ_E_UNSUPPORTED, "dtype=%d", dtype);
+    if (tokens < 1) return fail(VQ_E_INVALID, "need tokens >= 1");
+    if (tokens > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "tokens below 2^31");
+    if (!cb || !out.counts || !out.dist) return fail(VQ_E_INVALID, "null pointer");
+    if ((uintptr_t)cb & 15) return fail(VQ_E_INVALID, "the codebook must start at a multiple of 16 bytes");
+    if ((rc = check_vectors("x", x, token_stride, head_stride, dtype == VQ_F32 ? 4 : 2))) return rc;
+    const size_t need = vq_cache_lbg_ws_bytes(tokens, heads, dim, sub, K);
+    if (!ws || ws_bytes < need) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, need);
+    if ((uintptr_t)ws & 15) return fail(VQ_E_INVALID, "the workspace must start at a multiple of 16 bytes");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const SearchPlan p = vq_internal_search_plan(tokens, heads, dim, sub, 1);
+    double *part_dist = static_cast<double *>(ws);
+    float *part_sums = reinterpret_cast<float *>(part_dist + (int64_t)p.chunks * heads * (dim / sub));
+    const SearchArgs a = {{x, x}, {token_stride, token_stride}, {head_stride, head_stride}, {cb, cb}, tokens, heads, heads, dim, K, p.pw, p.chunk,
+                          nullptr, 0, 0, 0, nullptr, nullptr, part_sums, part_dist};
+    hipError_t e = vq_internal_search(a, sub, dtype, true, p.blocks, st);
+    if (e == hipSuccess) e = vq_internal_lbg_gather(a, sub, p.chunks, out, st);
+    if (e != hipSuccess) return fail(VQ_E_HIP, "launch of k_cache_search failed: %s", hipGetErrorString(e));
+    return VQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -184,16 +253,28 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
     if ((rc = check_cache(k_codes, v_codes, k_cb, v_cb, cb_heads, heads, pages, page, dtype))) return rc;
     if (tokens < 0) return fail(VQ_E_INVALID, "need tokens >= 0");
     if (tokens > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "tokens below 2^31");
+    if (tokens > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "tokens below 2^31");
     if (tokens == 0) return VQ_OK;
     if (!slots) return fail(VQ_E_INVALID, "null pointer");
     if ((rc = check_vectors("k_out", k_out, dim, dim, 2))) return rc;
     if ((rc = check_vectors("v_out", v_out, dim, dim, 2))) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    ReadArgs a = {slots, tokens, pages, {k_cb, v_cb}, cb_heads, heads, dim, sub, K, page, {k_codes, v_codes}, {k_out, v_out}};
-    const dim3 grid(grid_for(tokens * heads * (dim / sub), 1 << 20), 2);
-    if (dtype == VQ_BF16) hipLaunchKernelGGL(k_cache_read<__bf16>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_cache_read<_Float16>, grid, dim3(256), 0, st, a);
-    LAUNCH_CHECK("k_cache_read");
+    // long reads: two workgroups for each compute unit, of 64 tokens at least
+    int64_t chunk = (tokens * heads * 2 + 511) / 512;
+    chunk = chunk < 64 ? 64 : chunk;
+    if ((tokens + chunk - 1) / chunk > 65535) chunk = (tokens + 65534) / 65535;
+    const ReadArgs a = {slots, tokens, pages, {k_cb, v_cb}, cb_heads, heads, K, page, page & (page - 1) ? -1 : __builtin_ctz(page), (int)chunk,
+                        {k_codes, v_codes}, {k_out, v_out}};
+    hipError_t e;
+    switch (dim) {
+        case 32: e = launch_read<32>(a, sub, st); break;
+        case 64: e = launch_read<64>(a, sub, st); break;
+        case 96: e = launch_read<96>(a, sub, st); break;
+        case 128: e = launch_read<128>(a, sub, st); break;
+        case 192: e = launch_read<192>(a, sub, st); break;
+        default: e = launch_read<256>(a, sub, st); break;
+    }
+    if (e != hipSuccess) return fail(VQ_E_HIP, "launch of k_cache_read failed: %s", hipGetErrorString(e));
     return VQ_OK;
 }
 
@@ -250,27 +331,15 @@ size_t vq_cache_lbg_ws_bytes(int64_t tokens, int heads, int dim, int sub, int K)
 int vq_cache_lbg_accum(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens, const float *cb, int heads, int dim,
                        int sub, int K, int dtype, double *sums, int64_t *counts, double *dist, void *ws, size_t ws_bytes,
                        void *stream) {
-    int rc = check_shape(heads, dim, sub, K);
-    if (rc) return rc;
-    if (dtype != VQ_F32 && dtype != VQ_BF16 && dtype != VQ_F16) return fail(VQ_E_UNSUPPORTED, "dtype=%d", dtype);
-    if (tokens < 1) return fail(VQ_E_INVALID, "need tokens >= 1");
-    if (tokens > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "tokens below 2^31");
-    if (!cb || !sums || !counts || !dist) return fail(VQ_E_INVALID, "null pointer");
-    if ((uintptr_t)cb & 15) return fail(VQ_E_INVALID, "the codebook must start at a multiple of 16 bytes");
-    if ((rc = check_vectors("x", x, token_stride, head_stride, dtype == VQ_F32 ? 4 : 2))) return rc;
-    const size_t need = vq_cache_lbg_ws_bytes(tokens, heads, dim, sub, K);
-    if (!ws || ws_bytes < need) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, need);
-    if ((uintptr_t)ws & 15) return fail(VQ_E_INVALID, "the workspace must start at a multiple of 16 bytes");
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    const SearchPlan p = vq_internal_search_plan(tokens, heads, dim, sub, 1);
-    double *part_dist = static_cast<double *>(ws);
-    float *part_sums = reinterpret_cast<float *>(part_dist + (int64_t)p.chunks * heads * (dim / sub));
-    const SearchArgs a = {{x, x}, {token_stride, token_stride}, {head_stride, head_stride}, {cb, cb}, tokens, heads, heads, dim, K, p.pw, p.chunk,
-                          nullptr, 0, 0, 0, nullptr, nullptr, part_sums, part_dist};
-    hipError_t e = vq_internal_search(a, sub, dtype, true, p.blocks, st);
-    if (e == hipSuccess) e = vq_internal_lbg_gather(a, sub, p.chunks, sums, counts, dist, st);
-    if (e != hipSuccess) return fail(VQ_E_HIP, "launch of k_cache_search failed: %s", hipGetErrorString(e));
-    return VQ_OK;
+    if (!sums) return fail(VQ_E_INVALID, "null pointer");
+    return lbg(x, token_stride, head_stride, tokens, cb, sub, dtype, {heads, dim, K, sums, counts, dist, cb, nullptr}, ws, ws_bytes, stream);
+}
+
+int vq_cache_lbg_iterate(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens, const float *cb, int heads, int dim,
+                         int sub, int K, int dtype, float *cb_new, int64_t *counts, double *mean_dist, void *ws, size_t ws_bytes,
+                         void *stream) {
+    if (!cb_new) return fail(VQ_E_INVALID, "null pointer");
+    return lbg(x, token_stride, head_stride, tokens, cb, sub, dtype, {heads, dim, K, nullptr, counts, mean_dist, cb, cb_new}, ws, ws_bytes, stream);
 }
 
 int vq_cache_lbg_finish(const double *sums, const int64_t *counts, const double *dist, const float *cb_old, int heads, int dim,
@@ -278,8 +347,8 @@ int vq_cache_lbg_finish(const double *sums, const int64_t *counts, const double 
     int rc = check_shape(heads, dim, sub, K);
     if (rc) return rc;
     if (!sums || !counts || !dist || !cb_old || !cb_new || !mean_dist) return fail(VQ_E_INVALID, "null pointer");
-    hipLaunchKernelGGL(k_lbg_close, dim3(grid_for((int64_t)heads * K * dim, 4096)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       sums, counts, dist, cb_old, heads, dim, sub, K, cb_new, mean_dist);
+    hipLaunchKernelGGL(k_lbg_close, dim3(heads * (dim / sub)), dim3(256), 0, static_cast<hipStream_t>(stream), sums, counts, dist, cb_old, dim, sub,
+                       K, cb_new, mean_dist);
     LAUNCH_CHECK("k_lbg_close");
     return VQ_OK;
 }

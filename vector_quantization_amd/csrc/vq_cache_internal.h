@@ -64,7 +64,16 @@ struct SearchPlan {
 // both: 2 where keys and values are searched by one launch
 VQ_HIDDEN SearchPlan vq_internal_search_plan(int64_t tokens, int heads, int dim, int sub, int both);
 VQ_HIDDEN hipError_t vq_internal_search(const SearchArgs &a, int sub, int dtype, bool train, int blocks, hipStream_t stream);
-VQ_HIDDEN hipError_t vq_internal_lbg_gather(const SearchArgs &a, int sub, int chunks, double *sums, int64_t *counts, double *dist, hipStream_t stream);
+// What an LBG iteration leaves: sums and dist, or, where cb_new is given, the new codebook and the mean distance.
+struct LbgOut {
+    int heads, dim, K;
+    double *sums;
+    int64_t *counts;
+    double *dist;
+    const float *cb_old;
+    float *cb_new;
+};
+VQ_HIDDEN hipError_t vq_internal_lbg_gather(const SearchArgs &a, int sub, int chunks, const LbgOut &out, hipStream_t stream);
 
 // How an attention call is laid out: RB * 16 rows to a workgroup of NW waves.
 struct AttendPlan {

@@ -319,23 +319,52 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
     }
 }
 
-// Adds the chunks' sums, in fp64 and in their order: a workgroup for each head and part, a thread for each codeword.
-__global__ __launch_bounds__(256) void k_lbg_gather(const float *part_sums, const double *part_dist, int chunks, int heads, int dim, int sub, int K,
-                                                    double *sums, int64_t *counts, double *dist) {
-    const int parts = dim / sub, h = blockIdx.x / parts, m = blockIdx.x % parts, k = threadIdx.x;
-    const int64_t groups = (int64_t)heads * parts;
-    for (int e = 0; e <= sub; ++e) {
-        double s = 0.0;
-        for (int c = 0; c < chunks; ++c) s += (double)part_sums[((c * groups + blockIdx.x) * (sub + 1) + e) * 256 + k];
-        if (k >= K) continue;
-        if (e < sub) sums[((int64_t)h * K + k) * dim + m * sub + e] = s / (double)SUM_SCALE;
-        else counts[(int64_t)blockIdx.x * K + k] = (int64_t)s;
+// Adds the chunks' sums, in fp64 and in a fixed order: a workgroup for each head and part, four threads for each codeword, each of
+// them a quarter of the chunks.  Reads (sub + 1) KB a chunk once; with `closing` it also divides, and the sums are not stored.
+constexpr int GATHER_SIDE = 4;
+template <int SUB>
+__global__ __launch_bounds__(256 * GATHER_SIDE) void k_lbg_gather(const float *__restrict__ part_sums, const double *__restrict__ part_dist, int chunks,
+                                                                  const LbgOut out) {
+    __shared__ double s_sum[GATHER_SIDE - 1][SUB + 1][256], s_away[256 * GATHER_SIDE], s_n[256 * GATHER_SIDE];
+    const int parts = out.dim / SUB, h = blockIdx.x / parts, m = blockIdx.x % parts;
+    const int k = threadIdx.x & 255, side = threadIdx.x >> 8;
+    const int64_t groups = (int64_t)out.heads * parts;
+    double sum[SUB + 1];
+#pragma unroll
+    for (int e = 0; e <= SUB; ++e) sum[e] = 0.0;
+#pragma unroll 4
+    for (int c = side; c < chunks; c += GATHER_SIDE) {
+        const float *p = part_sums + (c * groups + blockIdx.x) * ((SUB + 1) * 256) + k;
+#pragma unroll
+        for (int e = 0; e <= SUB; ++e) sum[e] += (double)p[e * 256];
     }
-    if (k == 0) {
-        double d = 0.0;
-        for (int c = 0; c < chunks; ++c) d += part_dist[c * groups + blockIdx.x];
-        dist[blockIdx.x] = d;
+    double away = 0.0;
+    for (int c = threadIdx.x; c < chunks; c += 256 * GATHER_SIDE) away += part_dist[c * groups + blockIdx.x];
+    s_away[threadIdx.x] = away;
+    s_n[threadIdx.x] = sum[SUB];                                          // every vector that counts is a member of one codeword
+    if (side > 0)
+#pragma unroll
+        for (int e = 0; e <= SUB; ++e) s_sum[side - 1][e][k] = sum[e];
+    __syncthreads();
+    for (int o = 128 * GATHER_SIDE; o; o >>= 1) {
+        if ((int)threadIdx.x < o) s_away[threadIdx.x] += s_away[threadIdx.x + o], s_n[threadIdx.x] += s_n[threadIdx.x + o];
+        __syncthreads();
     }
+    if (side > 0) return;
+#pragma unroll
+    for (int e = 0; e <= SUB; ++e)
+        for (int x = 0; x < GATHER_SIDE - 1; ++x) sum[e] += s_sum[x][e][k];
+    if (k < out.K) {
+        const int64_t at = ((int64_t)h * out.K + k) * out.dim + m * SUB;
+        out.counts[(int64_t)blockIdx.x * out.K + k] = (int64_t)sum[SUB];
+#pragma unroll
+        for (int e = 0; e < SUB; ++e) {
+            const double s = sum[e] * (1.0 / (double)SUM_SCALE);
+            if (out.cb_new) out.cb_new[at + e] = sum[SUB] > 0.0 ? (float)(s / sum[SUB]) : out.cb_old[at + e];
+            else out.sums[at + e] = s;
+        }
+    }
+    if (k == 0) out.dist[blockIdx.x] = out.cb_new ? (s_n[0] > 0.0 ? s_away[0] / s_n[0] : 0.0) : s_away[0];
 }
 
 template <typename T, typename C, int SUB, bool TRAIN>
@@ -362,7 +391,10 @@ SearchPlan vq_internal_search_plan(int64_t tokens, int heads, int dim, int sub, 
     p.pw = parts % 8 ? 4 : 8;
     const int64_t side = SEARCH_WAVES / p.pw;                             // token ranges side by side in one workgroup
     const int64_t base = (int64_t)heads * (parts / p.pw) * both;
-    const int64_t most = (tokens + 32 * side - 1) / (32 * side), least = (tokens + 4096 * side - 1) / (4096 * side);
+    // A write is spread as thinly as there are tokens; a training chunk of fewer than 128 costs more to gather than it saves.  No
+    // chunk is longer than 4096: its sums are fp32, its counts exact.
+    const int fewest = both == 2 ? 32 : 128;
+    const int64_t most = (tokens + fewest * side - 1) / (fewest * side), least = (tokens + 4096 * side - 1) / (4096 * side);
     int64_t n = (2 * CUS + base - 1) / base;
     n = n < most ? n : most;
     n = n > least ? n : least;
@@ -385,8 +417,10 @@ hipError_t vq_internal_search(const SearchArgs &a, int sub, int dtype, bool trai
     return hipGetLastError();
 }
 
-hipError_t vq_internal_lbg_gather(const SearchArgs &a, int sub, int chunks, double *sums, int64_t *counts, double *dist, hipStream_t stream) {
-    hipLaunchKernelGGL(k_lbg_gather, dim3(a.heads * (a.dim / sub)), dim3(256), 0, stream, a.part_sums, a.part_dist, chunks, a.heads, a.dim, sub, a.K,
-                       sums, counts, dist);
+hipError_t vq_internal_lbg_gather(const SearchArgs &a, int sub, int chunks, const LbgOut &out, hipStream_t stream) {
+    const dim3 grid(a.heads * (a.dim / sub)), block(256 * GATHER_SIDE);
+    if (sub == 2) hipLaunchKernelGGL(k_lbg_gather<2>, grid, block, 0, stream, a.part_sums, a.part_dist, chunks, out);
+    else if (sub == 4) hipLaunchKernelGGL(k_lbg_gather<4>, grid, block, 0, stream, a.part_sums, a.part_dist, chunks, out);
+    else hipLaunchKernelGGL(k_lbg_gather<8>, grid, block, 0, stream, a.part_sums, a.part_dist, chunks, out);
     return hipGetLastError();
 }
