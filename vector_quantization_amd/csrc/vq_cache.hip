@@ -4,10 +4,6 @@
 
 #include "vq_cache_internal.h"
 
-#ifndef VQ_RB
-#define VQ_RB 4
-#define VQ_NW 4
-#endif
 
 namespace {
 
@@ -163,33 +159,41 @@ int grid_for(int64_t items, int64_t most) {
 
 int64_t clamp_hint(int64_t n) { return n > 0x7fffffff ? 0x7fffffff : n; }
 
-// How many rows a workgroup takes, and into how many pieces the context is cut.  Host arithmetic on sizes alone.
+// How many rows a workgroup takes at a time and how many workgroups a head gets.  Host arithmetic on sizes alone.
 struct Attention {
     AttendPlan p;
-    int64_t row_tiles;
-    int splits, split_tiles;
-    size_t ws;
+    int parts, join_at, join_rows;
+    size_t slots, ws;
 };
+// The least that a workgroup is given: under two tiles a wave, staging and joining outweigh what is shared out.
+constexpr int LEAST_TILES = 16;
 
-Attention plan_attention(int64_t rows, int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q, int64_t max_kv) {
+Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q, int64_t max_kv) {
     constexpr int CUS = 256;
     Attention r;
     const int Kp = rows_padded(K), group = q_heads / heads;
     const int64_t per_seq = max_q * group;
-    r.p.rb = per_seq <= 16 ? 1 : dim >= 192 ? 2 : VQ_RB;
-    r.p.nw = r.p.rb == 1 ? 8 : dim >= 192 ? 4 : VQ_NW;
-    r.p.values_in_lds = values_in_lds(Kp, dim, sub);
-    const size_t tables = key_bytes(Kp, dim, sub) + (r.p.values_in_lds ? (size_t)Kp * dim * 2 : 0), join = join_bytes(r.p.nw, r.p.rb, dim);
-    r.p.lds = tables > join ? tables : join;
-    r.row_tiles = (per_seq + r.p.rb * 16 - 1) / (r.p.rb * 16);
-    const int64_t base = r.row_tiles * heads * seqs, tiles = (max_kv + TILE - 1) / TILE;
-    int64_t splits = (2 * CUS + base - 1) / base;
-    const int64_t most = (tiles + 2 * r.p.nw - 1) / (2 * r.p.nw);
-    splits = splits < most ? splits : most;
-    splits = splits < 1 ? 1 : splits > 256 ? 256 : splits;
-    r.split_tiles = (int)((tiles + splits - 1) / splits);
-    r.splits = (int)((tiles + r.split_tiles - 1) / r.split_tiles);
-    r.ws = r.splits > 1 ? (size_t)r.splits * rows * q_heads * (dim * 4 + 8) : 0;
+    // Behind the tables lie the waves' maxima and sums, and at least one wave's rows.  More than 16 rows a sequence go 32 at a time,
+    // so that a look-up serves twice the products, unless the value table then no longer fits but would beside 16.
+    const size_t keys = key_bytes(Kp, dim, sub), values = (size_t)Kp * dim * 2, row = (size_t)(dim + 4) * 4;
+    auto waves = [&](int rb) { return rb == 2 && dim >= 192 ? 4 : 8; };
+    auto fits = [&](int rb, size_t tables) { return tables + (size_t)waves(rb) * rb * 16 * 8 + rb * 16 * row <= LDS_MOST; };
+    r.p.rb = per_seq <= 16 ? 1 : fits(2, keys + values) ? 2 : fits(1, keys + values) ? 1 : fits(2, keys) ? 2 : 1;
+    r.p.nw = waves(r.p.rb);
+    r.p.values_in_lds = fits(r.p.rb, keys + values);
+    const int rows = r.p.rb * 16;
+    const size_t ml = (size_t)r.p.nw * rows * 8, tables = keys + (r.p.values_in_lds ? values : 0);
+    const size_t room = (LDS_MOST - tables - ml) / row, most = (size_t)r.p.nw * rows;      // (room >= rows: it fits)
+    r.join_at = (int)tables;
+    r.join_rows = (int)(room < most ? room : most);
+    r.p.lds = tables + ml + r.join_rows * row;
+    const int64_t tiles = (per_seq + rows - 1) / rows * seqs * ((max_kv + TILE - 1) / TILE);      // a head has at most so many, by the caller's word
+    int64_t parts = (CUS + heads - 1) / heads;
+    if (parts * heads > CUS && parts > 1) --parts;
+    parts = parts < tiles / LEAST_TILES ? parts : tiles / LEAST_TILES;
+    r.parts = (int)(parts < 1 ? 1 : parts);
+    r.slots = r.parts > 1 ? (size_t)2 * heads * r.parts : 0;
+    r.ws = r.slots * (rows * ((size_t)dim * 4 + 8)) + r.slots / 2 * sizeof(AttendNote);
     return r;
 }
 
@@ -281,9 +285,9 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
 size_t vq_cache_attention_ws_bytes(int64_t rows, int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q,
                                    int64_t max_kv) {
     if (rows <= 0 || q_heads <= 0 || q_heads > 4096 || seqs <= 0 || max_q < 1 || max_kv < 1 || check_shape(heads, dim, sub, K) ||
-        q_heads % heads || rows > 0x7fffffff)
+        q_heads % heads)
         return 0;
-    return plan_attention(rows, q_heads, heads, dim, sub, K, seqs, clamp_hint(max_q), clamp_hint(max_kv)).ws;
+    return plan_attention(q_heads, heads, dim, sub, K, seqs, clamp_hint(max_q), clamp_hint(max_kv)).ws;
 }
 
 int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t rows, int q_heads, const void *k_cb,
@@ -297,7 +301,8 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
     if (q_heads <= 0 || q_heads % heads) return fail(VQ_E_INVALID, "q_heads=%d: a positive multiple of heads (%d)", q_heads, heads);
     if (q_heads > 4096) return fail(VQ_E_UNSUPPORTED, "q_heads=%d: at most 4096", q_heads);
     if (rows < 0 || seqs < 0 || width < 0) return fail(VQ_E_INVALID, "need rows, seqs and width >= 0");
-    if (rows > 0x7fffffff || (int64_t)width * page > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "rows and width * page below 2^31");
+    if (rows * (q_heads / heads) > 0x3fffffff || (int64_t)width * page > 0x7fffffff)
+        return fail(VQ_E_UNSUPPORTED, "rows * q_heads / heads below 2^30, width * page below 2^31");
     if (max_q < 1 || max_kv < 1) return fail(VQ_E_INVALID, "need max_q and max_kv >= 1");
     if (!(fabs(scale) < 1e38)) return fail(VQ_E_INVALID, "scale must be finite and below 1e38 in size");
     if (rows == 0 || seqs == 0) return VQ_OK;
@@ -307,15 +312,16 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
     if ((rc = check_vectors("out", out, dim, dim, 2))) return rc;
     max_q = clamp_hint(max_q);
     max_kv = clamp_hint(max_kv);
-    const Attention r = plan_attention(rows, q_heads, heads, dim, sub, K, seqs, max_q, max_kv);
+    const Attention r = plan_attention(q_heads, heads, dim, sub, K, seqs, max_q, max_kv);
     if (r.ws > 0 && (!ws || ws_bytes < r.ws)) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, r.ws);
     if (r.ws > 0 && ((uintptr_t)ws & 15)) return fail(VQ_E_INVALID, "the workspace must start at a multiple of 16 bytes");
     float *part_o = static_cast<float *>(ws);
+    float2 *part_ml = reinterpret_cast<float2 *>(part_o + r.slots * r.p.rb * 16 * dim);
     AttendArgs a = {q, q_token_stride, q_head_stride, rows, q_heads, {k_cb, v_cb}, cb_heads, heads, K, rows_padded(K), {k_codes, v_codes}, pages,
-                    page, table, seqs, width, kv_lens, starts, (float)(scale * 1.4426950408889634), out, lse, r.splits, r.split_tiles, part_o,
-                    reinterpret_cast<float2 *>(part_o + (int64_t)r.splits * rows * q_heads * dim)};
-    const int64_t items = r.row_tiles * r.splits;
-    const dim3 grid(heads, (unsigned)(items > 65535 ? 65535 : items), seqs);
+                    page, table, seqs, width, kv_lens, starts, (float)fmax(fabs(scale) * 1.4426950408889634, 1e-37), scale < 0 ? 0x80008000u : 0u,
+                    out, lse, r.parts, LEAST_TILES, r.join_at, r.join_rows, part_o, part_ml,
+                    reinterpret_cast<AttendNote *>(part_ml + r.slots * r.p.rb * 16)};
+    const dim3 grid(heads, r.parts);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const hipError_t e = (dtype == VQ_BF16 ? vq_internal_attend_bf16 : vq_internal_attend_f16)(a, r.p, dim, sub, grid, st);
     if (e != hipSuccess) return fail(VQ_E_HIP, "launch of k_cache_attend failed: %s", hipGetErrorString(e));

@@ -35,12 +35,20 @@ struct AttendArgs {
     const int32_t *table;
     int seqs, width;
     const int32_t *kv_lens, *starts;
-    float scale2;                      // scale * log2(e)
+    float scale2;                      // |scale| * log2(e), above 0: maxima can be taken before it
+    uint32_t flip;                     // the sign bits of two 16-bit numbers where scale < 0: q is negated instead
     void *out;
     float *lse;
-    int splits, split_tiles;           // the context is cut into pieces of split_tiles tiles; the last takes what is left
-    float *part_o;                     // (splits, rows * q_heads, D), against part_ml's maximum
-    float2 *part_ml;                   // (splits, rows * q_heads): maximum (base 2) and sum
+    int parts, least_tiles;            // workgroups a head at most; a workgroup gets least_tiles tiles at least
+    int join_at, join_rows;            // LDS behind the tables: its place, and how many rows' sums fit there
+    float *part_o;                     // (slots, rows of an item, D), against part_ml's maximum; two slots a workgroup
+    float2 *part_ml;                   // (slots, rows of an item): maximum (base 2) and sum
+    struct AttendNote *notes;          // one a workgroup
+};
+
+// An item (tile of rows `tile` of sequence `seq`) whose parts the workgroups up to `last` of a head hold.
+struct AttendNote {
+    int seq, tile, last, unused;
 };
 
 struct SearchArgs {
@@ -102,8 +110,6 @@ __host__ __device__ inline int rows_padded(int K) {
 }
 __host__ __device__ inline int key_stride(int Kp, int SUB) { return (Kp + 1) * SUB * 2; }
 inline size_t key_bytes(int Kp, int D, int SUB) { return ((size_t)(D / SUB) * key_stride(Kp, SUB) + 15) / 16 * 16; }
-inline size_t join_bytes(int NW, int RB, int D) { return (size_t)NW * RB * 16 * (D + 4) * 4 + (size_t)NW * RB * 16 * 8; }
-inline bool values_in_lds(int Kp, int D, int SUB) { return key_bytes(Kp, D, SUB) + (size_t)Kp * D * 2 <= LDS_MOST; }
 
 
 #endif
