@@ -171,7 +171,7 @@ constexpr int LEAST_TILES = 16;
 Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q, int64_t max_kv) {
     constexpr int CUS = 256;
     Attention r;
-    const int Kp = rows_padded(K), group = q_heads / heads;
+    const int Kp = dim <= 128 ? 256 : rows_padded(K), group = q_heads / heads;      // (as k_cache_attend lays out its tables)
     const int64_t per_seq = max_q * group;
     // Behind the tables lie the waves' maxima and sums, and at least one wave's rows.  More than 16 rows a sequence go 32 at a time,
     // so that a look-up serves twice the products, unless the value table then no longer fits but would beside 16.
@@ -187,10 +187,12 @@ Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int se
     r.join_at = (int)tables;
     r.join_rows = (int)(room < most ? room : most);
     r.p.lds = tables + ml + r.join_rows * row;
-    const int64_t tiles = (per_seq + rows - 1) / rows * seqs * ((max_kv + TILE - 1) / TILE);      // a head has at most so many, by the caller's word
+    // a head has at most so many items and tiles, by the caller's word
+    const int64_t items = (per_seq + rows - 1) / rows * seqs, tiles = items * ((max_kv + TILE - 1) / TILE);
+    const int64_t wanted = tiles / LEAST_TILES > items ? tiles / LEAST_TILES : items;
     int64_t parts = (CUS + heads - 1) / heads;
     if (parts * heads > CUS && parts > 1) --parts;
-    parts = parts < tiles / LEAST_TILES ? parts : tiles / LEAST_TILES;
+    parts = parts < wanted ? parts : wanted;
     r.parts = (int)(parts < 1 ? 1 : parts);
     r.slots = r.parts > 1 ? (size_t)2 * heads * r.parts : 0;
     r.ws = r.slots * (rows * ((size_t)dim * 4 + 8)) + r.slots / 2 * sizeof(AttendNote);

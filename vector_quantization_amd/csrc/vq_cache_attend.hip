@@ -52,28 +52,33 @@ __device__ inline void sequence(const AttendArgs &a, int b, int64_t &first, int 
     n_kv = n < 0 ? 0 : (n > most ? (int)most : n);
 }
 
-// NB consecutive bytes from an address that is a multiple of the largest power of two in NB (4 at most).
-template <int NB> __device__ inline void load_bytes(uint32_t *w, const uint8_t *p) {
+// Addresses that come out of registers say that they are global memory's: a flat load would count as an LDS access too, and every
+// wait for a look-up would wait for it.
+#define GLOBAL __attribute__((address_space(1)))
+typedef const GLOBAL uint8_t *global_bytes;
+
+// NB consecutive bytes from an address that is a multiple of the largest power of two in NB (16 at most).
+template <int NB> __device__ inline void load_bytes(uint32_t *w, global_bytes p) {
     if constexpr (NB % 16 == 0) {
 #pragma unroll
         for (int i = 0; i < NB / 16; ++i) {
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(p + 16 * i);
+            const u32x4 v = *(const GLOBAL u32x4 *)(p + 16 * i);
             w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
         }
     } else if constexpr (NB % 8 == 0) {
 #pragma unroll
         for (int i = 0; i < NB / 8; ++i) {
-            const u32x2 v = *reinterpret_cast<const u32x2 *>(p + 8 * i);
+            const u32x2 v = *(const GLOBAL u32x2 *)(p + 8 * i);
             w[2 * i] = v.x, w[2 * i + 1] = v.y;
         }
     } else if constexpr (NB % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < NB / 4; ++i) w[i] = *reinterpret_cast<const uint32_t *>(p + 4 * i);
+        for (int i = 0; i < NB / 4; ++i) w[i] = *(const GLOBAL uint32_t *)(p + 4 * i);
     } else if constexpr (NB % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < (NB + 3) / 4; ++i) {
-            w[i] = *reinterpret_cast<const uint16_t *>(p + 4 * i);
-            if (4 * i + 2 < NB) w[i] |= (uint32_t)*reinterpret_cast<const uint16_t *>(p + 4 * i + 2) << 16;
+            w[i] = *(const GLOBAL uint16_t *)(p + 4 * i);
+            if (4 * i + 2 < NB) w[i] |= (uint32_t)*(const GLOBAL uint16_t *)(p + 4 * i + 2) << 16;
         }
     } else {
         w[0] = 0;
@@ -84,11 +89,36 @@ template <int NB> __device__ inline void load_bytes(uint32_t *w, const uint8_t *
 
 // Look-ups name LDS by its byte offset: the kernel has no other LDS, so s_mem lies at 0, and an address is what the code and
 // the lane make of it without a base to be added each time.
-template <typename V> __device__ inline V lds(uint32_t at) { return *(const __attribute__((address_space(3))) V *)at; }
+template <typename V> __device__ inline V lds(uint32_t at) { return *(const __attribute__((address_space(3))) V *)(uintptr_t)at; }
 
 __device__ inline float wave_any_max(float v) {          // the maximum over the four lanes of one row
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
+}
+
+// A value that every lane holds, in scalar registers: what follows from it stays there.
+__device__ inline int64_t uniform(int64_t v) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
+}
+
+// v of the lane that the DPP control names, 0 where it names none or ROWS leaves this row of 16 lanes out.
+template <int CONTROL, int ROWS> __device__ inline int64_t moved(int64_t v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CONTROL, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CONTROL, ROWS, 0xf, false);
+    return (int64_t)(uint32_t)lo | (int64_t)hi << 32;
+}
+// The sum over the lanes up to this one.
+__device__ inline int64_t running(int64_t v) {
+    v += moved<0x111, 0xf>(v);       // one, two, four and eight lanes to the right inside a row
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);       // the last lane of a row to all of the next, for the second and the fourth
+    v += moved<0x143, 0xc>(v);       // lane 31 to the upper half
+    return v;
+}
+__device__ inline int64_t of_last_lane(int64_t v) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, 63) | (int64_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32;
 }
 
 // 8 numbers of a finished row, place = row * q_heads + head: v against the maximum `most` (base 2) and the sum of weights.
@@ -126,8 +156,10 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x, group = a.q_heads / a.heads;
-    const int Kp = a.Kp, kstride = key_stride(Kp, SUB);
-    const int k_at = VLDS ? Kp * D * 2 : 0;                       // the value table comes first: see look-ups
+    const int Kp = a.Kp;
+    // Up to 128 dims the tables are laid out for 256 codewords whatever K is, so that a look-up's part is an offset in its instruction.
+    const int room = D <= 128 ? 256 : Kp, kstride = key_stride(room, SUB);
+    const int k_at = VLDS ? room * D * 2 : 0;                     // the value table comes first: see look-ups
     const int64_t cb0 = a.cb_heads == 1 ? 0 : (int64_t)h * a.K * D;
     const T *k_cb = static_cast<const T *>(a.cb[0]) + cb0, *v_cb = static_cast<const T *>(a.cb[1]) + cb0;
     const int page16 = a.page >> 4;
@@ -139,28 +171,69 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) v_lane[u] = ((u * 16 + r) * E / SUB) * a.page + 4 * g;
 
-    // this workgroup's range; every wave works it out by itself, 64 sequences at a time
+    // Codebooks -> LDS, 16 bytes at a time, several loads under way at once; rows past K are zeros.  The first loads leave now and
+    // are on their way while the range is worked out.
+    constexpr int BATCH = D <= 128 ? 8 : 4;
+    u32x4 stage_k[BATCH], stage_v[VLDS ? BATCH : 1];
+    auto stage_load = [&](int i0) {
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+            const int i = i0 + x * NW * 64;
+            stage_k[x] = (u32x4){0, 0, 0, 0};
+            if constexpr (VLDS) stage_v[x] = (u32x4){0, 0, 0, 0};
+            if (i < a.K * (D / 8)) {
+                stage_k[x] = *reinterpret_cast<const u32x4 *>(k_cb + (int64_t)i * 8);
+                if constexpr (VLDS) stage_v[x] = *reinterpret_cast<const u32x4 *>(v_cb + (int64_t)i * 8);
+            }
+        }
+    };
+    auto stage_store = [&](int i0) {
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+            const int i = i0 + x * NW * 64, k = i / (D / 8), c = i % (D / 8);
+            if (i >= Kp * (D / 8)) continue;
+            if constexpr (SUB == 8) {
+                *reinterpret_cast<u32x4 *>(s_mem + k_at + c * kstride + k * 16) = stage_k[x];
+            } else if constexpr (SUB == 4) {
+                *reinterpret_cast<u32x2 *>(s_mem + k_at + (2 * c) * kstride + k * 8) = stage_k[x].xy;
+                *reinterpret_cast<u32x2 *>(s_mem + k_at + (2 * c + 1) * kstride + k * 8) = stage_k[x].zw;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t *>(s_mem + k_at + (4 * c + j) * kstride + k * 4) = stage_k[x][j];
+            }
+            if constexpr (VLDS) *reinterpret_cast<u32x4 *>(s_mem + i * 16) = stage_v[x];
+        }
+    };
+    stage_load(threadIdx.x);
+
+    // This workgroup's range.  Every wave works it out by itself: 64 sequences at a time, the tiles of rows of a long one 64 at a time too.
     auto cost_of_sequence = [&](int b) -> int64_t {
-        if (b >= a.seqs) return 0;
-        int64_t first;
-        int n_q, n_kv;
-        sequence(a, b, first, n_q, n_kv);
+        int64_t first = 0, sum = 0;
+        int n_q = 0, n_kv = 0;
+        if (b < a.seqs) sequence(a, b, first, n_q, n_kv);
         const int tiles = (n_q * group + ROWS - 1) / ROWS;
-        int64_t sum = 0;
-        for (int t = 0; t < tiles; ++t) sum += cost_of<RB>(t, n_q, n_kv, group);
+        if (tiles == 1) sum = cost_of<RB>(0, n_q, n_kv, group);
+        for (uint64_t todo = __ballot(tiles > 1); todo; todo &= todo - 1) {
+            const int of = __builtin_ctzll(todo), x_q = __shfl(n_q, of), x_kv = __shfl(n_kv, of), x_tiles = __shfl(tiles, of);
+            int64_t part = 0;
+            for (int t = lane; t < x_tiles; t += 64) part += cost_of<RB>(t, x_q, x_kv, group);
+            part = of_last_lane(running(part));
+            if (lane == of) sum = part;
+        }
         return sum;
     };
-    auto running = [&](int64_t v) -> int64_t {                    // sum over the lanes up to this one
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t up = __shfl_up(v, o);
-            if (lane >= o) v += up;
-        }
-        return v;
-    };
     const int64_t mine = cost_of_sequence(lane);
-    int64_t all = __shfl(running(mine), 63);
-    for (int b0 = 64; b0 < a.seqs; b0 += 64) all += __shfl(running(cost_of_sequence(b0 + lane)), 63);
-    int64_t parts = all / a.least_tiles;
+    int64_t all = of_last_lane(running(mine));
+    for (int b0 = 64; b0 < a.seqs; b0 += 64) all += of_last_lane(running(cost_of_sequence(b0 + lane)));
+    // (a workgroup for every item at least, as far as they go: an item has costs of its own)
+    int64_t items = 0;
+    for (int b0 = 0; b0 < a.seqs; b0 += 64) {
+        int64_t first = 0;
+        int n_q = 0, n_kv = 0;
+        if (b0 + lane < a.seqs) sequence(a, b0 + lane, first, n_q, n_kv);
+        items += of_last_lane(running((n_q * group + ROWS - 1) / ROWS));
+    }
+    int64_t parts = all / a.least_tiles > items ? all / a.least_tiles : items;
     parts = parts < 1 ? 1 : parts > (int64_t)gridDim.y ? (int64_t)gridDim.y : parts;
     const int me = h * gridDim.y + blockIdx.y;
     const int64_t begin = all * blockIdx.y / parts, past = all * (blockIdx.y + 1) / parts;
@@ -168,50 +241,37 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
         if (a.parts > 1 && threadIdx.x == 0) a.notes[me] = AttendNote{-1, 0, 0, 0};
         return;
     }
-    int b = 0;
-    int64_t skip = begin;                                         // tiles of the work before the range, from sequence b on
+    int64_t skip = begin;                                         // first: of the work before sequence b; then of item (b, tile)
+    auto locate = [&](int64_t sum, int &at) -> bool {             // sum: the lanes' running costs; finds the lane that skip falls to
+        const bool here = skip < of_last_lane(sum);
+        at = here ? __builtin_ctzll(__ballot(sum > skip)) : 64;
+        skip -= at > 0 ? uniform(__shfl(sum, at - 1)) : 0;
+        return here;
+    };
+    int b = 0, tile = 0, at;
     for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-        const int64_t sum = running(b0 == 0 ? mine : cost_of_sequence(b0 + lane)), whole = __shfl(sum, 63);
-        if (skip < whole) {
-            const int at = __builtin_ctzll(__ballot(sum > skip));
-            b = b0 + at;
-            if (at > 0) skip -= __shfl(sum, at - 1);
-            break;
-        }
-        skip -= whole;
+        const bool here = locate(running(b0 == 0 ? mine : cost_of_sequence(b0 + lane)), at);
+        b = b0 + at;
+        if (here) break;
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    int tile = 0;
+    {
+        int64_t first;
+        int n_q, n_kv;
+        sequence(a, b < a.seqs ? b : 0, first, n_q, n_kv);
+        const int tiles = (n_q * group + ROWS - 1) / ROWS;
+        for (int t0 = 0; t0 < tiles; t0 += 64) {
+            const int t = t0 + lane;
+            const bool here = locate(running(t < tiles ? cost_of<RB>(t, n_q, n_kv, group) : 0), at);
+            tile = t0 + at;
+            if (here) break;
+        }
+    }
     int64_t left = past - begin, now = begin - skip;              // now: where item (b, tile) begins
 
-    // codebooks -> LDS, 16 bytes at a time, several loads under way at once; rows past K are zeros
-    constexpr int BATCH = 4;
-    for (int i0 = threadIdx.x; i0 < Kp * (D / 8); i0 += BATCH * NW * 64) {
-        u32x4 kv[BATCH], vv[BATCH];
-#pragma unroll
-        for (int x = 0; x < BATCH; ++x) {
-            const int i = i0 + x * NW * 64;
-            kv[x] = vv[x] = (u32x4){0, 0, 0, 0};
-            if (i < a.K * (D / 8)) {
-                kv[x] = *reinterpret_cast<const u32x4 *>(k_cb + (int64_t)i * 8);
-                if constexpr (VLDS) vv[x] = *reinterpret_cast<const u32x4 *>(v_cb + (int64_t)i * 8);
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < BATCH; ++x) {
-            const int i = i0 + x * NW * 64, k = i / (D / 8), c = i % (D / 8);
-            if (i >= Kp * (D / 8)) continue;
-            if constexpr (SUB == 8) {
-                *reinterpret_cast<u32x4 *>(s_mem + k_at + c * kstride + k * 16) = kv[x];
-            } else if constexpr (SUB == 4) {
-                *reinterpret_cast<u32x2 *>(s_mem + k_at + (2 * c) * kstride + k * 8) = kv[x].xy;
-                *reinterpret_cast<u32x2 *>(s_mem + k_at + (2 * c + 1) * kstride + k * 8) = kv[x].zw;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t *>(s_mem + k_at + (4 * c + j) * kstride + k * 4) = kv[x][j];
-            }
-            if constexpr (VLDS) *reinterpret_cast<u32x4 *>(s_mem + i * 16) = vv[x];
-        }
+    stage_store(threadIdx.x);
+    for (int i0 = threadIdx.x + BATCH * NW * 64; i0 < Kp * (D / 8); i0 += BATCH * NW * 64) {
+        stage_load(i0);
+        stage_store(i0);
     }
     __syncthreads();
 
@@ -227,12 +287,6 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
             continue;
         }
         const int tiles = tiles_of<RB>(tile, n_q, n_kv, group), cost = tiles < 1 ? 1 : tiles;
-        if (skip >= cost) {
-            skip -= cost;
-            now += cost;
-            ++tile;
-            continue;
-        }
         const int take = (int)(left < cost - skip ? left : cost - skip);
         const int lo = (int)skip < tiles ? (int)skip : tiles, hi = (int)skip + take < tiles ? (int)skip + take : tiles;
         const bool whole_item = take == cost;
@@ -261,115 +315,104 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
                 for (int e = 0; e < E; ++e) o[rb][u][e] = (f32x4){0, 0, 0, 0};
         }
 
-        // A wave's tiles: lo + wave, then every NW-th.  Codes are fetched AHEAD tiles before their use, page numbers one tile before their codes.
-        // Loads come back in the order of their issue, so a turn asks for page numbers first: the next turn's wait
-        // for them then leaves this turn's codes under way.
+        // A wave's tiles: lo + wave, then every NW-th.  Where their codes lie is worked out for 32 tiles at a time, a lane for each half of a
+        // tile (16 tokens, inside one page); a turn then takes its four addresses out of the lanes.  (Page numbers fetched and
+        // multiplied out turn by turn took longer than all the rest: a wave waits for every scalar step.)
+        // Codes are fetched AHEAD tiles before their use.
         constexpr int AHEAD = 2;
-        int t = lo + wave;
-        int pi = 2 * t / page16, off = 2 * t % page16, tp = t;   // page and 16-token group of the next page numbers to be fetched, and their tile
-        const int step_p = 2 * NW / page16, step_o = 2 * NW % page16;
-        int raw[2][2], at16[2][2], pages_of[AHEAD][2];           // page numbers and groups in two sets, taken in turn; a group < 0 is not there
-        uint32_t kc[AHEAD][2][KW], vc[AHEAD][2][U];
-        auto fetch_pages = [&](int set) {
+        int t = lo + wave, fetched = 0;                           // the tile in hand; how many have been fetched
+        uint64_t k_ptr = 0, v_ptr = 0, there = 0;                 // a lane's addresses; one bit a lane: its tokens lie in a page of the cache
+        auto place = [&]() {
+            const int tile32 = lo + wave + (fetched + (lane & 31)) * NW, group16 = 2 * tile32 + (lane >> 5);
+            const int at = group16 / page16, y = group16 - at * page16;
+            const bool in = tile32 < hi && group16 * 16 < n_kv;
+            const int n = in ? table[at] : -1;
+            const bool good = n >= 0 && n < a.pages;
+            const int64_t from = good ? (int64_t)n * page_bytes + head_at : head_at;      // (else page 0: read, not looked at)
+            k_ptr = (uint64_t)(a.codes[0] + (from + (int64_t)(good ? y : 0) * 16 * M));
+            v_ptr = (uint64_t)(a.codes[1] + (from + (good ? y : 0) * 16));
+            there = __ballot(good);
+        };
+        auto of_lane = [](uint64_t v, int from) -> global_bytes {
+            return (global_bytes)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, from) |
+                                  (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), from) << 32);
+        };
+        uint32_t kc[AHEAD][2][KW], vc[AHEAD][2][U], seen[AHEAD];   // seen: bits 0 and 1: the tile's halves are there
+        auto fetch = [&](int slot) {
+            const int at = fetched & 31;
+            if (at == 0) place();
+            seen[slot] = (uint32_t)(there >> at) & 1u | ((uint32_t)(there >> (32 + at)) & 1u) << 1;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                int x = pi, y = off + s;
-                if (y >= page16) x += 1, y = 0;
-                const bool in = tp * TILE + 16 * s < n_kv && tp < hi;
-                raw[set][s] = table[in ? x : 0];
-                at16[set][s] = in ? y : -1;
-            }
-            pi += step_p;
-            off += step_o;
-            tp += NW;
-            if (off >= page16) pi += 1, off -= page16;
-        };
-        auto fetch = [&](int slot, int set) {
-            fetch_pages(1 - set);
+                load_bytes<NB>(kc[slot][s], of_lane(k_ptr, 32 * s + at) + k_lane);
+                const global_bytes from = of_lane(v_ptr, 32 * s + at);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int n = __builtin_amdgcn_readfirstlane(raw[set][s]), y = __builtin_amdgcn_readfirstlane(at16[set][s]);
-                const bool there = y >= 0 && n >= 0 && n < a.pages;
-                const int group16 = there ? y * 16 : 0;
-                const int64_t base = (there ? n : 0) * page_bytes + head_at;
-                pages_of[slot][s] = there ? n : -1;
-                const uint8_t *k_from = a.codes[0] + (base + group16 * M), *v_from = a.codes[1] + (base + group16);
-                load_bytes<NB>(kc[slot][s], k_from + k_lane);
-#pragma unroll
-                for (int u = 0; u < U; ++u) vc[slot][s][u] = *reinterpret_cast<const uint32_t *>(v_from + v_lane[u]);
+                for (int u = 0; u < U; ++u) vc[slot][s][u] = *(const GLOBAL uint32_t *)(from + v_lane[u]);
             }
+            ++fetched;
         };
-        static_assert(AHEAD == 2, "a turn's slot of codes is also its set of page numbers");
+        static_assert(AHEAD == 2, "turns go by twos");
         if (t < hi) {
-            fetch_pages(0);
-            fetch(0, 0);
-            fetch(1, 1);
+            fetch(0);
+            fetch(1);
         }
-        auto turn = [&](int slot) {
-            uint32_t k_now[2][KW], v_now[2][U];
-            const int pg_now[2] = {pages_of[slot][0], pages_of[slot][1]};
+        // Look-ups.  Up to 128 dims all of a tile's go first, so that they pass through LDS one behind the other; beyond, registers are
+        // short and they go one step before their use.  Either way the tile's codes are done with before the next ones are fetched to
+        // their registers: where old and new are both alive, the new ones are copied, and a copy waits for its load.
+        constexpr bool FIRST = D <= 128;
+        auto look_k = [&](uint32_t const (&codes)[KW], int ks) -> u32x4 {
+            u32x4 x;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-#pragma unroll
-                for (int i = 0; i < KW; ++i) k_now[s][i] = kc[slot][s][i] & fold;
-#pragma unroll
-                for (int u = 0; u < U; ++u) v_now[s][u] = vc[slot][s][u] & fold;
+            for (int j = 0; j < 8 / SUB; ++j) {
+                const int n = ks * (8 / SUB) + j;                // the lane's n-th part, g * NB + n of the vector
+                const uint32_t code = ((codes[n / 4] & fold) >> (8 * (n % 4))) & 255u;
+                const uint32_t at = k_at + g * NB * kstride + n * kstride + code * (SUB * 2);
+                if constexpr (SUB == 8) x = lds<u32x4>(at);
+                else if constexpr (SUB == 4) {
+                    const u32x2 v = lds<u32x2>(at);
+                    x[2 * j] = v.x, x[2 * j + 1] = v.y;
+                } else x[j] = lds<uint32_t>(at);
             }
-            fetch(slot, slot);                                   // (past the end: page 0, not looked at)
-            // Look-ups.  With few waves all of a tile's go first, so that they pass through LDS one behind the other; with many, the waves
-            // hide each other's and registers count for more.
-            constexpr bool FIRST = NW <= 8 && D <= 128;
-            auto look_k = [&](int s, int ks) -> u32x4 {
-                u32x4 x;
+            return x;
+        };
+        auto look_v = [&](uint32_t c0, uint32_t c1, int u, uint32_t (&x)[8][E / 2]) {
+            const uint32_t codes[2] = {c0 & fold, c1 & fold};
 #pragma unroll
-                for (int j = 0; j < 8 / SUB; ++j) {
-                    const int n = ks * (8 / SUB) + j;            // the lane's n-th part, g * NB + n of the vector
-                    const uint32_t code = (k_now[s][n / 4] >> (8 * (n % 4))) & 255u;
-                    const uint32_t at = k_at + g * NB * kstride + n * kstride + code * (SUB * 2);
-                    if constexpr (SUB == 8) x = lds<u32x4>(at);
-                    else if constexpr (SUB == 4) {
-                        const u32x2 v = lds<u32x2>(at);
-                        x[2 * j] = v.x, x[2 * j + 1] = v.y;
-                    } else x[j] = lds<uint32_t>(at);
+            for (int j = 0; j < 8; ++j) {
+                uint32_t at;
+                if constexpr (VLDS && D == 128) {
+                    // a row has 256 bytes: the code is the second byte of the address, put there with the first in one go
+                    at = __builtin_amdgcn_perm(codes[j / 4], (uint32_t)(r * E * 2), 0x0c0c0000u | (4u + j % 4) << 8);
+                } else {
+                    uint32_t code = (codes[j / 4] >> (8 * (j % 4))) & 255u;
+                    if constexpr (!VLDS) code = code < (uint32_t)a.K ? code : (uint32_t)a.K - 1;
+                    at = code * (D * 2) + r * E * 2;
                 }
-                return x;
-            };
-            auto look_v = [&](int u, uint32_t (&x)[8][E / 2]) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t at;
-                    if constexpr (VLDS && D == 128) {
-                        // a row has 256 bytes: the code is the second byte of the address, put there with the first in one go
-                        at = __builtin_amdgcn_perm(v_now[j / 4][u], (uint32_t)(r * E * 2), 0x0c0c0000u | (4u + j % 4) << 8);
-                    } else {
-                        uint32_t code = (v_now[j / 4][u] >> (8 * (j % 4))) & 255u;
-                        if constexpr (!VLDS) code = code < (uint32_t)a.K ? code : (uint32_t)a.K - 1;
-                        at = code * (D * 2) + r * E * 2;
-                    }
-                    at += u * 16 * E * 2;
-                    const uint8_t *from = reinterpret_cast<const uint8_t *>(v_cb) + (VLDS ? 0 : at);
-                    if constexpr (E == 8) {
-                        const u32x4 v = VLDS ? lds<u32x4>(at) : *reinterpret_cast<const u32x4 *>(from);
-                        x[j][0] = v.x, x[j][1] = v.y, x[j][2] = v.z, x[j][3] = v.w;
-                    } else if constexpr (E == 4) {
-                        const u32x2 v = VLDS ? lds<u32x2>(at) : *reinterpret_cast<const u32x2 *>(from);
-                        x[j][0] = v.x, x[j][1] = v.y;
-                    } else x[j][0] = VLDS ? lds<uint32_t>(at) : *reinterpret_cast<const uint32_t *>(from);
-                }
-            };
+                at += u * 16 * E * 2;
+                const uint8_t *from = reinterpret_cast<const uint8_t *>(v_cb) + (VLDS ? 0 : at);
+                if constexpr (E == 8) {
+                    const u32x4 v = VLDS ? lds<u32x4>(at) : *reinterpret_cast<const u32x4 *>(from);
+                    x[j][0] = v.x, x[j][1] = v.y, x[j][2] = v.z, x[j][3] = v.w;
+                } else if constexpr (E == 4) {
+                    const u32x2 v = VLDS ? lds<u32x2>(at) : *reinterpret_cast<const u32x2 *>(from);
+                    x[j][0] = v.x, x[j][1] = v.y;
+                } else x[j][0] = VLDS ? lds<uint32_t>(at) : *reinterpret_cast<const uint32_t *>(from);
+            }
+        };
+        auto turn = [&](int slot) {
             f32x4 z[RB][2];
             uint32_t vx[FIRST ? U : 1][8][E / 2];
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) z[rb][0] = z[rb][1] = (f32x4){0, 0, 0, 0};
+            const uint32_t have = seen[slot];
             if constexpr (FIRST) {
                 u32x4 kx[2][KS];
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+                for (int ks = 0; ks < KS; ++ks) kx[0][ks] = look_k(kc[slot][0], ks), kx[1][ks] = look_k(kc[slot][1], ks);
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) kx[s][ks] = look_k(s, ks);
-#pragma unroll
-                for (int u = 0; u < U; ++u) look_v(u, vx[u]);
+                for (int u = 0; u < U; ++u) look_v(vc[slot][0][u], vc[slot][1][u], u, vx[u]);
                 __builtin_amdgcn_sched_barrier(0);
+                fetch(slot);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -381,14 +424,14 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        const u32x4 x = look_k(s, ks);
+                        const u32x4 x = look_k(kc[slot][s], ks);
 #pragma unroll
                         for (int rb = 0; rb < RB; ++rb) z[rb][s] = mfma16<T>(x, q[rb][ks], z[rb][s]);
                     }
             }
             // weights
             u32x4 w[RB];
-            const bool whole = pg_now[0] >= 0 && pg_now[1] >= 0 && t * TILE + TILE - 1 <= all_see;
+            const bool whole = have == 3 && t * TILE + TILE - 1 <= all_see;
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 if (!whole) {
@@ -396,7 +439,7 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
                     for (int s = 0; s < 2; ++s)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (pg_now[s] < 0 || t * TILE + 16 * s + 4 * g + i > sees[rb]) z[rb][s][i] = -INFINITY;
+                            if (!(have >> s & 1) || t * TILE + 16 * s + 4 * g + i > sees[rb]) z[rb][s][i] = -INFINITY;
                 }
                 float best = -INFINITY;
 #pragma unroll
@@ -427,7 +470,7 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 uint32_t(&x)[8][E / 2] = vx[FIRST ? u : 0];
-                if constexpr (!FIRST) look_v(u, x);
+                if constexpr (!FIRST) look_v(vc[slot][0][u], vc[slot][1][u], u, x);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     u32x4 v;
@@ -438,16 +481,20 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
                     for (int rb = 0; rb < RB; ++rb) o[rb][u][e] = mfma16<T>(v, w[rb], o[rb][u][e]);
                 }
             }
+            if constexpr (!FIRST) {
+                __builtin_amdgcn_sched_barrier(0);
+                fetch(slot);
+            }
             t += NW;
         };
         __builtin_amdgcn_s_waitcnt(0x0f70);                       // all loads: inside the loop no wait is left but those of the codes
-        while (t < hi) {
-            turn(0);
-            if (t >= hi) break;
+        while (t + NW < hi) {                                     // (left in one place only: leaving after the first turn as well would make
+            turn(0);                                              // every wait for its codes one for all loads)
             turn(1);
         }
+        if (t < hi) turn(0);
 
-        // Join the waves: maxima and sums first, then every wave's part against the common maximum, added in the waves' order, as many
+        // Join the waves: maxima and sums first, then every wave's part weighted by its maximum, added in the waves' order, as many
         // waves at a time as LDS has room for beside the tables.
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
@@ -459,19 +506,9 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
         if (g == 0)
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) s_ml[wave * ROWS + rb * 16 + r] = make_float2(top[rb], total[rb]);
-        __syncthreads();
-        float keep[RB];
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            float most = -INFINITY;
-#pragma unroll 4
-            for (int x = 0; x < NW; ++x) most = fmaxf(most, s_ml[x * ROWS + rb * 16 + r].x);
-            keep[rb] = top[rb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[rb] - most);
-        }
         constexpr int EACH = (ROWS * (D / 8) + NW * 64 - 1) / (NW * 64);       // pieces of 8 numbers a thread adds up
         f32x4 v0[EACH], v1[EACH];
-#pragma unroll
-        for (int n = 0; n < EACH; ++n) v0[n] = v1[n] = (f32x4){0, 0, 0, 0};
+        float weight[EACH][NW], most[EACH], sum[EACH];
         const int at_once = a.join_rows / rows_here;
         for (int w0 = 0; w0 < NW; w0 += at_once) {
             if (wave >= w0 && wave < w0 + at_once)
@@ -484,42 +521,50 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                                for (int e = 0; e < E; ++e) p[(u * 16 + 4 * g + i) * E + e] = o[rb][u][e][i] * keep[rb];
+                                for (int e = 0; e < E; ++e) p[(u * 16 + 4 * g + i) * E + e] = o[rb][u][e][i];
                     }
             __syncthreads();
 #pragma unroll
             for (int n = 0; n < EACH; ++n) {
                 const int i = threadIdx.x + n * NW * 64, x = i / (D / 8), c = i % (D / 8);
-                if (x < rows_here)
-                    for (int y = w0; y < w0 + at_once && y < NW; ++y) {
-                        const float *p = s_o + ((y - w0) * rows_here + x) * (D + 4) + c * 8;
-                        v0[n] += *reinterpret_cast<const f32x4 *>(p);
-                        v1[n] += *reinterpret_cast<const f32x4 *>(p + 4);
+                if (x >= rows_here) continue;
+                if (w0 == 0) {
+                    v0[n] = v1[n] = (f32x4){0, 0, 0, 0};
+                    float2 ml[NW];
+#pragma unroll
+                    for (int y = 0; y < NW; ++y) ml[y] = s_ml[y * ROWS + x];
+                    most[n] = -INFINITY, sum[n] = 0.0f;
+#pragma unroll
+                    for (int y = 0; y < NW; ++y) most[n] = fmaxf(most[n], ml[y].x);
+#pragma unroll
+                    for (int y = 0; y < NW; ++y) {
+                        weight[n][y] = ml[y].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[y].x - most[n]);
+                        sum[n] += ml[y].y * weight[n][y];
                     }
+                }
+#pragma unroll
+                for (int y = 0; y < NW; ++y) {
+                    if (y < w0 || y >= w0 + at_once) continue;
+                    const float *p = s_o + ((y - w0) * rows_here + x) * (D + 4) + c * 8;
+                    v0[n] += *reinterpret_cast<const f32x4 *>(p) * weight[n][y];
+                    v1[n] += *reinterpret_cast<const f32x4 *>(p + 4) * weight[n][y];
+                }
             }
-            __syncthreads();
+            if (w0 + at_once < NW) __syncthreads();
         }
         const int slot = 2 * me + (skip == 0 ? 1 : 0);
 #pragma unroll
         for (int n = 0; n < EACH; ++n) {
             const int i = threadIdx.x + n * NW * 64, x = i / (D / 8), c = i % (D / 8);
             if (x >= rows_here) continue;
-            float most = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-            for (int y = 0; y < NW; ++y) most = fmaxf(most, s_ml[y * ROWS + x].x);
-#pragma unroll 4
-            for (int y = 0; y < NW; ++y) {
-                const float2 ml = s_ml[y * ROWS + x];
-                sum += ml.x == -INFINITY ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - most);
-            }
             if (whole_item) {
                 const int row = row0 + x;
-                store_row<T>(a, (first + row / group) * a.q_heads + h * group + row % group, D, c, v0[n], v1[n], most, sum);
+                store_row<T>(a, (first + row / group) * a.q_heads + h * group + row % group, D, c, v0[n], v1[n], most[n], sum[n]);
             } else {
                 float *p = a.part_o + ((int64_t)slot * ROWS + x) * D + c * 8;
                 *reinterpret_cast<f32x4 *>(p) = v0[n];
                 *reinterpret_cast<f32x4 *>(p + 4) = v1[n];
-                if (c == 0) a.part_ml[(int64_t)slot * ROWS + x] = make_float2(most, sum);
+                if (c == 0) a.part_ml[(int64_t)slot * ROWS + x] = make_float2(most[n], sum[n]);
             }
         }
         if (!whole_item && skip == 0) note = AttendNote{b, tile, (int)(((now + cost) * parts + all - 1) / all) - 1, 0};
