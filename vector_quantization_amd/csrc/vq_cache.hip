@@ -86,11 +86,9 @@ template <int D, int SUB> hipError_t launch_read(const ReadArgs &a, hipStream_t 
     const size_t book = (size_t)a.K * D * 2;
     const dim3 grid(a.heads, (unsigned)((a.tokens + a.chunk - 1) / a.chunk), 2);
     if (a.chunk >= a.K) {
-        if (book > 48 * 1024) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_cache_read<D, SUB, true>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)book);
-            if (e != hipSuccess) return e;
-        }
+        static std::atomic<uint64_t> allowed{0};
+        const hipError_t e = vq_internal_allow_lds(reinterpret_cast<const void *>(k_cache_read<D, SUB, true>), allowed);
+        if (e != hipSuccess) return e;
         hipLaunchKernelGGL((k_cache_read<D, SUB, true>), grid, dim3(512), book, stream, a);
     } else hipLaunchKernelGGL((k_cache_read<D, SUB, false>), grid, dim3(512), 0, stream, a);
     return hipGetLastError();
@@ -165,25 +163,22 @@ struct Attention {
     int parts, join_at, join_rows;
     size_t slots, ws;
 };
-// The least that a workgroup is given: under two tiles a wave, staging and joining outweigh what is shared out.
-constexpr int LEAST_TILES = 16;
-
 Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q, int64_t max_kv) {
     constexpr int CUS = 256;
     Attention r;
     const int Kp = dim <= 128 ? 256 : rows_padded(K), group = q_heads / heads;      // (as k_cache_attend lays out its tables)
     const int64_t per_seq = max_q * group;
-    // Behind the tables lie the waves' maxima and sums, and at least one wave's rows.  More than 16 rows a sequence go 32 at a time,
+    // Behind the tables lie the waves' maxima and sums, and 16 rows of at least one wave.  More than 16 rows a sequence go 32 at a time,
     // so that a look-up serves twice the products, unless the value table then no longer fits but would beside 16.
     const size_t keys = key_bytes(Kp, dim, sub), values = (size_t)Kp * dim * 2, row = (size_t)(dim + 4) * 4;
     auto waves = [&](int rb) { return rb == 2 && dim >= 192 ? 4 : 8; };
-    auto fits = [&](int rb, size_t tables) { return tables + (size_t)waves(rb) * rb * 16 * 8 + rb * 16 * row <= LDS_MOST; };
-    r.p.rb = per_seq <= 16 ? 1 : fits(2, keys + values) ? 2 : fits(1, keys + values) ? 1 : fits(2, keys) ? 2 : 1;
+    auto fits = [&](int rb, size_t tables) { return tables + (size_t)waves(rb) * rb * 16 * 8 + 16 * row <= LDS_MOST; };
+    r.p.rb = per_seq <= 16 ? 1 : fits(2, keys + values) || !fits(1, keys + values) ? 2 : 1;
     r.p.nw = waves(r.p.rb);
     r.p.values_in_lds = fits(r.p.rb, keys + values);
     const int rows = r.p.rb * 16;
     const size_t ml = (size_t)r.p.nw * rows * 8, tables = keys + (r.p.values_in_lds ? values : 0);
-    const size_t room = (LDS_MOST - tables - ml) / row, most = (size_t)r.p.nw * rows;      // (room >= rows: it fits)
+    const size_t room = (LDS_MOST - tables - ml) / row, most = (size_t)r.p.nw * rows;      // (room >= 16: it fits)
     r.join_at = (int)tables;
     r.join_rows = (int)(room < most ? room : most);
     r.p.lds = tables + ml + r.join_rows * row;
@@ -226,6 +221,17 @@ int lbg(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens
 }
 
 }  // namespace
+
+hipError_t vq_internal_allow_lds(const void *kernel, std::atomic<uint64_t> &allowed) {
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;        // (further devices are asked every time)
+    if (allowed.load(std::memory_order_acquire) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_MOST);
+    if (e == hipSuccess) allowed.fetch_or(bit, std::memory_order_release);
+    return e;
+}
 
 extern "C" {
 
@@ -321,7 +327,7 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
     float2 *part_ml = reinterpret_cast<float2 *>(part_o + r.slots * r.p.rb * 16 * dim);
     AttendArgs a = {q, q_token_stride, q_head_stride, rows, q_heads, {k_cb, v_cb}, cb_heads, heads, K, rows_padded(K), {k_codes, v_codes}, pages,
                     page, table, seqs, width, kv_lens, starts, (float)fmax(fabs(scale) * 1.4426950408889634, 1e-37), scale < 0 ? 0x80008000u : 0u,
-                    out, lse, r.parts, LEAST_TILES, r.join_at, r.join_rows, part_o, part_ml,
+                    out, lse, r.parts, r.join_at, r.join_rows, part_o, part_ml,
                     reinterpret_cast<AttendNote *>(part_ml + r.slots * r.p.rb * 16)};
     const dim3 grid(heads, r.parts);
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -143,6 +143,11 @@ template <int RB> __device__ inline int cost_of(int tile, int n_q, int n_kv, int
     return n < 1 ? 1 : n;
 }
 
+// Where a part of the work begins: parts of equal length, to a tile; it rises with the part, and both kernels work it out alike.
+__device__ inline int64_t part_begin(int64_t all, int parts, int part) {
+    return part >= parts ? all : (int64_t)((double)all / (double)parts * (double)part);
+}
+
 // One head's work is all its items side by side, (sequence, tile of rows) after (sequence, tile of rows), cut into as many equal
 // ranges of tiles as there are workgroups: causal and ragged lengths are balanced by themselves, and a workgroup stages its tables once.
 // A range may begin and end inside an item.  Such an item's parts go to the workspace (`slots`, two a workgroup: the part that begins
@@ -156,14 +161,14 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x, group = a.q_heads / a.heads;
-    const int Kp = a.Kp;
-    // Up to 128 dims the tables are laid out for 256 codewords whatever K is, so that a look-up's part is an offset in its instruction.
-    const int room = D <= 128 ? 256 : Kp, kstride = key_stride(room, SUB);
-    const int k_at = VLDS ? room * D * 2 : 0;                     // the value table comes first: see look-ups
+    // Up to 128 dims the tables have room for 256 codewords whatever K is: any code is inside them as it is, and a look-up's part is
+    // an offset in its instruction.
+    const int Kp = D <= 128 ? 256 : a.Kp, kstride = key_stride(Kp, SUB);
+    const int k_at = VLDS ? Kp * D * 2 : 0;                       // the value table comes first: see look-ups
     const int64_t cb0 = a.cb_heads == 1 ? 0 : (int64_t)h * a.K * D;
     const T *k_cb = static_cast<const T *>(a.cb[0]) + cb0, *v_cb = static_cast<const T *>(a.cb[1]) + cb0;
     const int page16 = a.page >> 4;
-    const uint32_t fold = (uint32_t)(Kp - 1) * 0x01010101u;     // keeps codes of no codeword inside the tables
+    const uint32_t fold = D <= 128 ? ~0u : (uint32_t)(Kp - 1) * 0x01010101u;      // keeps codes of no codeword inside the tables
     const int64_t page_bytes = (int64_t)a.heads * a.page * M;
     const int64_t head_at = (int64_t)h * a.page * M;
     const uint32_t k_lane = r * M + g * NB;
@@ -207,38 +212,38 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
     stage_load(threadIdx.x);
 
     // This workgroup's range.  Every wave works it out by itself: 64 sequences at a time, the tiles of rows of a long one 64 at a time too.
-    auto cost_of_sequence = [&](int b) -> int64_t {
+    int seq_first = 0, seq_q = 0, seq_kv = 0, held = 0;           // a lane's sequence: the lanes hold those from `held` on
+    int64_t items = 0;
+    auto costs_from = [&](int b0) -> int64_t {                    // running cost of the 64 sequences from b0 on, which the lanes hold then
         int64_t first = 0, sum = 0;
-        int n_q = 0, n_kv = 0;
-        if (b < a.seqs) sequence(a, b, first, n_q, n_kv);
-        const int tiles = (n_q * group + ROWS - 1) / ROWS;
-        if (tiles == 1) sum = cost_of<RB>(0, n_q, n_kv, group);
+        seq_q = seq_kv = 0;
+        if (b0 + lane < a.seqs) sequence(a, b0 + lane, first, seq_q, seq_kv);
+        seq_first = (int)first;
+        held = b0;
+        const int tiles = (seq_q * group + ROWS - 1) / ROWS;
+        items += of_last_lane(running(tiles));
+        if (tiles == 1) sum = cost_of<RB>(0, seq_q, seq_kv, group);
         for (uint64_t todo = __ballot(tiles > 1); todo; todo &= todo - 1) {
-            const int of = __builtin_ctzll(todo), x_q = __shfl(n_q, of), x_kv = __shfl(n_kv, of), x_tiles = __shfl(tiles, of);
+            const int of = __builtin_ctzll(todo), x_q = __shfl(seq_q, of), x_kv = __shfl(seq_kv, of), x_tiles = __shfl(tiles, of);
             int64_t part = 0;
             for (int t = lane; t < x_tiles; t += 64) part += cost_of<RB>(t, x_q, x_kv, group);
             part = of_last_lane(running(part));
             if (lane == of) sum = part;
         }
-        return sum;
+        return running(sum);
     };
-    const int64_t mine = cost_of_sequence(lane);
-    int64_t all = of_last_lane(running(mine));
-    for (int b0 = 64; b0 < a.seqs; b0 += 64) all += of_last_lane(running(cost_of_sequence(b0 + lane)));
-    // (a workgroup for every item at least, as far as they go: an item has costs of its own)
-    int64_t items = 0;
-    for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-        int64_t first = 0;
-        int n_q = 0, n_kv = 0;
-        if (b0 + lane < a.seqs) sequence(a, b0 + lane, first, n_q, n_kv);
-        items += of_last_lane(running((n_q * group + ROWS - 1) / ROWS));
+    int64_t costs = costs_from(0), all = of_last_lane(costs);
+    for (int b0 = 64; b0 < a.seqs; b0 += 64) {
+        costs = costs_from(b0);
+        all += of_last_lane(costs);
     }
-    int64_t parts = all / a.least_tiles > items ? all / a.least_tiles : items;
-    parts = parts < 1 ? 1 : parts > (int64_t)gridDim.y ? (int64_t)gridDim.y : parts;
+    // (a workgroup for every item at least, as far as they go: an item has costs of its own)
+    int64_t most_parts = all / LEAST_TILES > items ? all / LEAST_TILES : items;
+    const int parts = most_parts < 1 ? 1 : most_parts > (int64_t)gridDim.y ? (int)gridDim.y : (int)most_parts;
     const int me = h * gridDim.y + blockIdx.y;
-    const int64_t begin = all * blockIdx.y / parts, past = all * (blockIdx.y + 1) / parts;
-    if ((int64_t)blockIdx.y >= parts || begin >= past) {
-        if (a.parts > 1 && threadIdx.x == 0) a.notes[me] = AttendNote{-1, 0, 0, 0};
+    const int64_t begin = uniform(part_begin(all, parts, blockIdx.y)), past = uniform(part_begin(all, parts, blockIdx.y + 1));
+    if ((int)blockIdx.y >= parts || begin >= past) {
+        if (a.parts > 1 && threadIdx.x == 0) a.notes[me] = AttendNote{-1, 0, 0, 0, 0, 0};
         return;
     }
     int64_t skip = begin;                                         // first: of the work before sequence b; then of item (b, tile)
@@ -250,21 +255,23 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
     };
     int b = 0, tile = 0, at;
     for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-        const bool here = locate(running(b0 == 0 ? mine : cost_of_sequence(b0 + lane)), at);
+        if (b0 != held) costs = costs_from(b0);
+        const bool here = locate(costs, at);
         b = b0 + at;
         if (here) break;
     }
-    {
-        int64_t first;
-        int n_q, n_kv;
-        sequence(a, b < a.seqs ? b : 0, first, n_q, n_kv);
-        const int tiles = (n_q * group + ROWS - 1) / ROWS;
-        for (int t0 = 0; t0 < tiles; t0 += 64) {
-            const int t = t0 + lane;
-            const bool here = locate(running(t < tiles ? cost_of<RB>(t, n_q, n_kv, group) : 0), at);
-            tile = t0 + at;
-            if (here) break;
-        }
+    int first = 0, n_q = 0, n_kv = 0;                             // sequence b, out of the lane that holds it
+    if (b < a.seqs) {
+        first = __builtin_amdgcn_readlane(seq_first, b - held);
+        n_q = __builtin_amdgcn_readlane(seq_q, b - held);
+        n_kv = __builtin_amdgcn_readlane(seq_kv, b - held);
+    }
+    const int first_tiles = (n_q * group + ROWS - 1) / ROWS;
+    for (int t0 = 0; first_tiles > 1 && t0 < first_tiles; t0 += 64) {
+        const int t = t0 + lane;
+        const bool here = locate(running(t < first_tiles ? cost_of<RB>(t, n_q, n_kv, group) : 0), at);
+        tile = t0 + at;
+        if (here) break;
     }
     int64_t left = past - begin, now = begin - skip;              // now: where item (b, tile) begins
 
@@ -275,15 +282,16 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
     }
     __syncthreads();
 
-    AttendNote note = {-1, 0, 0, 0};
+    AttendNote note = {-1, 0, 0, 0, 0, 0};
     while (left > 0 && b < a.seqs) {
-        int64_t first;
-        int n_q, n_kv;
-        sequence(a, b, first, n_q, n_kv);
         const int n_rows = n_q * group;
         if (tile * ROWS >= n_rows) {
-            ++b;
             tile = 0;
+            if (++b < a.seqs) {
+                int64_t x;
+                sequence(a, b, x, n_q, n_kv);
+                first = (int)x;
+            }
             continue;
         }
         const int tiles = tiles_of<RB>(tile, n_q, n_kv, group), cost = tiles < 1 ? 1 : tiles;
@@ -303,7 +311,7 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
         for (int rb = 0; rb < RB; ++rb) {
             const int row = rb * 16 + r < rows_here ? row0 + rb * 16 + r : row0;
             const int i = row / group, head = h * group + row % group;
-            const T *p = static_cast<const T *>(a.q) + (first + i) * a.q_token_stride + head * a.q_head_stride + g * (D / 4);
+            const T *p = static_cast<const T *>(a.q) + (int64_t)(first + i) * a.q_token_stride + head * a.q_head_stride + g * (D / 4);
             sees[rb] = back + i;
 #pragma unroll
             for (int s = 0; s < KS; ++s) q[rb][s] = *reinterpret_cast<const u32x4 *>(p + 8 * s) ^ a.flip;
@@ -407,18 +415,26 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
             const uint32_t have = seen[slot];
             if constexpr (FIRST) {
                 u32x4 kx[2][KS];
+                auto values = [&]() {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) look_v(vc[slot][0][u], vc[slot][1][u], u, vx[u]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch(slot);
+                };
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) kx[0][ks] = look_k(kc[slot][0], ks), kx[1][ks] = look_k(kc[slot][1], ks);
-#pragma unroll
-                for (int u = 0; u < U; ++u) look_v(vc[slot][0][u], vc[slot][1][u], u, vx[u]);
-                __builtin_amdgcn_sched_barrier(0);
-                fetch(slot);
+                if constexpr (RB == 1) values();
+                else __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int s = 0; s < 2; ++s)
 #pragma unroll
                         for (int rb = 0; rb < RB; ++rb) z[rb][s] = mfma16<T>(kx[s][ks], q[rb][ks], z[rb][s]);
+                if constexpr (RB > 1) {                          // (more rows: the values take the keys' registers)
+                    __builtin_amdgcn_sched_barrier(0);
+                    values();
+                }
             } else {
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
@@ -506,68 +522,75 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
         if (g == 0)
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) s_ml[wave * ROWS + rb * 16 + r] = make_float2(top[rb], total[rb]);
-        constexpr int EACH = (ROWS * (D / 8) + NW * 64 - 1) / (NW * 64);       // pieces of 8 numbers a thread adds up
-        f32x4 v0[EACH], v1[EACH];
-        float weight[EACH][NW], most[EACH], sum[EACH];
-        const int at_once = a.join_rows / rows_here;
-        for (int w0 = 0; w0 < NW; w0 += at_once) {
-            if (wave >= w0 && wave < w0 + at_once)
+        constexpr int EACH = (16 * (D / 8) + NW * 64 - 1) / (NW * 64);         // pieces of 8 numbers a thread adds up
+        const int slot = 2 * me + (skip == 0 ? 1 : 0);
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-                    if (rb * 16 + r < rows_here) {
-                        float *p = s_o + ((wave - w0) * rows_here + rb * 16 + r) * (D + 4);
+        for (int rb = 0; rb < RB; ++rb) {
+            const int rows_rb = rows_here - rb * 16 < 16 ? rows_here - rb * 16 : 16;
+            if (rows_rb <= 0) break;
+            if (rb > 0) __syncthreads();                          // the sums of the rows before go to the same place
+            const int at_once = a.join_rows / rows_rb;
+            f32x4 v0[EACH], v1[EACH];
+            float weight[EACH][NW], most[EACH], sum[EACH];
+            for (int w0 = 0; w0 < NW; w0 += at_once) {
+                if (wave >= w0 && wave < w0 + at_once && r < rows_rb) {
+                    f32x4 *p = reinterpret_cast<f32x4 *>(s_o + ((wave - w0) * rows_rb + r) * (D + 4)) + g * E;
 #pragma unroll
-                        for (int u = 0; u < U; ++u)
+                    for (int u = 0; u < U; ++u)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
+                        for (int j = 0; j < E; ++j) {            // 4 chunks of E numbers side by side, written four numbers at a time
+                            f32x4 v;
 #pragma unroll
-                                for (int e = 0; e < E; ++e) p[(u * 16 + 4 * g + i) * E + e] = o[rb][u][e][i];
+                            for (int n = 0; n < 4; ++n) v[n] = o[rb][u][(4 * j + n) % E][(4 * j + n) / E];
+                            p[u * 4 * E + j] = v;
+                        }
+                }
+                __syncthreads();
+#pragma unroll
+                for (int n = 0; n < EACH; ++n) {
+                    const int i = threadIdx.x + n * NW * 64, x = i / (D / 8), c = i % (D / 8);
+                    if (x >= rows_rb) continue;
+                    if (w0 == 0) {
+                        v0[n] = v1[n] = (f32x4){0, 0, 0, 0};
+                        float2 ml[NW];
+#pragma unroll
+                        for (int y = 0; y < NW; ++y) ml[y] = s_ml[y * ROWS + rb * 16 + x];
+                        most[n] = -INFINITY, sum[n] = 0.0f;
+#pragma unroll
+                        for (int y = 0; y < NW; ++y) most[n] = fmaxf(most[n], ml[y].x);
+#pragma unroll
+                        for (int y = 0; y < NW; ++y) {
+                            weight[n][y] = ml[y].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[y].x - most[n]);
+                            sum[n] += ml[y].y * weight[n][y];
+                        }
                     }
-            __syncthreads();
+#pragma unroll
+                    for (int y = 0; y < NW; ++y) {
+                        if (y < w0 || y >= w0 + at_once) continue;
+                        const float *p = s_o + ((y - w0) * rows_rb + x) * (D + 4) + c * 8;
+                        v0[n] += *reinterpret_cast<const f32x4 *>(p) * weight[n][y];
+                        v1[n] += *reinterpret_cast<const f32x4 *>(p + 4) * weight[n][y];
+                    }
+                }
+                if (w0 + at_once < NW) __syncthreads();
+            }
 #pragma unroll
             for (int n = 0; n < EACH; ++n) {
                 const int i = threadIdx.x + n * NW * 64, x = i / (D / 8), c = i % (D / 8);
-                if (x >= rows_here) continue;
-                if (w0 == 0) {
-                    v0[n] = v1[n] = (f32x4){0, 0, 0, 0};
-                    float2 ml[NW];
-#pragma unroll
-                    for (int y = 0; y < NW; ++y) ml[y] = s_ml[y * ROWS + x];
-                    most[n] = -INFINITY, sum[n] = 0.0f;
-#pragma unroll
-                    for (int y = 0; y < NW; ++y) most[n] = fmaxf(most[n], ml[y].x);
-#pragma unroll
-                    for (int y = 0; y < NW; ++y) {
-                        weight[n][y] = ml[y].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[y].x - most[n]);
-                        sum[n] += ml[y].y * weight[n][y];
-                    }
-                }
-#pragma unroll
-                for (int y = 0; y < NW; ++y) {
-                    if (y < w0 || y >= w0 + at_once) continue;
-                    const float *p = s_o + ((y - w0) * rows_here + x) * (D + 4) + c * 8;
-                    v0[n] += *reinterpret_cast<const f32x4 *>(p) * weight[n][y];
-                    v1[n] += *reinterpret_cast<const f32x4 *>(p + 4) * weight[n][y];
+                if (x >= rows_rb) continue;
+                if (whole_item) {
+                    const int row = row0 + rb * 16 + x;
+                    store_row<T>(a, (int64_t)(first + row / group) * a.q_heads + h * group + row % group, D, c, v0[n], v1[n], most[n], sum[n]);
+                } else {
+                    const int64_t at = (int64_t)slot * ROWS + rb * 16 + x;
+                    float *p = a.part_o + at * D + c * 8;
+                    *reinterpret_cast<f32x4 *>(p) = v0[n];
+                    *reinterpret_cast<f32x4 *>(p + 4) = v1[n];
+                    if (c == 0) a.part_ml[at] = make_float2(most[n], sum[n]);
                 }
             }
-            if (w0 + at_once < NW) __syncthreads();
         }
-        const int slot = 2 * me + (skip == 0 ? 1 : 0);
-#pragma unroll
-        for (int n = 0; n < EACH; ++n) {
-            const int i = threadIdx.x + n * NW * 64, x = i / (D / 8), c = i % (D / 8);
-            if (x >= rows_here) continue;
-            if (whole_item) {
-                const int row = row0 + x;
-                store_row<T>(a, (first + row / group) * a.q_heads + h * group + row % group, D, c, v0[n], v1[n], most[n], sum[n]);
-            } else {
-                float *p = a.part_o + ((int64_t)slot * ROWS + x) * D + c * 8;
-                *reinterpret_cast<f32x4 *>(p) = v0[n];
-                *reinterpret_cast<f32x4 *>(p + 4) = v1[n];
-                if (c == 0) a.part_ml[(int64_t)slot * ROWS + x] = make_float2(most[n], sum[n]);
-            }
-        }
-        if (!whole_item && skip == 0) note = AttendNote{b, tile, (int)(((now + cost) * parts + all - 1) / all) - 1, 0};
+        if (!whole_item && skip == 0) note = AttendNote{b, tile, parts, 0, now + cost - 1, all};
         __syncthreads();                                          // the next item's sums go to the same place
 
         left -= take;
@@ -588,7 +611,11 @@ __global__ __launch_bounds__(256) void k_cache_join(const AttendArgs a) {
     int64_t first;
     int n_q, n_kv;
     sequence(a, note.seq, first, n_q, n_kv);
-    const int pieces = note.last - (int)blockIdx.y + 1;
+    int last = (int)((double)note.end / ((double)note.all / (double)note.parts));      // the part that the item's last tile falls to, to one or two
+    last = last < note.parts - 1 ? last : note.parts - 1;
+    while (last > 0 && part_begin(note.all, note.parts, last) > note.end) --last;
+    while (last < note.parts - 1 && part_begin(note.all, note.parts, last + 1) <= note.end) ++last;
+    const int pieces = last - (int)blockIdx.y + 1;
     auto slot = [&](int s) -> int64_t { return s == 0 ? 2 * (int64_t)me + 1 : 2 * ((int64_t)me + s); };
     for (int i = threadIdx.x; i < ROWS * (D / 8); i += 256) {
         const int x = i / (D / 8), c = i % (D / 8), row = note.tile * ROWS + x;
@@ -614,10 +641,9 @@ template <int D, int SUB, int RB, int NW, bool VLDS>
 hipError_t launch(const AttendArgs &a, const AttendPlan &p, dim3 grid, hipStream_t stream) {
     using T = VQ_CACHE_TYPE;
     auto *kernel = k_cache_attend<T, D, SUB, RB, NW, VLDS>;
-    if (p.lds > 48 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
-        if (e != hipSuccess) return e;
-    }
+    static std::atomic<uint64_t> allowed{0};                      // devices that know of the LDS this kernel takes, a bit each
+    const hipError_t e = vq_internal_allow_lds(reinterpret_cast<const void *>(kernel), allowed);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, grid, dim3(NW * 64), p.lds, stream, a);
     if (a.parts > 1) hipLaunchKernelGGL((k_cache_join<T, D, RB>), grid, dim3(256), 0, stream, a);
     return hipGetLastError();

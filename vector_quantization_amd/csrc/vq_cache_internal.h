@@ -3,6 +3,7 @@
 #define VQ_CACHE_INTERNAL_H
 
 #include <hip/hip_runtime.h>
+#include <atomic>
 #include <math.h>
 #include <stdint.h>
 
@@ -13,6 +14,8 @@
 
 VQ_HIDDEN int vq_internal_fail(int code, const char *message);
 VQ_HIDDEN int vq_internal_device(int *cus);
+// Lets a kernel take all of the LDS on the current device, once for each (`allowed`: the kernel's own, a bit a device).
+VQ_HIDDEN hipError_t vq_internal_allow_lds(const void *kernel, std::atomic<uint64_t> &allowed);
 
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
@@ -39,16 +42,18 @@ struct AttendArgs {
     uint32_t flip;                     // the sign bits of two 16-bit numbers where scale < 0: q is negated instead
     void *out;
     float *lse;
-    int parts, least_tiles;            // workgroups a head at most; a workgroup gets least_tiles tiles at least
+    int parts;                         // workgroups a head at most
     int join_at, join_rows;            // LDS behind the tables: its place, and how many rows' sums fit there
     float *part_o;                     // (slots, rows of an item, D), against part_ml's maximum; two slots a workgroup
     float2 *part_ml;                   // (slots, rows of an item): maximum (base 2) and sum
     struct AttendNote *notes;          // one a workgroup
 };
 
-// An item (tile of rows `tile` of sequence `seq`) whose parts the workgroups up to `last` of a head hold.
+// An item (tile of rows `tile` of sequence `seq`) that begins in one workgroup's part and ends, with tile `end` of all the head's work, in a
+// later one's.
 struct AttendNote {
-    int seq, tile, last, unused;
+    int seq, tile, parts, unused;
+    int64_t end, all;
 };
 
 struct SearchArgs {
@@ -95,6 +100,8 @@ VQ_HIDDEN hipError_t vq_internal_attend_bf16(const AttendArgs &a, const AttendPl
 VQ_HIDDEN hipError_t vq_internal_attend_f16(const AttendArgs &a, const AttendPlan &p, int dim, int sub, dim3 grid, hipStream_t stream);
 
 constexpr int LDS_MOST = 160 * 1024;
+// The least that a workgroup is given: under two tiles a wave, staging and joining outweigh what is shared out.
+constexpr int LEAST_TILES = 16;
 constexpr int TILE = 32;              // tokens a wave takes at a time: two groups of 16, each inside one page
 
 constexpr int value_chunk(int D, int SUB) {

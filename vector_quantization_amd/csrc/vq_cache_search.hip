@@ -85,11 +85,13 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
     // the codewords: operand of step 1, and in fp32 for steps 2 and 3; rows past K lie far away
     u32x4 A[NT][NM];
     float reach = 0.0f;                                                   // max |c|^2, infinite if any codeword is not finite
+    Numbers<C, SUB> raws[NT];                                             // all loads first: a call on a few tokens is their latency
+#pragma unroll
+    for (int t = 0; t < NT; ++t) raws[t] = *reinterpret_cast<const Numbers<C, SUB> *>(cb + (int64_t)(t * 32 + col < a.K ? t * 32 + col : a.K - 1) * a.dim);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int k = t * 32 + col;
-        Numbers<C, SUB> raw;
-        if (k < a.K) raw = *reinterpret_cast<const Numbers<C, SUB> *>(cb + (int64_t)k * a.dim);
+        const Numbers<C, SUB> raw = raws[t];
         float c[SUB], norm = 0.0f;
         uint32_t cp[CP][H2];
 #pragma unroll

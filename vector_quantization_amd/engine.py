@@ -13,6 +13,9 @@ from ._lib import lib, check, VQ_MODE_EXACT, VQ_MODE_FAST, VQ_PAD_EDGE, VQ_PAD_Z
 from .cache import CacheOps
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 
@@ -48,6 +51,10 @@ class HipEngine(CacheOps):
 
     # -- plumbing ----------------------------------------------------------------------------
     def _stream(self):
+        """The handle of torch's current stream on the engine's device (by torch's own short way where it has one: a
+        tenth of a microsecond instead of two)."""
+        if _raw_stream is not None:
+            return ctypes.c_void_p(_raw_stream(self.device.index))
         return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
 
     def _workspace(self, K, d, N=0):
