@@ -55,29 +55,58 @@ __global__ __launch_bounds__(512) void k_cache_read(const ReadArgs a) {
     const int64_t slots = a.pages * a.page;
     const uint8_t *codes = a.codes[which] + (int64_t)h * a.page * M;
     uint8_t *out = static_cast<uint8_t *>(a.out[which]);
-    for (int64_t i = begin * CH + threadIdx.x; i < end * CH; i += 512) {
-        const int64_t t = i / CH;
-        const int c = (int)(i % CH);
-        const int64_t slot = a.slots[t];
-        u32x4 v = {0, 0, 0, 0};
-        if (slot >= 0 && slot < slots) {
-            const int64_t p = a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page;
-            const int o = (int)(slot - p * a.page);
-            const uint8_t *q = codes + p * a.heads * a.page * M + (which == 0 ? (int64_t)o * M + c * N : (int64_t)c * N * a.page + o);
-            const int step = which == 0 ? 1 : a.page;
+    // Four pieces a turn in a long read: slots, codes and look-ups of all four are under way together (65536 tokens of 8 heads and 128
+    // dims: 103 -> 92 us).  A short one has no four to take.
+    constexpr int AT_ONCE = LDS ? 4 : 1;
+    for (int64_t i0 = begin * CH + threadIdx.x; i0 < end * CH; i0 += AT_ONCE * 512) {
+        int64_t slot[AT_ONCE];
+        int code[AT_ONCE][N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                int code = q[(int64_t)j * step];
-                code = code < a.K ? code : a.K - 1;
-                const uint8_t *w = (LDS ? s_book : book) + code * (D * 2) + c * 16 + j * (SUB * 2);
-                if constexpr (SUB == 8) v = *reinterpret_cast<const u32x4 *>(w);
-                else if constexpr (SUB == 4) {
-                    const u32x2 x = *reinterpret_cast<const u32x2 *>(w);
-                    v[2 * j] = x.x, v[2 * j + 1] = x.y;
-                } else v[j] = *reinterpret_cast<const uint32_t *>(w);
-            }
+        for (int n = 0; n < AT_ONCE; ++n) {
+            const int64_t i = i0 + n * 512;
+            slot[n] = i < end * CH ? a.slots[i / CH] : -1;
         }
-        *reinterpret_cast<u32x4 *>(out + (t * a.heads + h) * (D * 2) + c * 16) = v;
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n) {
+            const int c = (int)((i0 + n * 512) % CH);
+            const bool there = slot[n] >= 0 && slot[n] < slots;
+            const int64_t at = there ? slot[n] : 0, p = a.page_shift >= 0 ? at >> a.page_shift : at / a.page;
+            const int o = (int)(at - p * a.page);
+            const uint8_t *q = codes + p * a.heads * a.page * M;
+            if (which == 0) {                                     // a key's codes lie side by side
+                q += (int64_t)o * M + c * N;
+                uint32_t w;
+                if constexpr (N == 1) w = *q;
+                else if constexpr (N == 2) w = *reinterpret_cast<const uint16_t *>(q);
+                else w = *reinterpret_cast<const uint32_t *>(q);
+#pragma unroll
+                for (int j = 0; j < N; ++j) code[n][j] = w >> (8 * j) & 255u;
+            } else {
+                q += (int64_t)c * N * a.page + o;
+#pragma unroll
+                for (int j = 0; j < N; ++j) code[n][j] = q[(int64_t)j * a.page];
+            }
+            if (!there) slot[n] = -1;
+        }
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n) {
+            const int64_t i = i0 + n * 512;
+            if (i >= end * CH) continue;
+            const int c = (int)(i % CH);
+            u32x4 v = {0, 0, 0, 0};
+            if (slot[n] >= 0)
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const int k = code[n][j] < a.K ? code[n][j] : a.K - 1;
+                    const uint8_t *w = (LDS ? s_book : book) + k * (D * 2) + c * 16 + j * (SUB * 2);
+                    if constexpr (SUB == 8) v = *reinterpret_cast<const u32x4 *>(w);
+                    else if constexpr (SUB == 4) {
+                        const u32x2 x = *reinterpret_cast<const u32x2 *>(w);
+                        v[2 * j] = x.x, v[2 * j + 1] = x.y;
+                    } else v[j] = *reinterpret_cast<const uint32_t *>(w);
+                }
+            *reinterpret_cast<u32x4 *>(out + (i / CH * a.heads + h) * (D * 2) + c * 16) = v;
+        }
     }
 }
 
