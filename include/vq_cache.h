@@ -12,7 +12,8 @@
  *   v_codes    (pages, heads, parts, page) bytes: the codes of a page's tokens lie side by side, as the second
  *              product of attention takes them
  *   slot       page number * page + place in the page
- * dim is 32, 64, 96, 128, 192 or 256; sub is 2, 4 or 8; K is 1 to 256; page is a multiple of 16.
+ * dim is 32, 64, 96, 128, 192 or 256; sub is 2, 4 or 8; K is 1 to 256; page is a multiple of 16, at most 2^20; heads is
+ * at most 1024; pages and tokens are below 2^31.
  *
  * The conventions of vq_hip.h hold (device pointers, stream, status codes, vq_last_error, nothing allocated).
  * Every call reads its lengths, slots and page numbers on the device and may be captured into a HIP graph.
@@ -55,11 +56,12 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
 /* Causal attention of packed sequences' newest tokens over the cache.  Sequence b owns rows starts[b] to
  * starts[b + 1] of q (rows, q_heads, dim) and the first kv_lens[b] tokens of the pages table[b, 0 .. width); its
  * rows are the newest of those tokens: row i of n_q sees tokens 0 to kv_lens[b] - n_q + i.  Query heads are
- * grouped: head h reads cache head h / (q_heads / heads).
+ * grouped: head h reads cache head h / (q_heads / heads).  rows * q_heads / heads is below 2^30, width * page below 2^31,
+ * q_heads at most 4096, seqs at most 65535.  out and lse overlap no other tensor of the call.
  *   out (rows, q_heads, dim) = softmax(scale * q k^T) v      lse (rows, q_heads, nullable) = log sum exp(scale * q k^T)
- * A row that sees no token gets zeros and minus infinity; rows of no sequence are left as they were.  Lengths past
+ * A row that sees no token, or whose scores are all minus infinity, gets zeros and minus infinity; rows of no sequence are left as they were.  Lengths past
  * the table's width are cut to it; the tokens of a page number outside [0, pages) are not seen.  Codewords have to be
- * finite.  max_q and max_kv, the longest of the sequences' rows and lengths as the caller knows them, only shape
+ * finite; a code of K or more stands for some codeword or for zeros.  max_q and max_kv, the longest of the sequences' rows and lengths as the caller knows them, only shape
  * the launch: any value of 1 or more gives the same sums, up to the order of addition.
  * `starts` rises, from 0 or more to `rows` or less.  dtype: VQ_BF16 or VQ_F16. */
 size_t vq_cache_attention_ws_bytes(int64_t rows, int q_heads, int heads, int dim, int sub, int K, int seqs,
@@ -73,10 +75,10 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
 
 /* The accumulating half of an LBG iteration of float codebooks: over `tokens` tokens' vectors x, for each head,
  * part and codeword, the sum and number of the vectors nearest to it (as in vq_cache_write), and for each head and part
- * the sum of the least squared distances.  A vector of numbers that are not all finite is left out of all three.
+ * the sum of the least squared distances.  A vector of which a number is 2^100 or more in size, or no number, is left out of all three.
  * sums (heads, K, dim) fp64, counts (heads, parts, K) int64, dist (heads, parts) fp64 are overwritten; the result
- * does not depend on timing.  cb is (heads, K, dim) fp32; x is of any of the three types, its finite numbers below
- * 2^90 in size.  Adding several calls' sums, counts and dist gives those of their tokens together. */
+ * does not depend on timing.  cb is (heads, K, dim) fp32; x is of any of the three types; at most 65535 chunks
+ * of 4096 tokens (268 million) a call; a codeword's sum over a chunk stays below 2^104 (of numbers below 2^92 it always does).  Adding several calls' sums, counts and dist gives those of their tokens together. */
 size_t vq_cache_lbg_ws_bytes(int64_t tokens, int heads, int dim, int sub, int K);
 int vq_cache_lbg_accum(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens,
                        const float *cb, int heads, int dim, int sub, int K, int dtype,

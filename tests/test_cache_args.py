@@ -174,3 +174,70 @@ def test_engine_lbg_refuses_what_does_not_fit(eng):
         train_cache_codebooks(eng, x, 300, 4)
     with pytest.raises(ValueError, match="cut into"):
         train_cache_codebooks(eng, x, 4, 5)
+
+
+# ---- training over several processes ---------------------------------------------------------------------------------
+
+class HostEngine:
+    """cache_lbg_accum / cache_lbg_finish by their definitions, on the host."""
+    device = torch.device("cpu")
+
+    def cache_lbg_accum(self, x, cb, sub):
+        T, H, D = x.shape
+        K, M = cb.shape[1], D // sub
+        xs, cs = x.double().reshape(T, H, M, sub), cb.double().reshape(H, K, M, sub)
+        d = (xs[:, :, None] - cs[None]).square().sum(-1)                  # (T, H, K, M)
+        least, code = d.min(2)
+        hot = torch.nn.functional.one_hot(code, K).double()                # (T, H, M, K)
+        sums = torch.einsum("thmk,thme->hkme", hot, xs).reshape(H, K, D)
+        return sums, hot.sum(0).long(), least.sum(0)
+
+    def cache_lbg_finish(self, sums, counts, dist, cb):
+        H, K, D = cb.shape
+        M = counts.shape[1]
+        n = counts.permute(0, 2, 1).repeat_interleave(D // M, 2).double()
+        return torch.where(n > 0, sums / n.clamp(min=1), cb.double()).float(), dist / counts.sum(-1).clamp(min=1)
+
+
+def clouds():
+    g = torch.Generator().manual_seed(1)
+    return torch.randn((301, 2, 16), generator=g) + 4 * torch.randint(-1, 2, (301, 2, 16), generator=g)
+
+
+def _rank(rank, world, port, out):
+    import torch.distributed as dist
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=world)
+    x = clouds()
+    mine = x[:113] if rank == 0 else x[113:]
+    res = train_cache_codebooks(HostEngine(), mine, 8, 4, group=dist.group.WORLD, log=None)
+    torch.save((res.codebook, res.iters_per_stage, res.distortions), f"{out}/{rank}.pt")
+    dist.destroy_process_group()
+
+
+def test_training_over_two_processes(tmp_path):
+    """Shards of unequal size train what one process trains on all vectors; both ranks end with the same bits."""
+    import socket
+    import torch.multiprocessing as mp
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    mp.start_processes(_rank, args=(2, port, str(tmp_path)), nprocs=2, start_method="spawn")
+    (cb0, it0, d0), (cb1, it1, d1) = (torch.load(tmp_path / f"{r}.pt", weights_only=True) for r in range(2))
+    one = train_cache_codebooks(HostEngine(), clouds(), 8, 4, log=None)
+    assert torch.equal(cb0, cb1) and it0 == it1 and d0 == d1
+    assert it0 == one.iters_per_stage and len(one.distortions) == sum(it0)
+    assert one.codebook.shape == (2, 8, 16)
+    # sums of 301 numbers in fp64 in two orders: the same to 301 * 2^-53 of their size, then one rounding to fp32 and its like in each iteration
+    assert (cb0 - one.codebook).abs().max() <= 2.0 ** -22 * one.codebook.abs().max()
+    assert one.distortions[-1] < one.distortions[0]
+
+
+def test_training_log_and_stop_rule():
+    lines = []
+    res = train_cache_codebooks(HostEngine(), clouds(), 4, 4, log=lines.append)
+    assert len(lines) == 2 and all(line.startswith("Converged at iter") for line in lines)
+    assert res.converged_iter == [n - 1 for n in res.iters_per_stage]
+    short = train_cache_codebooks(HostEngine(), clouds(), 4, 4, log=None, max_iterations=1)
+    assert short.iters_per_stage == [1, 1] and short.converged_iter == [-1, -1]
+    flat = train_cache_codebooks(HostEngine(), torch.ones(9, 1, 16), 4, 4, log=None)      # no spread: nothing to part, nothing diverges
+    assert torch.equal(flat.codebook, torch.ones(1, 4, 16)) and flat.distortions[-1] == 0.0

@@ -185,6 +185,29 @@ def test_write_hard_values(eng, dtype, case):
     assert torch.equal(vc.cpu().permute(0, 3, 1, 2).reshape(144, H, D // sub)[:T].long(), torch.from_numpy(codes64(x.flip(0), cb.flip(1), sub)[0]))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [1, 7, 100, 255])
+def test_large_vectors_keep_to_the_codewords_there_are(eng, K, dtype):
+    """Vectors of numbers near 1e18, and far larger and smaller ones, beside a codebook that does not fill its tile."""
+    T, H, D, sub = 96, 1, 32, 4
+    x = (data(7, (T, H, D), torch.float32) * (10.0 ** torch.arange(10, 34).repeat_interleave(4)).reshape(T, 1, 1)).to(dtype)
+    x[32:36] = torch.tensor([1e18, -1e18, 0.9e18, 1.1e18]).to(dtype).reshape(4, 1, 1)
+    cb = torch.zeros((H, K, D)) if K == 1 else data(8, (H, K, D), torch.float32)
+    code = torch.from_numpy(codes64(x, cb.to(dtype), sub)[0])
+    if dtype != torch.float32:
+        kc, vc = eng.cache_buffers(6, 16, H, D, sub)
+        eng.cache_write(x.to(DEV), x.to(DEV), torch.arange(T, device=DEV), cb.to(dtype).to(DEV), cb.to(dtype).to(DEV), kc, vc)
+        assert torch.equal(kc.cpu().transpose(1, 2).reshape(T, H, D // sub).long(), code)
+        assert torch.equal(vc.cpu().permute(0, 3, 1, 2).reshape(T, H, D // sub).long(), code)
+    code = torch.from_numpy(codes64(x, cb, sub)[0])
+    counted = (x.double().abs() < 2.0 ** 100).reshape(T, H, -1, sub).all(-1)
+    assert not counted.all() and counted.any()
+    _, counts, dist = eng.cache_lbg_accum(x.to(DEV), cb.to(DEV), sub)
+    for m in range(D // sub):
+        assert torch.equal(counts[0, m].cpu(), torch.bincount(code[:, 0, m][counted[:, 0, m]], minlength=K))
+    assert dist.isfinite().all()
+
+
 def test_write_strides_and_shared_codebook(eng):
     """Keys and values inside one larger tensor, copies where their vectors do not start at multiples of 16 bytes, one codebook for all heads."""
     T, H, D, sub, K, page = 77, 4, 64, 4, 256, 16
@@ -278,6 +301,20 @@ def test_attention_peaked_and_large_scores(eng):
         case[0] = case[0] * 8
         out, lse = eng.cache_attention(*[t.to(DEV) for t in case], 30, scale=scale, want_lse=True)
         check_attention(out, lse, attention64(*case, 4, scale), 300)
+
+
+@pytest.mark.parametrize("n_q,n_kv", [([1, 1], [40, 700]), ([30, 3], [300, 60])])
+def test_attention_nan_stays_in_its_row(eng, n_q, n_kv):
+    """A query that is no number gives a row and a logarithm that are none, and leaves the rows beside it as they are."""
+    case = list(attention_case(n_q, n_kv, 4, 2, 64, 4, 256, 16, torch.bfloat16, seed=25))
+    clean = eng.cache_attention(*[t.to(DEV) for t in case], max(n_q), want_lse=True)
+    case[0][1, 2, 5] = math.nan
+    out, lse = eng.cache_attention(*[t.to(DEV) for t in case], max(n_q), want_lse=True)
+    bad = torch.zeros((sum(n_q), 4), dtype=torch.bool, device=DEV)
+    bad[1, 2] = True
+    assert out[bad].isnan().all() and torch.equal(lse.isnan(), bad)
+    check_attention(out[~bad], lse[~bad], [t.reshape(bad.shape + t.shape[2:])[~bad.cpu()] for t in attention64(*case, 4, 0.125)], max(n_kv))
+    assert clean[0].isfinite().all()
 
 
 def test_attention_rows_of_no_sequence_bad_pages_and_codes(eng):

@@ -162,7 +162,7 @@ class CacheOps:
         and the first kv_lens[b] (int32) tokens of the pages table[b] (int32, (sequences, width)); its rows are the newest
         of those tokens, whose keys and values are in the cache already.  Query head h reads cache head
         h // (q_heads / heads).  A row that sees no token gets zeros (and a logarithm of minus infinity); rows of no
-        sequence are left as they were in `out`, and are undefined where the call allocates it.
+        sequence are left as they were in `out`, and are undefined in what the call allocates.  `out` overlaps no other argument.
         max_q, max_kv: the longest of the sequences' rows and lengths, as the host knows them; they shape the launch only
         (max_kv None: what the table can hold).  scale: 1 / sqrt(dim) if None.
         Returns out (rows, q_heads, dim), with want_lse also the natural logarithm of each row's sum of exponentials
@@ -212,8 +212,8 @@ class CacheOps:
     def cache_lbg_accum(self, x, cb, sub):
         """The accumulating half of an LBG iteration of float codebooks cb (heads, K, dim) float32 over the vectors
         x (tokens, heads, dim): for each codeword the sum (heads, K, dim) float64 and number (heads, parts, K) int64 of the
-        sub-vectors nearest to it, and the sum of their squared distances (heads, parts) float64.  A sub-vector of numbers
-        that are not all finite is left out.  Shards' results are added."""
+        sub-vectors nearest to it, and the sum of their squared distances (heads, parts) float64.  A sub-vector of
+        which a number is 2^100 or more in size, or NaN, is left out.  Shards' results are added."""
         device = self.device
         tokens, heads, K, dim, parts = self._lbg_arguments(x, cb, sub)
         make = torch.empty if tokens else torch.zeros

@@ -179,12 +179,7 @@ int check_vectors(const char *name, const void *p, int64_t token_stride, int64_t
     return VQ_OK;
 }
 
-int grid_for(int64_t items, int64_t most) {
-    const int64_t g = (items + 255) / 256;
-    return (int)(g < 1 ? 1 : (g > most ? most : g));
-}
-
-int64_t clamp_hint(int64_t n) { return n > 0x7fffffff ? 0x7fffffff : n; }
+int64_t at_most(int64_t n, int64_t most) { return n < most ? n : most; }
 
 // How many rows a workgroup takes at a time and how many workgroups a head gets.  Host arithmetic on sizes alone.
 struct Attention {
@@ -196,7 +191,7 @@ Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int se
     constexpr int CUS = 256;
     Attention r;
     const int Kp = dim <= 128 ? 256 : rows_padded(K), group = q_heads / heads;      // (as k_cache_attend lays out its tables)
-    const int64_t per_seq = max_q * group;
+    const int64_t per_seq = at_most(max_q, 0x3fffffff) * group;
     // Behind the tables lie the waves' maxima and sums, and 16 rows of at least one wave.  More than 16 rows a sequence go 32 at a time,
     // so that a look-up serves twice the products, unless the value table then no longer fits but would beside 16.
     const size_t keys = key_bytes(Kp, dim, sub), values = (size_t)Kp * dim * 2, row = (size_t)(dim + 4) * 4;
@@ -212,7 +207,8 @@ Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int se
     r.join_rows = (int)(room < most ? room : most);
     r.p.lds = tables + ml + r.join_rows * row;
     // a head has at most so many items and tiles, by the caller's word
-    const int64_t items = (per_seq + rows - 1) / rows * seqs, tiles = items * ((max_kv + TILE - 1) / TILE);
+    const int64_t items = at_most(at_most((per_seq + rows - 1) / rows, 0x3fffffff) * seqs, 0x3fffffff);
+    const int64_t tiles = items * ((at_most(max_kv, 0x7fffffff) + TILE - 1) / TILE);
     const int64_t wanted = tiles / LEAST_TILES > items ? tiles / LEAST_TILES : items;
     int64_t parts = (CUS + heads - 1) / heads;
     if (parts * heads > CUS && parts > 1) --parts;
@@ -234,11 +230,12 @@ int lbg(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens
     if (!cb || !out.counts || !out.dist) return fail(VQ_E_INVALID, "null pointer");
     if ((uintptr_t)cb & 15) return fail(VQ_E_INVALID, "the codebook must start at a multiple of 16 bytes");
     if ((rc = check_vectors("x", x, token_stride, head_stride, dtype == VQ_F32 ? 4 : 2))) return rc;
+    const SearchPlan p = vq_internal_search_plan(tokens, heads, dim, sub, 1);
+    if (p.blocks > 65535) return fail(VQ_E_UNSUPPORTED, "tokens=%lld: at most 65535 chunks of 4096 in one call", (long long)tokens);
     const size_t need = vq_cache_lbg_ws_bytes(tokens, heads, dim, sub, K);
     if (!ws || ws_bytes < need) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, need);
     if ((uintptr_t)ws & 15) return fail(VQ_E_INVALID, "the workspace must start at a multiple of 16 bytes");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const SearchPlan p = vq_internal_search_plan(tokens, heads, dim, sub, 1);
     double *part_dist = static_cast<double *>(ws);
     float *part_sums = reinterpret_cast<float *>(part_dist + (int64_t)p.chunks * heads * (dim / sub));
     const SearchArgs a = {{x, x}, {token_stride, token_stride}, {head_stride, head_stride}, {cb, cb}, tokens, heads, heads, dim, K, p.pw, p.chunk,
@@ -294,7 +291,6 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
     if ((rc = check_cache(k_codes, v_codes, k_cb, v_cb, cb_heads, heads, pages, page, dtype))) return rc;
     if (tokens < 0) return fail(VQ_E_INVALID, "need tokens >= 0");
     if (tokens > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "tokens below 2^31");
-    if (tokens > 0x7fffffff) return fail(VQ_E_UNSUPPORTED, "tokens below 2^31");
     if (tokens == 0) return VQ_OK;
     if (!slots) return fail(VQ_E_INVALID, "null pointer");
     if ((rc = check_vectors("k_out", k_out, dim, dim, 2))) return rc;
@@ -324,7 +320,7 @@ size_t vq_cache_attention_ws_bytes(int64_t rows, int q_heads, int heads, int dim
     if (rows <= 0 || q_heads <= 0 || q_heads > 4096 || seqs <= 0 || max_q < 1 || max_kv < 1 || check_shape(heads, dim, sub, K) ||
         q_heads % heads)
         return 0;
-    return plan_attention(q_heads, heads, dim, sub, K, seqs, clamp_hint(max_q), clamp_hint(max_kv)).ws;
+    return plan_attention(q_heads, heads, dim, sub, K, seqs, max_q, max_kv).ws;
 }
 
 int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t rows, int q_heads, const void *k_cb,
@@ -338,7 +334,7 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
     if (q_heads <= 0 || q_heads % heads) return fail(VQ_E_INVALID, "q_heads=%d: a positive multiple of heads (%d)", q_heads, heads);
     if (q_heads > 4096) return fail(VQ_E_UNSUPPORTED, "q_heads=%d: at most 4096", q_heads);
     if (rows < 0 || seqs < 0 || width < 0) return fail(VQ_E_INVALID, "need rows, seqs and width >= 0");
-    if (rows * (q_heads / heads) > 0x3fffffff || (int64_t)width * page > 0x7fffffff)
+    if (rows > 0x3fffffff || rows * (q_heads / heads) > 0x3fffffff || (int64_t)width * page > 0x7fffffff)
         return fail(VQ_E_UNSUPPORTED, "rows * q_heads / heads below 2^30, width * page below 2^31");
     if (max_q < 1 || max_kv < 1) return fail(VQ_E_INVALID, "need max_q and max_kv >= 1");
     if (!(fabs(scale) < 1e38)) return fail(VQ_E_INVALID, "scale must be finite and below 1e38 in size");
@@ -347,8 +343,6 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
     if ((!table && width > 0) || !kv_lens || !starts) return fail(VQ_E_INVALID, "null pointer");
     if ((rc = check_vectors("q", q, q_token_stride, q_head_stride, 2))) return rc;
     if ((rc = check_vectors("out", out, dim, dim, 2))) return rc;
-    max_q = clamp_hint(max_q);
-    max_kv = clamp_hint(max_kv);
     const Attention r = plan_attention(q_heads, heads, dim, sub, K, seqs, max_q, max_kv);
     if (r.ws > 0 && (!ws || ws_bytes < r.ws)) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, r.ws);
     if (r.ws > 0 && ((uintptr_t)ws & 15)) return fail(VQ_E_INVALID, "the workspace must start at a multiple of 16 bytes");

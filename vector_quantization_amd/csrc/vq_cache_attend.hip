@@ -124,11 +124,11 @@ __device__ inline int64_t of_last_lane(int64_t v) {
 // 8 numbers of a finished row, place = row * q_heads + head: v against the maximum `most` (base 2) and the sum of weights.
 template <typename T>
 __device__ inline void store_row(const AttendArgs &a, int64_t place, int D, int c, f32x4 v0, f32x4 v1, float most, float sum) {
-    const float over = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float over = sum == 0.0f ? 0.0f : 1.0f / sum;              // 0: the row sees no token (of any other the largest weight is 1 or more)
     *reinterpret_cast<u32x4 *>(static_cast<T *>(a.out) + place * D + c * 8) =
         (u32x4){pack2<T>(v0[0] * over, v0[1] * over), pack2<T>(v0[2] * over, v0[3] * over),
                 pack2<T>(v1[0] * over, v1[1] * over), pack2<T>(v1[2] * over, v1[3] * over)};
-    if (c == 0 && a.lse) a.lse[place] = sum > 0.0f ? most * 0.69314718055994531f + logf(sum) : -INFINITY;
+    if (c == 0 && a.lse) a.lse[place] = sum == 0.0f ? -INFINITY : most * 0.69314718055994531f + logf(sum);
 }
 
 // The tiles that the rows of one item see: rows tile * RB * 16 on of a sequence, whose row i sees tokens 0 .. n_kv - n_q + i.

@@ -13,7 +13,6 @@
 #define VQ_HIDDEN __attribute__((visibility("hidden")))
 
 VQ_HIDDEN int vq_internal_fail(int code, const char *message);
-VQ_HIDDEN int vq_internal_device(int *cus);
 // Lets a kernel take all of the LDS on the current device, once for each (`allowed`: the kernel's own, a bit a device).
 VQ_HIDDEN hipError_t vq_internal_allow_lds(const void *kernel, std::atomic<uint64_t> &allowed);
 

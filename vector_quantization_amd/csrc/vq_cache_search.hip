@@ -33,8 +33,10 @@ constexpr Terms terms_of(int xp, int cp) {
 }
 
 constexpr int SEARCH_WAVES = 8;
-constexpr float FAR_SCORE = 1e38f, FAR_NUMBER = 1e18f, BOUND_MOST = 1e30f;
+constexpr float FAR_SCORE = 1e38f, FAR_NUMBER = 1e18f, BOUND_MOST = 1e30f, SIZE_MOST = 1e34f;
+// Rows past K lie at FAR_NUMBER: a vector within SIZE_MOST (1e17 long) and codewords within BOUND_MOST (1.5e15) are nearer to each other.
 constexpr float SUM_SCALE = 16777216.0f;       // lifts fp32's smallest numbers into bf16's normal range
+constexpr float COUNTED = 0x1p100f;            // training leaves out what is larger: times SUM_SCALE it would leave fp32
 
 __device__ inline uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
         const bool upper = h1 < l1;
         const float best = upper ? h1 : l1, second = least(upper ? l1 : h1, least(l2, h2));
         const float bound = 0.5f * reach + __builtin_amdgcn_sqrtf(size) * far;
-        bool open = !(second - best > bound * 1.52587890625e-5f + 1e-36f) || !(bound < BOUND_MOST);
+        bool open = !(second - best > bound * 1.52587890625e-5f + 1e-36f) || !(bound < BOUND_MOST) || !(size < SIZE_MOST);
         const int group = __builtin_bit_cast(uint32_t, best) & 15;
 
         // step 2: the two halves of a wave take four codewords each
@@ -253,7 +255,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
         } else {
             bool fine = token < end;
 #pragma unroll
-            for (int e = 0; e < SUB; ++e) fine = fine && fabsf(x[e]) < INFINITY;
+            for (int e = 0; e < SUB; ++e) fine = fine && fabsf(x[e]) < COUNTED;
             // sums by products with the one-hot numbers of the codewords: number = 16 hi + lo, and
             // sum[hi][lo] = sum over vectors of (x where its hi is this row) * (1 where its lo is this column)
             if (hh == 0) {
@@ -393,10 +395,10 @@ SearchPlan vq_internal_search_plan(int64_t tokens, int heads, int dim, int sub, 
     p.pw = parts % 8 ? 4 : 8;
     const int64_t side = SEARCH_WAVES / p.pw;                             // token ranges side by side in one workgroup
     const int64_t base = (int64_t)heads * (parts / p.pw) * both;
-    // A write is spread as thinly as there are tokens; a training chunk of fewer than 128 costs more to gather than it saves.  No
-    // chunk is longer than 4096: its sums are fp32, its counts exact.
-    const int fewest = both == 2 ? 32 : 128;
-    const int64_t most = (tokens + fewest * side - 1) / (fewest * side), least = (tokens + 4096 * side - 1) / (4096 * side);
+    // A write is spread as thinly as there are tokens; a training chunk of fewer than 128 costs more to gather than it saves, and none is
+    // longer than 4096: its sums are fp32.
+    const int fewest = both == 2 ? 32 : 128, longest = both == 2 ? 1 << 24 : 4096;
+    const int64_t most = (tokens + fewest * side - 1) / (fewest * side), least = (tokens + longest * side - 1) / (longest * side);
     int64_t n = (2 * CUS + base - 1) / base;
     n = n < most ? n : most;
     n = n > least ? n : least;

@@ -4736,15 +4736,9 @@ int run_sort(const SRC &src, bool row_words_ok, int64_t N, int d, void *sorted, 
 // ------------------------------------------------------------------------------------------------
 // C ABI
 // ------------------------------------------------------------------------------------------------
-// What vq_cache.hip shares with this file (not exported): the error text and the table of device properties.
+// What vq_cache.hip shares with this file (not exported): the error text.
 __attribute__((visibility("hidden"))) int vq_internal_fail(int code, const char *message) {
     return fail(code, "%s", message);
-}
-__attribute__((visibility("hidden"))) int vq_internal_device(int *cus) {
-    DeviceInfo di;
-    const int rc = device_info(di);
-    if (rc == VQ_OK) *cus = di.cus;
-    return rc;
 }
 
 extern "C" {
