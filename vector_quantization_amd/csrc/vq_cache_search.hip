@@ -53,11 +53,12 @@ template <typename V, int N> struct alignas(N * sizeof(V) < 16 ? N * sizeof(V) :
     V v[N];
 };
 
-__device__ inline void halves(float v, float &lo, float &hi) {      // the value of lane l and of lane l + 32, in both
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+// a and b: what lanes l and l + 32 found for the lower vectors and for the upper ones.  To each lane, both findings about its own.
+__device__ inline void to_owners(float &a, float &b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
     const uint32_t first = r[0], second = r[1];
-    lo = __builtin_bit_cast(float, first);
-    hi = __builtin_bit_cast(float, second);
+    a = __builtin_bit_cast(float, first);
+    b = __builtin_bit_cast(float, second);
 }
 
 // The lesser of two finite scores, without the canonicalisation that fminf of unknown bits brings.
@@ -69,9 +70,12 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
     constexpr int XP = PIECES<T>, CP = PIECES<C>, H2 = SUB / 2;
     constexpr Terms TM = terms_of(XP, CP);
     constexpr int PAIRS = TM.n * H2 + 2, NM = (PAIRS * 2 + 15) / 16;     // slots in pairs; the last two hold the norm
+    // Where a vector's slots fit into one half of the operand, the codewords stand in both: a lane of the upper half then
+    // gives its own vector's numbers there, and none have to be moved.
+    constexpr bool TWICE = PAIRS <= 4;
     __shared__ float s_tab[SEARCH_WAVES][NT * 32 * SUB];
-    __shared__ int16_t s_lab[TRAIN ? SEARCH_WAVES : 1][32];
-    __shared__ __align__(16) uint32_t s_x[TRAIN ? SEARCH_WAVES : 1][XP][32][H2];
+    __shared__ int16_t s_lab[TRAIN ? SEARCH_WAVES : 1][64];
+    __shared__ __align__(16) uint32_t s_x[TRAIN ? SEARCH_WAVES : 1][XP][64][H2];
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int which = blockIdx.z, parts = a.dim / SUB, per = parts / a.pw;
@@ -83,6 +87,9 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
     float *tab = s_tab[wave];
     const C *cb = static_cast<const C *>(a.cb[which]) + (a.cb_heads == 1 ? 0 : (int64_t)h * a.K * a.dim) + m * SUB;
     const T *x0 = static_cast<const T *>(a.x[which]) + h * a.head_stride[which] + m * SUB;
+
+    const int64_t slots = a.pages * a.page, page_bytes = (int64_t)a.heads * a.page * parts;
+    uint8_t *codes = which == 0 ? a.k_codes + (int64_t)h * a.page * parts + m : a.v_codes + ((int64_t)h * parts + m) * a.page;
 
     // the codewords: operand of step 1, and in fp32 for steps 2 and 3; rows past K lie far away
     u32x4 A[NT][NM];
@@ -118,7 +125,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
 #pragma unroll
         for (int n = 0; n < NM; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) A[t][n][j] = hh ? pair(8 * n + 4 + j) : pair(8 * n + j);
+            for (int j = 0; j < 4; ++j) A[t][n][j] = hh && !TWICE ? pair(8 * n + 4 + j) : pair(8 * n + j);
         if (hh == 0)
 #pragma unroll
             for (int e = 0; e < SUB; ++e) tab[k * SUB + e] = k < a.K ? c[e] : FAR_NUMBER;
@@ -138,11 +145,14 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
         return *reinterpret_cast<const Numbers<T, SUB> *>(x0 + t * a.token_stride[which]);
     };
     Numbers<T, SUB> next;
-    if (begin < end) next = fetch(begin + col);
-    for (int64_t t0 = begin; t0 < end; t0 += 32) {
+    if (begin < end) next = fetch(begin + lane);
+    for (int64_t t0 = begin; t0 < end; t0 += 64) {
+        // A lane has a vector of its own.  Step 1 takes the lower 32 lanes' and then the upper 32 lanes', the rest all 64.
         const Numbers<T, SUB> raw = next;
-        if (t0 + 32 < end) next = fetch(t0 + 32 + col);
-        const int64_t token = t0 + col;
+        if (t0 + 64 < end) next = fetch(t0 + 64 + lane);
+        const int64_t token = t0 + lane;
+        int64_t slot = -1;
+        if constexpr (!TRAIN) slot = a.slots[token < end ? token : end - 1];
         float x[SUB], size = 0.0f;
         uint32_t xp[XP][H2];
 #pragma unroll
@@ -158,19 +168,13 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
 #pragma unroll
             for (int p = 0; p < XP; ++p) xp[p][i] = p0[p] | p1[p] << 16;
         }
-        auto pair = [&](int s) -> uint32_t {
-            return s < TM.n * H2 ? xp[TM.x[s / H2]][s % H2] : s == TM.n * H2 ? 0x3f803f80u : s == TM.n * H2 + 1 ? 0x3f80u : 0u;
+        auto pair = [](int s, uint32_t const (&of)[XP][H2]) -> uint32_t {
+            return s < TM.n * H2 ? of[TM.x[s / H2]][s % H2] : s == TM.n * H2 ? 0x3f803f80u : s == TM.n * H2 + 1 ? 0x3f80u : 0u;
         };
-        u32x4 B[NM];
-#pragma unroll
-        for (int n = 0; n < NM; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) B[n][j] = hh ? pair(8 * n + 4 + j) : pair(8 * n + j);
-
         // step 1
-        float m1 = FAR_SCORE * 3.0f, m2 = FAR_SCORE * 3.0f;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        float m1[2], m2[2];
+        m1[0] = m1[1] = m2[0] = m2[1] = FAR_SCORE * 3.0f;
+        auto score = [&](int half, int t, u32x4 const (&B)[NM]) {
             f32x16 s = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
             for (int n = 0; n < NM; ++n)
@@ -181,43 +185,67 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) v = fminf(fminf(v, s[8 * q + i]), s[8 * q + i + 1]);
                 const float key = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) & ~15u) | (uint32_t)(2 * t + q));
-                m2 = __builtin_amdgcn_fmed3f(m1, m2, key);
-                m1 = least(m1, key);
+                m2[half] = __builtin_amdgcn_fmed3f(m1[half], m2[half], key);
+                m1[half] = least(m1[half], key);
+            }
+        };
+        if constexpr (TWICE) {
+            u32x4 B[2][NM];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t own = pair(j, xp);
+                B[0][0][j] = hh ? 0u : own, B[1][0][j] = hh ? own : 0u;
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) score(0, t, B[0]), score(1, t, B[1]);
+        } else {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t of[XP][H2];
+#pragma unroll
+                for (int p = 0; p < XP; ++p)
+#pragma unroll
+                    for (int i = 0; i < H2; ++i) of[p][i] = __builtin_amdgcn_permlane32_swap(xp[p][i], xp[p][i], false, false)[half];
+                u32x4 B[NM];
+#pragma unroll
+                for (int n = 0; n < NM; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) B[n][j] = hh ? pair(8 * n + 4 + j, of) : pair(8 * n + j, of);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) score(half, t, B);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        float l1, h1, l2, h2;
-        halves(m1, l1, h1);
-        halves(m2, l2, h2);
+        float l1 = m1[0], h1 = m1[1], l2 = m2[0], h2 = m2[1];
+        to_owners(l1, h1);
+        to_owners(l2, h2);
         const bool upper = h1 < l1;
         const float best = upper ? h1 : l1, second = least(upper ? l1 : h1, least(l2, h2));
         const float bound = 0.5f * reach + __builtin_amdgcn_sqrtf(size) * far;
         bool open = !(second - best > bound * 1.52587890625e-5f + 1e-36f) || !(bound < BOUND_MOST) || !(size < SIZE_MOST);
         const int group = __builtin_bit_cast(uint32_t, best) & 15;
 
-        // step 2: the two halves of a wave take four codewords each
+        // step 2: rows k0 to k0 + 3 and k0 + 8 to k0 + 11
         const int k0 = group * 16 + 4 * (int)upper;
         uint32_t d1 = 0x7f800000u, d2 = 0x7f800000u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 8; ++j) {
             float d = 0.0f;
 #pragma unroll
             for (int e = 0; e < SUB; ++e) {
-                const float v = x[e] - tab[(k0 + 8 * hh + j) * SUB + e];
+                const float v = x[e] - tab[(k0 + j + (j & 4)) * SUB + e];
                 d = __builtin_fmaf(v, v, d);
             }
-            const uint32_t key = (__builtin_bit_cast(uint32_t, d) & ~3u) | j;
+            const uint32_t key = (__builtin_bit_cast(uint32_t, d) & ~7u) | j;
             d2 = max(min(d1, d2), min(max(d1, d2), key));
             d1 = min(d1, key);
         }
-        const auto r1 = __builtin_amdgcn_permlane32_swap(d1, d1, false, false);
-        const auto r2 = __builtin_amdgcn_permlane32_swap(d2, d2, false, false);
-        const bool right = r1[1] < r1[0];
-        const uint32_t near = right ? r1[1] : r1[0], other = min(right ? r1[0] : r1[1], min(r2[0], r2[1]));
-        open = open || !(__builtin_bit_cast(float, other) > __builtin_bit_cast(float, near) * 1.00000763f + 1e-36f);
-        int code = k0 + (right ? 8 : 0) + (int)(near & 3u);
+        open = open || !(__builtin_bit_cast(float, d2) > __builtin_bit_cast(float, d1) * 1.00000763f + 1e-36f);
+        const int nth = d1 & 7u;
+        int code = k0 + nth + (nth & 4);
 
         // step 3
-        uint64_t todo = __ballot(open && token < end) & 0xffffffffu;
+        uint64_t todo = __ballot(open && token < end);
         while (todo) {
             const int v = __builtin_ctzll(todo);
             todo &= todo - 1;
@@ -241,16 +269,14 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
                 const int k_o = __shfl_xor(k_best, o);
                 if (d_o < d || (d_o == d && k_o < k_best)) d = d_o, k_best = k_o;
             }
-            if (col == v) code = k_best < 256 ? k_best : 0;
+            if (lane == v) code = k_best < 256 ? k_best : 0;
         }
 
         if constexpr (!TRAIN) {
-            const int64_t slot = hh == 0 && token < end ? a.slots[token] : -1;
-            if (slot >= 0 && slot < a.pages * a.page) {
+            if (token < end && slot >= 0 && slot < slots) {
                 const int64_t p = a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page;
                 const int o = (int)(slot - p * a.page);
-                if (which == 0) a.k_codes[((p * a.heads + h) * a.page + o) * parts + m] = (uint8_t)code;
-                else a.v_codes[((p * a.heads + h) * parts + m) * a.page + o] = (uint8_t)code;
+                codes[p * page_bytes + (which == 0 ? o * parts : o)] = (uint8_t)code;
             }
         } else {
             bool fine = token < end;
@@ -258,55 +284,57 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
             for (int e = 0; e < SUB; ++e) fine = fine && fabsf(x[e]) < COUNTED;
             // sums by products with the one-hot numbers of the codewords: number = 16 hi + lo, and
             // sum[hi][lo] = sum over vectors of (x where its hi is this row) * (1 where its lo is this column)
-            if (hh == 0) {
-                if (fine) {
-                    double f = 0.0;
+            if (fine) {
+                double f = 0.0;
 #pragma unroll
-                    for (int e = 0; e < SUB; ++e) {
-                        const double w = (double)x[e] - (double)tab[code * SUB + e];
-                        f += w * w;
-                    }
-                    away += f <= INFINITY ? f : INFINITY;
+                for (int e = 0; e < SUB; ++e) {
+                    const double w = (double)x[e] - (double)tab[code * SUB + e];
+                    f += w * w;
                 }
-                s_lab[wave][col] = fine ? (int16_t)code : (int16_t)-1;
+                away += f <= INFINITY ? f : INFINITY;
+            }
+            s_lab[wave][lane] = fine ? (int16_t)code : (int16_t)-1;
 #pragma unroll
-                for (int i = 0; i < H2; ++i) {
-                    uint32_t p0[XP], p1[XP];
-                    split<XP>(x[2 * i] * SUM_SCALE, p0);
-                    split<XP>(x[2 * i + 1] * SUM_SCALE, p1);
+            for (int i = 0; i < H2; ++i) {
+                uint32_t p0[XP], p1[XP];
+                split<XP>(x[2 * i] * SUM_SCALE, p0);
+                split<XP>(x[2 * i + 1] * SUM_SCALE, p1);
 #pragma unroll
-                    for (int p = 0; p < XP; ++p) s_x[wave][p][col][i] = p0[p] | p1[p] << 16;
-                }
+                for (int p = 0; p < XP; ++p) s_x[wave][p][lane][i] = p0[p] | p1[p] << 16;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             const int row = lane & 15, g = lane >> 4;
-            u32x4 member, lows;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int la = s_lab[wave][8 * g + 2 * j], lb = s_lab[wave][8 * g + 2 * j + 1];
-                member[j] = ((la >> 4) == row ? 0xffffu : 0u) | ((lb >> 4) == row ? 0xffff0000u : 0u);
-                lows[j] = ((la & 15) == row ? 0x3f80u : 0u) | ((lb & 15) == row ? 0x3f800000u : 0u);
-            }
-            const bf16x8 lo8 = __builtin_bit_cast(bf16x8, lows);
+            for (int half = 0; half < 2; ++half) {
+                const int first = 32 * half + 8 * g;
+                u32x4 member, lows;
 #pragma unroll
-            for (int p = 0; p < XP; ++p)
-#pragma unroll
-                for (int i = 0; i < H2; ++i) {
-                    u32x4 e0, e1;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t va = s_x[wave][p][8 * g + 2 * j][i], vb = s_x[wave][p][8 * g + 2 * j + 1][i];
-                        e0[j] = __builtin_amdgcn_perm(vb, va, 0x05040100u) & member[j];
-                        e1[j] = __builtin_amdgcn_perm(vb, va, 0x07060302u) & member[j];
-                    }
-                    sum[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e0), lo8, sum[2 * i], 0, 0, 0);
-                    sum[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e1), lo8, sum[2 * i + 1], 0, 0, 0);
+                for (int j = 0; j < 4; ++j) {
+                    const int la = s_lab[wave][first + 2 * j], lb = s_lab[wave][first + 2 * j + 1];
+                    member[j] = ((la >> 4) == row ? 0xffffu : 0u) | ((lb >> 4) == row ? 0xffff0000u : 0u);
+                    lows[j] = ((la & 15) == row ? 0x3f80u : 0u) | ((lb & 15) == row ? 0x3f800000u : 0u);
                 }
-            u32x4 ones;
+                const bf16x8 lo8 = __builtin_bit_cast(bf16x8, lows);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) ones[j] = member[j] & 0x3f803f80u;
-            sum[SUB] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), lo8, sum[SUB], 0, 0, 0);
+                for (int p = 0; p < XP; ++p)
+#pragma unroll
+                    for (int i = 0; i < H2; ++i) {
+                        u32x4 e0, e1;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t va = s_x[wave][p][first + 2 * j][i], vb = s_x[wave][p][first + 2 * j + 1][i];
+                            e0[j] = __builtin_amdgcn_perm(vb, va, 0x05040100u) & member[j];
+                            e1[j] = __builtin_amdgcn_perm(vb, va, 0x07060302u) & member[j];
+                        }
+                        sum[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e0), lo8, sum[2 * i], 0, 0, 0);
+                        sum[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e1), lo8, sum[2 * i + 1], 0, 0, 0);
+                    }
+                u32x4 ones;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ones[j] = member[j] & 0x3f803f80u;
+                sum[SUB] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), lo8, sum[SUB], 0, 0, 0);
+            }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
@@ -318,7 +346,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
 #pragma unroll
             for (int i = 0; i < 4; ++i) a.part_sums[(place * (SUB + 1) + e) * 256 + (4 * (lane >> 4) + i) * 16 + (lane & 15)] = sum[e][i];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) away += __shfl_xor(away, o);
+        for (int o = 1; o < 64; o <<= 1) away += __shfl_xor(away, o);
         if (lane == 0) a.part_dist[place] = away;
     }
 }
@@ -397,12 +425,12 @@ SearchPlan vq_internal_search_plan(int64_t tokens, int heads, int dim, int sub, 
     const int64_t base = (int64_t)heads * (parts / p.pw) * both;
     // A write is spread as thinly as there are tokens; a training chunk of fewer than 128 costs more to gather than it saves, and none is
     // longer than 4096: its sums are fp32.
-    const int fewest = both == 2 ? 32 : 128, longest = both == 2 ? 1 << 24 : 4096;
+    const int fewest = both == 2 ? 64 : 128, longest = both == 2 ? 1 << 24 : 4096;
     const int64_t most = (tokens + fewest * side - 1) / (fewest * side), least = (tokens + longest * side - 1) / (longest * side);
     int64_t n = (2 * CUS + base - 1) / base;
     n = n < most ? n : most;
     n = n > least ? n : least;
-    p.chunk = (int)(((tokens + n * side - 1) / (n * side) + 31) / 32 * 32);
+    p.chunk = (int)(((tokens + n * side - 1) / (n * side) + 63) / 64 * 64);
     p.blocks = (int)((tokens + p.chunk * side - 1) / (p.chunk * side));
     p.chunks = (int)(p.blocks * side);
     return p;
