@@ -64,6 +64,10 @@ __device__ inline void to_owners(float &a, float &b) {
 // The lesser of two finite scores, without the canonicalisation that fminf of unknown bits brings.
 __device__ inline float least(float a, float b) { return __builtin_amdgcn_fmed3f(-FAR_SCORE * 3.0f, a, b); }
 
+// Where codeword k starts in a wave's table in LDS: 16 rows and a pad, so that the same rows of different groups, which is what the lanes
+// ask for at once in step 2, lie in different banks.
+template <int SUB> __device__ constexpr int row_at(int k) { return k * SUB + (k >> 4) * (SUB < 4 ? 2 : 4); }
+
 // T: the vectors' type, C: the codebook's; NT: groups of 32 codewords.
 template <typename T, typename C, int SUB, int NT, bool TRAIN>
 __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const SearchArgs a) {
@@ -73,7 +77,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
     // Where a vector's slots fit into one half of the operand, the codewords stand in both: a lane of the upper half then
     // gives its own vector's numbers there, and none have to be moved.
     constexpr bool TWICE = PAIRS <= 4;
-    __shared__ float s_tab[SEARCH_WAVES][NT * 32 * SUB];
+    __shared__ __align__(16) float s_tab[SEARCH_WAVES][row_at<SUB>(NT * 32)];
     __shared__ int16_t s_lab[TRAIN ? SEARCH_WAVES : 1][64];
     __shared__ __align__(16) uint32_t s_x[TRAIN ? SEARCH_WAVES : 1][XP][64][H2];
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
@@ -128,7 +132,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
             for (int j = 0; j < 4; ++j) A[t][n][j] = hh && !TWICE ? pair(8 * n + 4 + j) : pair(8 * n + j);
         if (hh == 0)
 #pragma unroll
-            for (int e = 0; e < SUB; ++e) tab[k * SUB + e] = k < a.K ? c[e] : FAR_NUMBER;
+            for (int e = 0; e < SUB; ++e) tab[row_at<SUB>(k) + e] = k < a.K ? c[e] : FAR_NUMBER;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) reach = fmaxf(reach, __shfl_xor(reach, o));
@@ -226,22 +230,22 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
         const int group = __builtin_bit_cast(uint32_t, best) & 15;
 
         // step 2: rows k0 to k0 + 3 and k0 + 8 to k0 + 11
-        const int k0 = group * 16 + 4 * (int)upper;
-        uint32_t d1 = 0x7f800000u, d2 = 0x7f800000u;
+        const int k0 = group * 16 + 4 * (int)upper, at0 = row_at<SUB>(group * 16) + (upper ? 4 * SUB : 0);
+        float d1 = FAR_SCORE * 3.0f, d2 = FAR_SCORE * 3.0f;               // (what is not finite here is open already)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             float d = 0.0f;
 #pragma unroll
             for (int e = 0; e < SUB; ++e) {
-                const float v = x[e] - tab[(k0 + j + (j & 4)) * SUB + e];
+                const float v = x[e] - tab[at0 + (j + (j & 4)) * SUB + e];
                 d = __builtin_fmaf(v, v, d);
             }
-            const uint32_t key = (__builtin_bit_cast(uint32_t, d) & ~7u) | j;
-            d2 = max(min(d1, d2), min(max(d1, d2), key));
-            d1 = min(d1, key);
+            const float key = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, d) & ~7u) | j);
+            d2 = __builtin_amdgcn_fmed3f(d1, d2, key);
+            d1 = least(d1, key);
         }
-        open = open || !(__builtin_bit_cast(float, d2) > __builtin_bit_cast(float, d1) * 1.00000763f + 1e-36f);
-        const int nth = d1 & 7u;
+        open = open || !(d2 > d1 * 1.00000763f + 1e-36f);
+        const int nth = __builtin_bit_cast(uint32_t, d1) & 7u;
         int code = k0 + nth + (nth & 4);
 
         // step 3
@@ -258,7 +262,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
                 double f = 0.0;
 #pragma unroll
                 for (int e = 0; e < SUB; ++e) {
-                    const double w = y[e] - (double)tab[k * SUB + e];
+                    const double w = y[e] - (double)tab[row_at<SUB>(k) + e];
                     f += w * w;
                 }
                 if (f < d) d = f, k_best = k;
@@ -288,7 +292,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
                 double f = 0.0;
 #pragma unroll
                 for (int e = 0; e < SUB; ++e) {
-                    const double w = (double)x[e] - (double)tab[code * SUB + e];
+                    const double w = (double)x[e] - (double)tab[row_at<SUB>(code) + e];
                     f += w * w;
                 }
                 away += f <= INFINITY ? f : INFINITY;
