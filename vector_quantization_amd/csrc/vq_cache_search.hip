@@ -4,9 +4,9 @@
 // which hands on what it cannot decide:
 //   1. Scores 1/2 |c|^2 - x.c of 32 vectors against 32 codewords at a time, v_mfma 32x32x16 bf16.  Numbers of wider types go in as two or three
 //      bf16 pieces each, and 1/2 |c|^2 as three further terms against ones, so a score comes out of the matrix unit whole.  A lane keeps the two
-//      least of the minima over groups of 8 codewords, the group's number in the low bits.  With B = 1/2 max |c|^2 + |x| max |c|, every
-//      score is off by at most 2^-18 B (up to 64 additions in fp32, dropped pieces, the group number), so a second-best group more
-//      than 2^-16 B behind holds no nearest codeword.
+//      least of the minima over groups of 8 codewords, the group's number in the low bits.  With B = 1/2 max |c|^2 + |x| max |c|, a
+//      score is off by 2^-18.5 B (bf16, 4 numbers) to 2^-16.7 B (fp32, 8 numbers): additions in fp32, dropped pieces, the group's number.
+//      A second-best group more than twice that behind (GAP) holds no nearest codeword.
 //   2. The 8 codewords of the best group by direct differences in fp32, each sum off by less than 2^-19 of itself.
 //   3. Vectors that either step leaves open (close calls, ties, values beyond fp32's range, what is not finite) are searched by the whole wave
 //      in fp64, by the definition: about one in a hundred.
@@ -61,6 +61,26 @@ __device__ inline void to_owners(float &a, float &b) {
     b = __builtin_bit_cast(float, second);
 }
 
+// The least of all lanes' numbers, in all.
+template <int CONTROL, int ROWS> __device__ inline uint32_t min_with(uint32_t v) {      // (a lane that the control names no other for: with itself)
+    return min(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CONTROL, ROWS, 0xf, false));
+}
+__device__ inline uint32_t wave_min(uint32_t v) {
+    v = min_with<0x111, 0xf>(v);     // one, two, four and eight lanes to the right inside a row of 16
+    v = min_with<0x112, 0xf>(v);
+    v = min_with<0x114, 0xf>(v);
+    v = min_with<0x118, 0xf>(v);
+    v = min_with<0x142, 0xa>(v);     // the last lane of a row to all of the next, for the second and the fourth
+    v = min_with<0x143, 0xc>(v);     // lane 31 to the upper half
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// All ones in each half of `labels` that equals that of `row`, zeros in the other.
+__device__ inline uint32_t equal_halves(uint32_t labels, uint32_t row) {
+    const u16x2 one = {1, 1};
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, labels ^ row), one) - one);
+}
+
 // The lesser of two finite scores, without the canonicalisation that fminf of unknown bits brings.
 __device__ inline float least(float a, float b) { return __builtin_amdgcn_fmed3f(-FAR_SCORE * 3.0f, a, b); }
 
@@ -78,8 +98,8 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
     // gives its own vector's numbers there, and none have to be moved.
     constexpr bool TWICE = PAIRS <= 4;
     __shared__ __align__(16) float s_tab[SEARCH_WAVES][row_at<SUB>(NT * 32)];
-    __shared__ int16_t s_lab[TRAIN ? SEARCH_WAVES : 1][64];
-    __shared__ __align__(16) uint32_t s_x[TRAIN ? SEARCH_WAVES : 1][XP][64][H2];
+    __shared__ __align__(16) uint16_t s_hi[TRAIN ? SEARCH_WAVES : 1][64], s_lo[TRAIN ? SEARCH_WAVES : 1][64];
+    __shared__ __align__(16) uint16_t s_x[TRAIN ? SEARCH_WAVES : 1][XP][SUB][64];
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int which = blockIdx.z, parts = a.dim / SUB, per = parts / a.pw;
@@ -94,6 +114,10 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
 
     const int64_t slots = a.pages * a.page, page_bytes = (int64_t)a.heads * a.page * parts;
     uint8_t *codes = which == 0 ? a.k_codes + (int64_t)h * a.page * parts + m : a.v_codes + ((int64_t)h * parts + m) * a.page;
+
+    // See above: twice what a score may be off by, in steps of 2^-23 B.  Additions (a step each, whichever way the unit rounds), the group's
+    // number, dropped pieces, the norm's own sum; two steps for B, which is rounded too.
+    constexpr float GAP = 2 * (TM.n * SUB + 3 + 16 + 2 + SUB / 2 + 2) * 0x1p-23f;
 
     // the codewords: operand of step 1, and in fp32 for steps 2 and 3; rows past K lie far away
     u32x4 A[NT][NM];
@@ -226,7 +250,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
         const bool upper = h1 < l1;
         const float best = upper ? h1 : l1, second = least(upper ? l1 : h1, least(l2, h2));
         const float bound = 0.5f * reach + __builtin_amdgcn_sqrtf(size) * far;
-        bool open = !(second - best > bound * 1.52587890625e-5f + 1e-36f) || !(bound < BOUND_MOST) || !(size < SIZE_MOST);
+        bool open = !(second - best > bound * GAP + 1e-36f) || !(bound < BOUND_MOST) || !(size < SIZE_MOST);
         const int group = __builtin_bit_cast(uint32_t, best) & 15;
 
         // step 2: rows k0 to k0 + 3 and k0 + 8 to k0 + 11
@@ -257,23 +281,24 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
 #pragma unroll
             for (int e = 0; e < SUB; ++e) y[e] = (double)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x[e]), v));
             double d = INFINITY;
-            int k_best = 256;
-            for (int k = lane; k < a.K; k += 64) {
+            uint32_t k_best = 256;
+#pragma unroll 2
+            for (int k = lane; k < NT * 32; k += 64) {
                 double f = 0.0;
 #pragma unroll
                 for (int e = 0; e < SUB; ++e) {
                     const double w = y[e] - (double)tab[row_at<SUB>(k) + e];
                     f += w * w;
                 }
-                if (f < d) d = f, k_best = k;
+                if (k < a.K && f < d) d = f, k_best = k;
             }
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double d_o = __shfl_xor(d, o);
-                const int k_o = __shfl_xor(k_best, o);
-                if (d_o < d || (d_o == d && k_o < k_best)) d = d_o, k_best = k_o;
-            }
-            if (lane == v) code = k_best < 256 ? k_best : 0;
+            // distances are not negative: their bits are in their order, the upper halves first
+            const uint64_t bits = __builtin_bit_cast(uint64_t, d);
+            const uint32_t high = wave_min((uint32_t)(bits >> 32));
+            uint32_t low = (uint32_t)(bits >> 32) == high ? (uint32_t)bits : ~0u;
+            const uint32_t lowest = wave_min(low);
+            const uint32_t k_least = wave_min((uint32_t)(bits >> 32) == high && low == lowest ? k_best : 256u);
+            if (lane == v) code = k_least < 256u ? (int)k_least : 0;
         }
 
         if constexpr (!TRAIN) {
@@ -297,46 +322,36 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
                 }
                 away += f <= INFINITY ? f : INFINITY;
             }
-            s_lab[wave][lane] = fine ? (int16_t)code : (int16_t)-1;
+            s_hi[wave][lane] = fine ? (uint16_t)(code >> 4) : (uint16_t)0xffff;
+            s_lo[wave][lane] = (uint16_t)(code & 15);
 #pragma unroll
-            for (int i = 0; i < H2; ++i) {
-                uint32_t p0[XP], p1[XP];
-                split<XP>(x[2 * i] * SUM_SCALE, p0);
-                split<XP>(x[2 * i + 1] * SUM_SCALE, p1);
+            for (int e = 0; e < SUB; ++e) {
+                uint32_t piece[XP];
+                split<XP>(x[e] * SUM_SCALE, piece);
 #pragma unroll
-                for (int p = 0; p < XP; ++p) s_x[wave][p][lane][i] = p0[p] | p1[p] << 16;
+                for (int p = 0; p < XP; ++p) s_x[wave][p][e][lane] = (uint16_t)piece[p];
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            const int row = lane & 15, g = lane >> 4;
+            const uint32_t row = (lane & 15) * 0x10001u;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int first = 32 * half + 8 * g;
-                u32x4 member, lows;
+                const int first = 32 * half + 8 * (lane >> 4);
+                u32x4 member = *reinterpret_cast<const u32x4 *>(&s_hi[wave][first]), lows = *reinterpret_cast<const u32x4 *>(&s_lo[wave][first]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int la = s_lab[wave][first + 2 * j], lb = s_lab[wave][first + 2 * j + 1];
-                    member[j] = ((la >> 4) == row ? 0xffffu : 0u) | ((lb >> 4) == row ? 0xffff0000u : 0u);
-                    lows[j] = ((la & 15) == row ? 0x3f80u : 0u) | ((lb & 15) == row ? 0x3f800000u : 0u);
+                    member[j] = equal_halves(member[j], row);
+                    lows[j] = equal_halves(lows[j], row) & 0x3f803f80u;
                 }
                 const bf16x8 lo8 = __builtin_bit_cast(bf16x8, lows);
 #pragma unroll
                 for (int p = 0; p < XP; ++p)
 #pragma unroll
-                    for (int i = 0; i < H2; ++i) {
-                        u32x4 e0, e1;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t va = s_x[wave][p][first + 2 * j][i], vb = s_x[wave][p][first + 2 * j + 1][i];
-                            e0[j] = __builtin_amdgcn_perm(vb, va, 0x05040100u) & member[j];
-                            e1[j] = __builtin_amdgcn_perm(vb, va, 0x07060302u) & member[j];
-                        }
-                        sum[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e0), lo8, sum[2 * i], 0, 0, 0);
-                        sum[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e1), lo8, sum[2 * i + 1], 0, 0, 0);
+                    for (int e = 0; e < SUB; ++e) {
+                        const u32x4 of = *reinterpret_cast<const u32x4 *>(&s_x[wave][p][e][first]) & member;
+                        sum[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, of), lo8, sum[e], 0, 0, 0);
                     }
-                u32x4 ones;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) ones[j] = member[j] & 0x3f803f80u;
+                const u32x4 ones = member & 0x3f803f80u;
                 sum[SUB] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), lo8, sum[SUB], 0, 0, 0);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
