@@ -1,6 +1,7 @@
 // vq_cache.hip -- HIP kernels (gfx950 / CDNA4) and C ABI of the vector-quantised key-value cache (vq_cache.h).
 #include <stdarg.h>
 #include <stdio.h>
+#include <type_traits>
 
 #include "vq_cache_internal.h"
 
@@ -37,89 +38,156 @@ struct ReadArgs {
     void *out[2];
 };
 
-// Codes -> vectors.  A workgroup holds one head's codebook in LDS (both cache types have 2 bytes a number) and expands `chunk` tokens; a
-// thread writes 16 bytes, 8 numbers of 8 / SUB codewords.  Neighbouring threads read neighbouring parts, so the look-ups
-// never clash in the banks.  Bound by the writes.
-template <int D, int SUB, bool LDS>
-__global__ __launch_bounds__(512) void k_cache_read(const ReadArgs a) {
+// Codes -> vectors.  A thread writes 16 bytes, 8 numbers of 8 / SUB codewords; neighbouring threads write neighbouring ones.
+
+// The 16 bytes that N codes stand for, at place c of a vector.
+template <int D, int SUB> __device__ inline u32x4 expand(const uint8_t *book, uint32_t codes, int K, int c) {
+    u32x4 v;
+#pragma unroll
+    for (int j = 0; j < 8 / SUB; ++j) {
+        const int code = codes >> (8 * j) & 255u, k = code < K ? code : K - 1;
+        const uint8_t *w = book + k * (D * 2) + c * 16 + j * (SUB * 2);
+        if constexpr (SUB == 8) v = *reinterpret_cast<const u32x4 *>(w);
+        else if constexpr (SUB == 4) {
+            const u32x2 x = *reinterpret_cast<const u32x2 *>(w);
+            v[2 * j] = x.x, v[2 * j + 1] = x.y;
+        } else v[j] = *reinterpret_cast<const uint32_t *>(w);
+    }
+    return v;
+}
+// Where the codes of a slot lie: the head's first byte of its page, and its place in the page.  A slot outside the cache: false.
+__device__ inline bool locate(const ReadArgs &a, int64_t slot, int64_t page_bytes, int64_t &from, int &o) {
+    if (slot < 0 || slot >= a.pages * a.page) return false;
+    const int64_t p = a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page;
+    from = p * page_bytes;
+    o = (int)(slot - p * a.page);
+    return true;
+}
+
+// A few tokens: everything comes out of the caches.
+template <int D, int SUB>
+__global__ __launch_bounds__(512) void k_cache_read_few(const ReadArgs a) {
     constexpr int M = D / SUB, CH = D / 8, N = 8 / SUB;
-    extern __shared__ __align__(16) uint8_t s_book[];
     const int h = blockIdx.x, which = blockIdx.z;
     const uint8_t *book = static_cast<const uint8_t *>(a.cb[which]) + (a.cb_heads == 1 ? 0 : (int64_t)h * a.K * D * 2);
-    if constexpr (LDS) {
-        for (int i = threadIdx.x; i < a.K * CH; i += 512)
-            reinterpret_cast<u32x4 *>(s_book)[i] = reinterpret_cast<const u32x4 *>(book)[i];
-        __syncthreads();
-    }
     const int64_t begin = (int64_t)blockIdx.y * a.chunk, end = begin + a.chunk < a.tokens ? begin + a.chunk : a.tokens;
-    const int64_t slots = a.pages * a.page;
     const uint8_t *codes = a.codes[which] + (int64_t)h * a.page * M;
     uint8_t *out = static_cast<uint8_t *>(a.out[which]);
-    // Four pieces a turn in a long read: slots, codes and look-ups of all four are under way together (65536 tokens of 8 heads and 128
-    // dims: 103 -> 92 us).  A short one has no four to take.
-    constexpr int AT_ONCE = LDS ? 4 : 1;
-    for (int64_t i0 = begin * CH + threadIdx.x; i0 < end * CH; i0 += AT_ONCE * 512) {
-        int64_t slot[AT_ONCE];
-        int code[AT_ONCE][N];
+    for (int64_t i = begin * CH + threadIdx.x; i < end * CH; i += 512) {
+        const int c = (int)(i % CH);
+        int64_t from;
+        int o;
+        u32x4 v = {0, 0, 0, 0};
+        if (locate(a, a.slots[i / CH], (int64_t)a.heads * a.page * M, from, o)) {
+            uint32_t w = 0;
 #pragma unroll
-        for (int n = 0; n < AT_ONCE; ++n) {
-            const int64_t i = i0 + n * 512;
-            slot[n] = i < end * CH ? a.slots[i / CH] : -1;
+            for (int j = 0; j < N; ++j)
+                w |= (uint32_t)codes[from + (which == 0 ? (int64_t)o * M + c * N + j : (int64_t)(c * N + j) * a.page + o)] << (8 * j);
+            v = expand<D, SUB>(book, w, a.K, c);
         }
+        *reinterpret_cast<u32x4 *>(out + (i / CH * a.heads + h) * (D * 2) + c * 16) = v;
+    }
+}
+
+// Many: a workgroup holds one head's codebook in LDS (both cache types have 2 bytes a number) and expands `chunk` tokens, READ_TOKENS at a
+// time.  Their codes pass through LDS, where those of the next are put once they have come, so that they are fetched the way they lie: a
+// key's side by side, of the values one part of neighbouring tokens.  (Fetched as they are used, by threads of neighbouring parts,
+// the values' bytes came out of 16 lines a load, and reading the values took 85 us where the keys took 50.)
+constexpr int READ_TOKENS = 128;
+constexpr int read_row(int M) { return M + 4; }           // a token's codes in LDS, padded: the stores of one part go to different banks
+template <int D, int SUB>
+__global__ __launch_bounds__(512) void k_cache_read(const ReadArgs a) {
+    constexpr int M = D / SUB, CH = D / 8, N = 8 / SUB, ROW = read_row(M);
+    constexpr int WORDS = READ_TOKENS * M / 4, EACH_K = (WORDS + 511) / 512, EACH_V = M / 4;     // fetches a thread: words of keys' codes, values' bytes
+    extern __shared__ __align__(16) uint8_t s_book[];
+    uint8_t *s_codes = s_book + (size_t)a.K * D * 2;
+    uint8_t *s_there = s_codes + READ_TOKENS * ROW;
+    const int h = blockIdx.x, which = blockIdx.z;
+    const uint8_t *book = static_cast<const uint8_t *>(a.cb[which]) + (a.cb_heads == 1 ? 0 : (int64_t)h * a.K * D * 2);
+    for (int i = threadIdx.x; i < a.K * CH; i += 512) reinterpret_cast<u32x4 *>(s_book)[i] = reinterpret_cast<const u32x4 *>(book)[i];
+    const int64_t begin = (int64_t)blockIdx.y * a.chunk, end = begin + a.chunk < a.tokens ? begin + a.chunk : a.tokens;
+    const int64_t page_bytes = (int64_t)a.heads * a.page * M;
+    const uint8_t *codes = a.codes[which] + (int64_t)h * a.page * M;
+    uint8_t *out = static_cast<uint8_t *>(a.out[which]);
+
+    auto find = [&](int64_t token, int64_t &from, int &o) -> bool { return token < end && locate(a, a.slots[token], page_bytes, from, o); };
+    auto work = [&](auto keys) {                                  // (both sides' loops apart: each with its own registers)
+        constexpr bool KEYS = decltype(keys)::value;
+        constexpr int EACH = KEYS ? EACH_K : EACH_V;
+        uint32_t got[EACH];
+        bool there[KEYS ? EACH : 1];
+        auto fetch = [&](int64_t t0) {
+            int64_t from = 0;
+            int o = 0;
+            if constexpr (KEYS) {
 #pragma unroll
-        for (int n = 0; n < AT_ONCE; ++n) {
-            const int c = (int)((i0 + n * 512) % CH);
-            const bool there = slot[n] >= 0 && slot[n] < slots;
-            const int64_t at = there ? slot[n] : 0, p = a.page_shift >= 0 ? at >> a.page_shift : at / a.page;
-            const int o = (int)(at - p * a.page);
-            const uint8_t *q = codes + p * a.heads * a.page * M;
-            if (which == 0) {                                     // a key's codes lie side by side
-                q += (int64_t)o * M + c * N;
+                for (int n = 0; n < EACH; ++n) {
+                    const int i = threadIdx.x + n * 512;
+                    got[n] = 0;
+                    there[n] = i < WORDS && find(t0 + i / (M / 4), from, o);
+                    if (there[n]) got[n] = *reinterpret_cast<const uint32_t *>(codes + from + (int64_t)o * M + i % (M / 4) * 4);
+                }
+            } else {
+                there[0] = find(t0 + threadIdx.x % READ_TOKENS, from, o);
+#pragma unroll
+                for (int n = 0; n < EACH; ++n) {
+                    got[n] = 0;
+                    if (there[0]) got[n] = codes[from + (int64_t)(threadIdx.x / READ_TOKENS + 4 * n) * a.page + o];
+                }
+            }
+        };
+        auto put = [&]() {
+            if constexpr (KEYS) {
+#pragma unroll
+                for (int n = 0; n < EACH; ++n) {
+                    const int i = threadIdx.x + n * 512, t = i / (M / 4), w = i % (M / 4);
+                    if (i >= WORDS) continue;
+                    *reinterpret_cast<uint32_t *>(s_codes + t * ROW + w * 4) = got[n];
+                    if (w == 0) s_there[t] = there[n];
+                }
+            } else {
+                const int t = threadIdx.x % READ_TOKENS, m = threadIdx.x / READ_TOKENS;
+#pragma unroll
+                for (int n = 0; n < EACH; ++n) s_codes[t * ROW + m + 4 * n] = (uint8_t)got[n];
+                if (m == 0) s_there[t] = there[0];
+            }
+        };
+        fetch(begin);
+        for (int64_t t0 = begin; t0 < end; t0 += READ_TOKENS) {
+            put();
+            __syncthreads();
+            if (t0 + READ_TOKENS < end) fetch(t0 + READ_TOKENS);
+            const int here = end - t0 < READ_TOKENS ? (int)(end - t0) : READ_TOKENS;
+#pragma unroll 4
+            for (int i = threadIdx.x; i < here * CH; i += 512) {
+                const int t = i / CH, c = i % CH;
+                const uint8_t *q = s_codes + t * ROW + c * N;
                 uint32_t w;
                 if constexpr (N == 1) w = *q;
                 else if constexpr (N == 2) w = *reinterpret_cast<const uint16_t *>(q);
                 else w = *reinterpret_cast<const uint32_t *>(q);
-#pragma unroll
-                for (int j = 0; j < N; ++j) code[n][j] = w >> (8 * j) & 255u;
-            } else {
-                q += (int64_t)c * N * a.page + o;
-#pragma unroll
-                for (int j = 0; j < N; ++j) code[n][j] = q[(int64_t)j * a.page];
+                u32x4 v = expand<D, SUB>(s_book, w, a.K, c);
+                if (!s_there[t]) v = (u32x4){0, 0, 0, 0};
+                *reinterpret_cast<u32x4 *>(out + ((t0 + t) * a.heads + h) * (D * 2) + c * 16) = v;
             }
-            if (!there) slot[n] = -1;
+            __syncthreads();
         }
-#pragma unroll
-        for (int n = 0; n < AT_ONCE; ++n) {
-            const int64_t i = i0 + n * 512;
-            if (i >= end * CH) continue;
-            const int c = (int)(i % CH);
-            u32x4 v = {0, 0, 0, 0};
-            if (slot[n] >= 0)
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const int k = code[n][j] < a.K ? code[n][j] : a.K - 1;
-                    const uint8_t *w = (LDS ? s_book : book) + k * (D * 2) + c * 16 + j * (SUB * 2);
-                    if constexpr (SUB == 8) v = *reinterpret_cast<const u32x4 *>(w);
-                    else if constexpr (SUB == 4) {
-                        const u32x2 x = *reinterpret_cast<const u32x2 *>(w);
-                        v[2 * j] = x.x, v[2 * j + 1] = x.y;
-                    } else v[j] = *reinterpret_cast<const uint32_t *>(w);
-                }
-            *reinterpret_cast<u32x4 *>(out + (i / CH * a.heads + h) * (D * 2) + c * 16) = v;
-        }
-    }
+    };
+    if (which == 0) work(std::true_type{});
+    else work(std::false_type{});
 }
 
 template <int D, int SUB> hipError_t launch_read(const ReadArgs &a, hipStream_t stream) {
     // A codebook that a workgroup's tokens outweigh goes to LDS; for a few tokens the look-ups go to the caches instead.
-    const size_t book = (size_t)a.K * D * 2;
+    const size_t lds = (size_t)a.K * D * 2 + READ_TOKENS * (read_row(D / SUB) + 1);
+    static_assert(256 * D * 2 + READ_TOKENS * (read_row(D / SUB) + 1) <= LDS_MOST, "codebook and codes fit into LDS");
     const dim3 grid(a.heads, (unsigned)((a.tokens + a.chunk - 1) / a.chunk), 2);
     if (a.chunk >= a.K) {
         static std::atomic<uint64_t> allowed{0};
-        const hipError_t e = vq_internal_allow_lds(reinterpret_cast<const void *>(k_cache_read<D, SUB, true>), allowed);
+        const hipError_t e = vq_internal_allow_lds(reinterpret_cast<const void *>(k_cache_read<D, SUB>), allowed);
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((k_cache_read<D, SUB, true>), grid, dim3(512), book, stream, a);
-    } else hipLaunchKernelGGL((k_cache_read<D, SUB, false>), grid, dim3(512), 0, stream, a);
+        hipLaunchKernelGGL((k_cache_read<D, SUB>), grid, dim3(512), lds, stream, a);
+    } else hipLaunchKernelGGL((k_cache_read_few<D, SUB>), grid, dim3(512), 0, stream, a);
     return hipGetLastError();
 }
 
