@@ -149,6 +149,32 @@ def test_write_and_read(eng, T, H, D, sub, K, page, dtype):
         assert torch.equal(got_v[:, h].cpu().double(), want_v)
 
 
+LONG_READ = [
+    (5001, 16, 32, 8, 256, 16, torch.bfloat16), (9000, 8, 64, 2, 100, 48, torch.float16), (8500, 8, 96, 8, 255, 16, torch.bfloat16),
+    (8449, 8, 96, 2, 256, 64, torch.float16), (9001, 8, 128, 4, 256, 64, torch.bfloat16), (9000, 8, 192, 2, 7, 16, torch.float16),
+    (8300, 8, 256, 2, 256, 16, torch.bfloat16), (20001, 8, 256, 4, 256, 128, torch.bfloat16), (5001, 16, 64, 4, 16, 32, torch.float16),
+]
+
+
+@pytest.mark.parametrize("T,H,D,sub,K,page,dtype", LONG_READ)
+def test_long_read(eng, T, H, D, sub, K, page, dtype):
+    """Reads that keep the codebook in LDS, several turns of a workgroup, the last one ragged; codes of no codeword, slots of no page, one slot twice."""
+    M, pages = D // sub, -(-T // page) + 2
+    kc, vc = (t.to(DEV) for t in random_codes(6, pages, H, page, M, 256))
+    cbs = [data(s, (H, K, D), dtype).to(DEV) for s in (3, 4)]
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(5))[:T]
+    slots[T // 2:] = slots[T // 2:].sort()[0]                            # half of them in order, as a prompt lies
+    slots[3], slots[7], slots[T - 1], slots[130] = -1, pages * page, -(1 << 60), slots[129]
+    slots = slots.to(DEV)
+    keep = (slots >= 0) & (slots < pages * page)
+    p, o = torch.where(keep, slots, 0) // page, torch.where(keep, slots, 0) % page
+    h, m = torch.arange(H, device=DEV)[:, None], torch.arange(M, device=DEV)
+    got = eng.cache_read(slots, *cbs, kc, vc)
+    for x, codes, cb in zip(got, (kc[p, :, o], vc[p, :, :, o]), cbs):
+        want = cb.reshape(H, K, M, sub)[h, codes.long().clamp(max=K - 1), m].reshape(T, H, D)
+        assert torch.equal(x, torch.where(keep[:, None, None], want, 0))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("case", ["grid", "huge", "tiny", "nonfinite", "far codeword", "bad codebook", "close", "offset"])
 def test_write_hard_values(eng, dtype, case):

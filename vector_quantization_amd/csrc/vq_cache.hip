@@ -95,7 +95,7 @@ __global__ __launch_bounds__(512) void k_cache_read_few(const ReadArgs a) {
 // the values' bytes came out of 16 lines a load, and reading the values took 85 us where the keys took 50.)
 constexpr int READ_TOKENS = 128;
 constexpr int read_row(int M) { return M + 4; }           // a token's codes in LDS, padded: the stores of one part go to different banks
-template <int D, int SUB>
+template <int D, int SUB, bool PAST>                      // PAST: the vectors are stored past the caches
 __global__ __launch_bounds__(512) void k_cache_read(const ReadArgs a) {
     constexpr int M = D / SUB, CH = D / 8, N = 8 / SUB, ROW = read_row(M);
     constexpr int WORDS = READ_TOKENS * M / 4, EACH_K = (WORDS + 511) / 512, EACH_V = M / 4;     // fetches a thread: words of keys' codes, values' bytes
@@ -168,7 +168,9 @@ __global__ __launch_bounds__(512) void k_cache_read(const ReadArgs a) {
                 else w = *reinterpret_cast<const uint32_t *>(q);
                 u32x4 v = expand<D, SUB>(s_book, w, a.K, c);
                 if (!s_there[t]) v = (u32x4){0, 0, 0, 0};
-                *reinterpret_cast<u32x4 *>(out + ((t0 + t) * a.heads + h) * (D * 2) + c * 16) = v;
+                u32x4 *to = reinterpret_cast<u32x4 *>(out + ((t0 + t) * a.heads + h) * (D * 2) + c * 16);
+                if constexpr (PAST) __builtin_nontemporal_store(v, to);
+                else *to = v;
             }
             __syncthreads();
         }
@@ -177,17 +179,25 @@ __global__ __launch_bounds__(512) void k_cache_read(const ReadArgs a) {
     else work(std::false_type{});
 }
 
-template <int D, int SUB> hipError_t launch_read(const ReadArgs &a, hipStream_t stream) {
-    // A codebook that a workgroup's tokens outweigh goes to LDS; for a few tokens the look-ups go to the caches instead.
+template <int D, int SUB, bool PAST> hipError_t launch_read_many(const ReadArgs &a, dim3 grid, hipStream_t stream) {
     const size_t lds = (size_t)a.K * D * 2 + READ_TOKENS * (read_row(D / SUB) + 1);
     static_assert(256 * D * 2 + READ_TOKENS * (read_row(D / SUB) + 1) <= LDS_MOST, "codebook and codes fit into LDS");
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t e = vq_internal_allow_lds(reinterpret_cast<const void *>(k_cache_read<D, SUB, PAST>), allowed);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_cache_read<D, SUB, PAST>), grid, dim3(512), lds, stream, a);
+    return hipGetLastError();
+}
+
+template <int D, int SUB> hipError_t launch_read(const ReadArgs &a, hipStream_t stream) {
+    // A codebook that a workgroup's tokens outweigh goes to LDS; for a few tokens the look-ups go to the caches instead.
     const dim3 grid(a.heads, (unsigned)((a.tokens + a.chunk - 1) / a.chunk), 2);
-    if (a.chunk >= a.K) {
-        static std::atomic<uint64_t> allowed{0};
-        const hipError_t e = vq_internal_allow_lds(reinterpret_cast<const void *>(k_cache_read<D, SUB>), allowed);
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((k_cache_read<D, SUB>), grid, dim3(512), lds, stream, a);
-    } else hipLaunchKernelGGL((k_cache_read_few<D, SUB>), grid, dim3(512), 0, stream, a);
+    // What the last cache (256 MB) can keep for whoever reads it next is left there; more is stored past it.  Read and then added up by another
+    // kernel, 128 MiB of vectors took 56 us with the caches and 59 past them, 160 MiB 86 and 79, 192 MiB 108 and 90, 512 MiB 314 and
+    // 303 (by itself the read of 256 MiB takes 80 and 54).
+    if (a.chunk >= a.K) return a.tokens * a.heads * D * 4 > (int64_t)144 << 20 ? launch_read_many<D, SUB, true>(a, grid, stream) :
+                                                                                 launch_read_many<D, SUB, false>(a, grid, stream);
+    hipLaunchKernelGGL((k_cache_read_few<D, SUB>), grid, dim3(512), 0, stream, a);
     return hipGetLastError();
 }
 
