@@ -190,12 +190,14 @@ template <int D, int SUB, bool PAST> hipError_t launch_read_many(const ReadArgs 
 }
 
 template <int D, int SUB> hipError_t launch_read(const ReadArgs &a, hipStream_t stream) {
-    // A codebook that a workgroup's tokens outweigh goes to LDS; for a few tokens the look-ups go to the caches instead.
+    // A codebook goes to LDS where a workgroup's look-ups are worth the staging; those of a few tokens, and few of 16 bytes, go to the caches.
+    // (8 heads, 256 codewords, from the caches and through LDS, us: 128 dims by 4: 4.2 and 4.1 at 64 tokens, 10.8 and 7.5 at 4096; 256
+    // dims by 2: 2.9 and 5.4 at one token, 9.4 and 6.4 at 64; 2 heads, 256 dims by 8: 4.7 and 5.0 at 64, 6.1 and 6.5 at 4096.)
     const dim3 grid(a.heads, (unsigned)((a.tokens + a.chunk - 1) / a.chunk), 2);
     // What the last cache (256 MB) can keep for whoever reads it next is left there; more is stored past it.  Read and then added up by another
     // kernel, 128 MiB of vectors took 56 us with the caches and 59 past them, 160 MiB 86 and 79, 192 MiB 108 and 90, 512 MiB 314 and
     // 303 (by itself the read of 256 MiB takes 80 and 54).
-    if (a.chunk >= a.K) return a.tokens * a.heads * D * 4 > (int64_t)144 << 20 ? launch_read_many<D, SUB, true>(a, grid, stream) :
+    if ((a.tokens < a.chunk ? a.tokens : a.chunk) * (16 / SUB) >= a.K) return a.tokens * a.heads * D * 4 > (int64_t)144 << 20 ? launch_read_many<D, SUB, true>(a, grid, stream) :
                                                                                  launch_read_many<D, SUB, false>(a, grid, stream);
     hipLaunchKernelGGL((k_cache_read_few<D, SUB>), grid, dim3(512), 0, stream, a);
     return hipGetLastError();
@@ -262,7 +264,7 @@ int64_t at_most(int64_t n, int64_t most) { return n < most ? n : most; }
 // How many rows a workgroup takes at a time and how many workgroups a head gets.  Host arithmetic on sizes alone.
 struct Attention {
     AttendPlan p;
-    int parts, join_at, join_rows;
+    int parts, join_at, join_rows, seq_at;
     size_t slots, ws;
 };
 Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q, int64_t max_kv) {
@@ -274,16 +276,17 @@ Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int se
     // so that a look-up serves twice the products, unless the value table then no longer fits but would beside 16.
     const size_t keys = key_bytes(Kp, dim, sub), values = (size_t)Kp * dim * 2, row = (size_t)(dim + 4) * 4;
     auto waves = [&](int rb) { return rb == 2 && dim >= 192 ? 4 : 8; };
-    auto fits = [&](int rb, size_t tables) { return tables + (size_t)waves(rb) * rb * 16 * 8 + 16 * row <= LDS_MOST; };
+    auto fits = [&](int rb, size_t tables) { return tables + (size_t)waves(rb) * rb * 16 * 8 + 16 * row + SEQ_BYTES <= LDS_MOST; };
     r.p.rb = per_seq <= 16 ? 1 : fits(2, keys + values) || !fits(1, keys + values) ? 2 : 1;
     r.p.nw = waves(r.p.rb);
     r.p.values_in_lds = fits(r.p.rb, keys + values);
     const int rows = r.p.rb * 16;
     const size_t ml = (size_t)r.p.nw * rows * 8, tables = keys + (r.p.values_in_lds ? values : 0);
-    const size_t room = (LDS_MOST - tables - ml) / row, most = (size_t)r.p.nw * rows;      // (room >= 16: it fits)
+    const size_t room = (LDS_MOST - SEQ_BYTES - tables - ml) / row, most = (size_t)r.p.nw * rows;      // (room >= 16: it fits)
     r.join_at = (int)tables;
     r.join_rows = (int)(room < most ? room : most);
-    r.p.lds = tables + ml + r.join_rows * row;
+    r.seq_at = (int)(tables + ml + r.join_rows * row);
+    r.p.lds = r.seq_at + SEQ_BYTES;
     // a head has at most so many items and tiles, by the caller's word
     const int64_t items = at_most(at_most((per_seq + rows - 1) / rows, 0x3fffffff) * seqs, 0x3fffffff);
     const int64_t tiles = items * ((at_most(max_kv, 0x7fffffff) + TILE - 1) / TILE);
@@ -428,7 +431,7 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
     float2 *part_ml = reinterpret_cast<float2 *>(part_o + r.slots * r.p.rb * 16 * dim);
     AttendArgs a = {q, q_token_stride, q_head_stride, rows, q_heads, {k_cb, v_cb}, cb_heads, heads, K, rows_padded(K), {k_codes, v_codes}, pages,
                     page, table, seqs, width, kv_lens, starts, (float)fmax(fabs(scale) * 1.4426950408889634, 1e-37), scale < 0 ? 0x80008000u : 0u,
-                    out, lse, r.parts, r.join_at, r.join_rows, part_o, part_ml,
+                    out, lse, r.parts, r.join_at, r.join_rows, r.seq_at, part_o, part_ml,
                     reinterpret_cast<AttendNote *>(part_ml + r.slots * r.p.rb * 16)};
     const dim3 grid(heads, r.parts);
     hipStream_t st = static_cast<hipStream_t>(stream);

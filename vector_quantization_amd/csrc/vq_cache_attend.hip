@@ -91,6 +91,13 @@ template <int NB> __device__ inline void load_bytes(uint32_t *w, global_bytes p)
 // the lane make of it without a base to be added each time.
 template <typename V> __device__ inline V lds(uint32_t at) { return *(const __attribute__((address_space(3))) V *)(uintptr_t)at; }
 
+// A barrier that waits for LDS alone: loads and stores of global memory stay under way.
+__device__ inline void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 __device__ inline float wave_any_max(float v) {          // the maximum over the four lanes of one row
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
@@ -152,6 +159,10 @@ __device__ inline int64_t part_begin(int64_t all, int parts, int part) {
 // ranges of tiles as there are workgroups: causal and ragged lengths are balanced by themselves, and a workgroup stages its tables once.
 // A range may begin and end inside an item.  Such an item's parts go to the workspace (`slots`, two a workgroup: the part that begins
 // an item and the part that does not), and the workgroup that holds its beginning notes it for k_cache_join.
+struct Range {
+    int64_t left, skip, now, all;      // tiles to be done, of them already done by others in the first item, where that begins; all of the head's
+    int seq, tile, held, parts;        // the first item; the first of the 64 sequences beside this
+};
 template <typename T, int D, int SUB, int RB, int NW, bool VLDS>
 __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
     constexpr int M = D / SUB, KS = D / 32, NB = M / 4, KW = (NB + 3) / 4;
@@ -209,72 +220,76 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
             if constexpr (VLDS) *reinterpret_cast<u32x4 *>(s_mem + i * 16) = stage_v[x];
         }
     };
-    stage_load(threadIdx.x);
-
-    // This workgroup's range.  Every wave works it out by itself: 64 sequences at a time, the tiles of rows of a long one 64 at a time too.
-    int seq_first = 0, seq_q = 0, seq_kv = 0, held = 0;           // a lane's sequence: the lanes hold those from `held` on
-    int64_t items = 0;
-    auto costs_from = [&](int b0) -> int64_t {                    // running cost of the 64 sequences from b0 on, which the lanes hold then
-        int64_t first = 0, sum = 0;
-        seq_q = seq_kv = 0;
-        if (b0 + lane < a.seqs) sequence(a, b0 + lane, first, seq_q, seq_kv);
-        seq_first = (int)first;
-        held = b0;
-        const int tiles = (seq_q * group + ROWS - 1) / ROWS;
-        items += of_last_lane(running(tiles));
-        if (tiles == 1) sum = cost_of<RB>(0, seq_q, seq_kv, group);
-        for (uint64_t todo = __ballot(tiles > 1); todo; todo &= todo - 1) {
-            const int of = __builtin_ctzll(todo), x_q = __shfl(seq_q, of), x_kv = __shfl(seq_kv, of), x_tiles = __shfl(tiles, of);
-            int64_t part = 0;
-            for (int t = lane; t < x_tiles; t += 64) part += cost_of<RB>(t, x_q, x_kv, group);
-            part = of_last_lane(running(part));
-            if (lane == of) sum = part;
-        }
-        return running(sum);
-    };
-    int64_t costs = costs_from(0), all = of_last_lane(costs);
-    for (int b0 = 64; b0 < a.seqs; b0 += 64) {
-        costs = costs_from(b0);
-        all += of_last_lane(costs);
-    }
-    // (a workgroup for every item at least, as far as they go: an item has costs of its own)
-    int64_t most_parts = all / LEAST_TILES > items ? all / LEAST_TILES : items;
-    const int parts = most_parts < 1 ? 1 : most_parts > (int64_t)gridDim.y ? (int)gridDim.y : (int)most_parts;
+    // This workgroup's range, worked out by one wave while the tables arrive, and left in LDS with the rows and lengths of 64 sequences.  (All
+    // eight working it out for themselves took 11 thousand cycles to the last one's start, one wave 7.)  The sequences' loads go
+    // before the tables': they come back in order.
+    int *s_seq = reinterpret_cast<int *>(s_mem + a.seq_at);
+    Range *s_range = reinterpret_cast<Range *>(s_seq + 64 * 3);
     const int me = h * gridDim.y + blockIdx.y;
-    const int64_t begin = uniform(part_begin(all, parts, blockIdx.y)), past = uniform(part_begin(all, parts, blockIdx.y + 1));
-    if ((int)blockIdx.y >= parts || begin >= past) {
-        if (a.parts > 1 && threadIdx.x == 0) a.notes[me] = AttendNote{-1, 0, 0, 0, 0, 0};
-        return;
+    int64_t seq_first = 0;
+    int seq_q = 0, seq_kv = 0;                                    // a lane's sequence
+    if (wave == 0 && lane < a.seqs) sequence(a, lane, seq_first, seq_q, seq_kv);
+    __builtin_amdgcn_sched_barrier(0);
+    stage_load(threadIdx.x);
+    __builtin_amdgcn_sched_barrier(0);
+    if (wave == 0) {
+        int64_t items = 0;
+        int held = 0;                                             // the lanes hold the sequences from here on: 64 at a time,
+        auto costs_from = [&](int b0) -> int64_t {                // and their running cost; the tiles of rows of a long one go 64 at a time too
+            int64_t sum = 0;
+            if (b0 != held) {
+                seq_first = 0, seq_q = seq_kv = 0;
+                if (b0 + lane < a.seqs) sequence(a, b0 + lane, seq_first, seq_q, seq_kv);
+                held = b0;
+            }
+            const int tiles = (seq_q * group + ROWS - 1) / ROWS;
+            items += of_last_lane(running(tiles));
+            if (tiles == 1) sum = cost_of<RB>(0, seq_q, seq_kv, group);
+            for (uint64_t todo = __ballot(tiles > 1); todo; todo &= todo - 1) {
+                const int of = __builtin_ctzll(todo), x_q = __shfl(seq_q, of), x_kv = __shfl(seq_kv, of), x_tiles = __shfl(tiles, of);
+                int64_t part = 0;
+                for (int t = lane; t < x_tiles; t += 64) part += cost_of<RB>(t, x_q, x_kv, group);
+                part = of_last_lane(running(part));
+                if (lane == of) sum = part;
+            }
+            return running(sum);
+        };
+        int64_t costs = costs_from(0), all = of_last_lane(costs);
+        for (int b0 = 64; b0 < a.seqs; b0 += 64) {
+            costs = costs_from(b0);
+            all += of_last_lane(costs);
+        }
+        // (a workgroup for every item at least, as far as they go: an item has costs of its own)
+        const int64_t most_parts = all / LEAST_TILES > items ? all / LEAST_TILES : items;
+        const int parts = most_parts < 1 ? 1 : most_parts > (int64_t)gridDim.y ? (int)gridDim.y : (int)most_parts;
+        const int64_t begin = uniform(part_begin(all, parts, blockIdx.y)), past = uniform(part_begin(all, parts, blockIdx.y + 1));
+        const int64_t left = (int)blockIdx.y < parts && begin < past ? past - begin : 0;
+        int64_t skip = begin;                                     // first: of the work before sequence b; then of item (b, tile)
+        int b = 0, tile = 0, at;
+        auto locate = [&](int64_t sum) -> bool {                  // sum: the lanes' running costs; finds the lane that skip falls to
+            const bool here = skip < of_last_lane(sum);
+            at = here ? __builtin_ctzll(__ballot(sum > skip)) : 64;
+            skip -= at > 0 ? uniform(__shfl(sum, at - 1)) : 0;
+            return here;
+        };
+        for (int b0 = 0; left > 0 && b0 < a.seqs; b0 += 64) {
+            if (b0 != held) costs = costs_from(b0);
+            const bool here = locate(costs);
+            b = b0 + at;
+            if (here) break;
+        }
+        int n_q = 0, n_kv = 0;
+        if (left > 0 && b < a.seqs) n_q = __builtin_amdgcn_readlane(seq_q, b - held), n_kv = __builtin_amdgcn_readlane(seq_kv, b - held);
+        const int tiles = (n_q * group + ROWS - 1) / ROWS;
+        for (int t0 = 0; tiles > 1 && t0 < tiles; t0 += 64) {
+            const int t = t0 + lane;
+            const bool here = locate(running(t < tiles ? cost_of<RB>(t, n_q, n_kv, group) : 0));
+            tile = t0 + at;
+            if (here) break;
+        }
+        s_seq[3 * lane] = (int)seq_first, s_seq[3 * lane + 1] = seq_q, s_seq[3 * lane + 2] = seq_kv;
+        if (lane == 0) *s_range = Range{left, skip, begin - skip, all, b, tile, held, parts};
     }
-    int64_t skip = begin;                                         // first: of the work before sequence b; then of item (b, tile)
-    auto locate = [&](int64_t sum, int &at) -> bool {             // sum: the lanes' running costs; finds the lane that skip falls to
-        const bool here = skip < of_last_lane(sum);
-        at = here ? __builtin_ctzll(__ballot(sum > skip)) : 64;
-        skip -= at > 0 ? uniform(__shfl(sum, at - 1)) : 0;
-        return here;
-    };
-    int b = 0, tile = 0, at;
-    for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-        if (b0 != held) costs = costs_from(b0);
-        const bool here = locate(costs, at);
-        b = b0 + at;
-        if (here) break;
-    }
-    int first = 0, n_q = 0, n_kv = 0;                             // sequence b, out of the lane that holds it
-    if (b < a.seqs) {
-        first = __builtin_amdgcn_readlane(seq_first, b - held);
-        n_q = __builtin_amdgcn_readlane(seq_q, b - held);
-        n_kv = __builtin_amdgcn_readlane(seq_kv, b - held);
-    }
-    const int first_tiles = (n_q * group + ROWS - 1) / ROWS;
-    for (int t0 = 0; first_tiles > 1 && t0 < first_tiles; t0 += 64) {
-        const int t = t0 + lane;
-        const bool here = locate(running(t < first_tiles ? cost_of<RB>(t, n_q, n_kv, group) : 0), at);
-        tile = t0 + at;
-        if (here) break;
-    }
-    int64_t left = past - begin, now = begin - skip;              // now: where item (b, tile) begins
-
     stage_store(threadIdx.x);
     for (int i0 = threadIdx.x + BATCH * NW * 64; i0 < Kp * (D / 8); i0 += BATCH * NW * 64) {
         stage_load(i0);
@@ -282,31 +297,75 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
     }
     __syncthreads();
 
-    AttendNote note = {-1, 0, 0, 0, 0, 0};
-    while (left > 0 && b < a.seqs) {
-        const int n_rows = n_q * group;
-        if (tile * ROWS >= n_rows) {
-            tile = 0;
-            if (++b < a.seqs) {
-                int64_t x;
-                sequence(a, b, x, n_q, n_kv);
-                first = (int)x;
-            }
-            continue;
+    int64_t left = uniform(s_range->left), skip = uniform(s_range->skip), now = uniform(s_range->now);      // now: where item (b, tile) begins
+    int b = __builtin_amdgcn_readfirstlane(s_range->seq), tile = __builtin_amdgcn_readfirstlane(s_range->tile);
+    const int held = __builtin_amdgcn_readfirstlane(s_range->held);
+    int first = 0, n_q = 0, n_kv = 0;
+    auto take_sequence = [&]() {
+        if (b - held < 64) {
+            first = __builtin_amdgcn_readfirstlane(s_seq[3 * (b - held)]);
+            n_q = __builtin_amdgcn_readfirstlane(s_seq[3 * (b - held) + 1]);
+            n_kv = __builtin_amdgcn_readfirstlane(s_seq[3 * (b - held) + 2]);
+        } else {
+            int64_t x;
+            int y, z;
+            sequence(a, b, x, y, z);
+            first = (int)x, n_q = y, n_kv = z;
         }
-        const int tiles = tiles_of<RB>(tile, n_q, n_kv, group), cost = tiles < 1 ? 1 : tiles;
-        const int take = (int)(left < cost - skip ? left : cost - skip);
-        const int lo = (int)skip < tiles ? (int)skip : tiles, hi = (int)skip + take < tiles ? (int)skip + take : tiles;
-        const bool whole_item = take == cost;
-        const int32_t *table = a.table + (int64_t)b * a.width;
-        const int row0 = tile * ROWS, rows_here = n_rows - row0 < ROWS ? n_rows - row0 : ROWS;
-        const int back = n_kv - n_q;                              // row i sees tokens 0 .. back + i
-        const int all_see = back + row0 / group;                  // every row of the item sees tokens up to here
+    };
+    AttendNote note = {-1, 0, 0, 0, 0, 0};
 
-        u32x4 q[RB][KS];
-        int sees[RB];
-        f32x4 o[RB][U][E];
-        float top[RB], total[RB];
+    // The item in hand, from its first loads on.
+    int take = 0, cost = 1, row0 = 0, rows_here = 0, lo = 0, hi = 0, all_see = 0;
+    const int32_t *table = a.table;
+    u32x4 q[RB][KS];
+    int sees[RB];
+    // A wave's tiles: lo + wave, then every NW-th.  Where their codes lie is worked out for 32 tiles at a time, a lane for each half of a
+    // tile (16 tokens, inside one page); a turn then takes its four addresses out of the lanes.  (Page numbers fetched and
+    // multiplied out turn by turn took longer than all the rest: a wave waits for every scalar step.)
+    // Codes are fetched AHEAD tiles before their use.
+    constexpr int AHEAD = 2;
+    int t = lo + wave, fetched = 0;                           // the tile in hand; how many have been fetched
+    uint64_t k_ptr = 0, v_ptr = 0, there = 0;                 // a lane's addresses; one bit a lane: its tokens lie in a page of the cache
+    auto place = [&]() {
+        const int tile32 = lo + wave + (fetched + (lane & 31)) * NW, group16 = 2 * tile32 + (lane >> 5);
+        const int at = group16 / page16, y = group16 - at * page16;
+        const bool in = tile32 < hi && group16 * 16 < n_kv;
+        const int n = in ? table[at] : -1;
+        const bool good = n >= 0 && n < a.pages;
+        const int64_t from = good ? (int64_t)n * page_bytes + head_at : head_at;      // (else page 0: read, not looked at)
+        k_ptr = (uint64_t)(a.codes[0] + (from + (int64_t)(good ? y : 0) * 16 * M));
+        v_ptr = (uint64_t)(a.codes[1] + (from + (good ? y : 0) * 16));
+        there = __ballot(good);
+    };
+    auto of_lane = [](uint64_t v, int from) -> global_bytes {
+        return (global_bytes)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, from) |
+                              (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), from) << 32);
+    };
+    uint32_t kc[AHEAD][2][KW], vc[AHEAD][2][U], seen[AHEAD];   // seen: bits 0 and 1: the tile's halves are there
+    auto fetch = [&](int slot) {
+        const int at = fetched & 31;
+        if (at == 0) place();
+        seen[slot] = (uint32_t)(there >> at) & 1u | ((uint32_t)(there >> (32 + at)) & 1u) << 1;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            load_bytes<NB>(kc[slot][s], of_lane(k_ptr, 32 * s + at) + k_lane);
+            const global_bytes from = of_lane(v_ptr, 32 * s + at);
+#pragma unroll
+            for (int u = 0; u < U; ++u) vc[slot][s][u] = *(const GLOBAL uint32_t *)(from + v_lane[u]);
+        }
+        ++fetched;
+    };
+    static_assert(AHEAD == 2, "turns go by twos");
+    // Sends off the loads of item (b, tile): queries, page numbers, the codes of a wave's first tiles.
+    auto open = [&]() {
+        const int tiles = tiles_of<RB>(tile, n_q, n_kv, group), n_rows = n_q * group, back = n_kv - n_q;     // row i sees tokens 0 .. back + i
+        cost = tiles < 1 ? 1 : tiles;
+        take = (int)(left < cost - skip ? left : cost - skip);
+        lo = (int)skip < tiles ? (int)skip : tiles, hi = (int)skip + take < tiles ? (int)skip + take : tiles;
+        table = a.table + (int64_t)b * a.width;
+        row0 = tile * ROWS, rows_here = n_rows - row0 < ROWS ? n_rows - row0 : ROWS;
+        all_see = back + row0 / group;                            // every row of the item sees tokens up to here
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             const int row = rb * 16 + r < rows_here ? row0 + rb * 16 + r : row0;
@@ -314,55 +373,45 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
             const T *p = static_cast<const T *>(a.q) + (int64_t)(first + i) * a.q_token_stride + head * a.q_head_stride + g * (D / 4);
             sees[rb] = back + i;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) q[rb][s] = *reinterpret_cast<const u32x4 *>(p + 8 * s) ^ a.flip;
+            for (int s = 0; s < KS; ++s) q[rb][s] = *reinterpret_cast<const u32x4 *>(p + 8 * s);
+        }
+        t = lo + wave, fetched = 0;
+        if (t < hi) {
+            fetch(0);
+            fetch(1);
+        }
+    };
+    // On to the next item; false where there is none.
+    auto advance = [&]() -> bool {
+        left -= take;
+        now += cost;
+        skip = 0;
+        ++tile;
+        while (left > 0 && tile * ROWS >= n_q * group) {
+            tile = 0;
+            if (++b >= a.seqs) return false;
+            take_sequence();
+        }
+        return left > 0;
+    };
+    bool more = left > 0 && b < a.seqs;
+    if (more) {
+        take_sequence();
+        open();
+    }
+    while (more) {
+        f32x4 o[RB][U][E];
+        float top[RB], total[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
             top[rb] = -INFINITY;
             total[rb] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) q[rb][s] ^= a.flip;
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[rb][u][e] = (f32x4){0, 0, 0, 0};
-        }
-
-        // A wave's tiles: lo + wave, then every NW-th.  Where their codes lie is worked out for 32 tiles at a time, a lane for each half of a
-        // tile (16 tokens, inside one page); a turn then takes its four addresses out of the lanes.  (Page numbers fetched and
-        // multiplied out turn by turn took longer than all the rest: a wave waits for every scalar step.)
-        // Codes are fetched AHEAD tiles before their use.
-        constexpr int AHEAD = 2;
-        int t = lo + wave, fetched = 0;                           // the tile in hand; how many have been fetched
-        uint64_t k_ptr = 0, v_ptr = 0, there = 0;                 // a lane's addresses; one bit a lane: its tokens lie in a page of the cache
-        auto place = [&]() {
-            const int tile32 = lo + wave + (fetched + (lane & 31)) * NW, group16 = 2 * tile32 + (lane >> 5);
-            const int at = group16 / page16, y = group16 - at * page16;
-            const bool in = tile32 < hi && group16 * 16 < n_kv;
-            const int n = in ? table[at] : -1;
-            const bool good = n >= 0 && n < a.pages;
-            const int64_t from = good ? (int64_t)n * page_bytes + head_at : head_at;      // (else page 0: read, not looked at)
-            k_ptr = (uint64_t)(a.codes[0] + (from + (int64_t)(good ? y : 0) * 16 * M));
-            v_ptr = (uint64_t)(a.codes[1] + (from + (good ? y : 0) * 16));
-            there = __ballot(good);
-        };
-        auto of_lane = [](uint64_t v, int from) -> global_bytes {
-            return (global_bytes)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, from) |
-                                  (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), from) << 32);
-        };
-        uint32_t kc[AHEAD][2][KW], vc[AHEAD][2][U], seen[AHEAD];   // seen: bits 0 and 1: the tile's halves are there
-        auto fetch = [&](int slot) {
-            const int at = fetched & 31;
-            if (at == 0) place();
-            seen[slot] = (uint32_t)(there >> at) & 1u | ((uint32_t)(there >> (32 + at)) & 1u) << 1;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                load_bytes<NB>(kc[slot][s], of_lane(k_ptr, 32 * s + at) + k_lane);
-                const global_bytes from = of_lane(v_ptr, 32 * s + at);
-#pragma unroll
-                for (int u = 0; u < U; ++u) vc[slot][s][u] = *(const GLOBAL uint32_t *)(from + v_lane[u]);
-            }
-            ++fetched;
-        };
-        static_assert(AHEAD == 2, "turns go by twos");
-        if (t < hi) {
-            fetch(0);
-            fetch(1);
         }
         // Look-ups.  Up to 128 dims all of a tile's go first, so that they pass through LDS one behind the other; beyond, registers are
         // short and they go one step before their use.  Either way the tile's codes are done with before the next ones are fetched to
@@ -504,11 +553,26 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
             t += NW;
         };
         __builtin_amdgcn_s_waitcnt(0x0f70);                       // all loads: inside the loop no wait is left but those of the codes
+        // The two waves of a SIMD take turns in going first: left to itself the older one does, and the younger's last tiles are done with nobody
+        // to fill its waits (80 and 92 thousand cycles for 39 tiles each).
+        bool ahead = wave < NW / 2;
         while (t + NW < hi) {                                     // (left in one place only: leaving after the first turn as well would make
-            turn(0);                                              // every wait for its codes one for all loads)
+            if (ahead) __builtin_amdgcn_s_setprio(1);             // every wait for its codes one for all loads)
+            else __builtin_amdgcn_s_setprio(0);
+            ahead = !ahead;
+            turn(0);
             turn(1);
         }
+        __builtin_amdgcn_s_setprio(0);
         if (t < hi) turn(0);
+
+        // The next item's loads leave before this one's rows are joined, where there are registers for both.
+        constexpr bool EARLY = RB * D <= 192;
+        const bool whole_item = take == cost;
+        const int slot = 2 * me + (skip == 0 ? 1 : 0), its_first = first, its_row0 = row0, its_rows = rows_here;
+        if (!whole_item && skip == 0) note = AttendNote{b, tile, s_range->parts, 0, now + cost - 1, s_range->all};
+        more = advance();
+        if (EARLY && more) open();
 
         // Join the waves: maxima and sums first, then every wave's part weighted by its maximum, added in the waves' order, as many
         // waves at a time as LDS has room for beside the tables.
@@ -523,12 +587,11 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) s_ml[wave * ROWS + rb * 16 + r] = make_float2(top[rb], total[rb]);
         constexpr int EACH = (16 * (D / 8) + NW * 64 - 1) / (NW * 64);         // pieces of 8 numbers a thread adds up
-        const int slot = 2 * me + (skip == 0 ? 1 : 0);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            const int rows_rb = rows_here - rb * 16 < 16 ? rows_here - rb * 16 : 16;
+            const int rows_rb = its_rows - rb * 16 < 16 ? its_rows - rb * 16 : 16;
             if (rows_rb <= 0) break;
-            if (rb > 0) __syncthreads();                          // the sums of the rows before go to the same place
+            if (rb > 0) lds_barrier();                          // the sums of the rows before go to the same place
             const int at_once = a.join_rows / rows_rb;
             f32x4 v0[EACH], v1[EACH];
             float weight[EACH][NW], most[EACH], sum[EACH];
@@ -545,7 +608,7 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
                             p[u * 4 * E + j] = v;
                         }
                 }
-                __syncthreads();
+                lds_barrier();
 #pragma unroll
                 for (int n = 0; n < EACH; ++n) {
                     const int i = threadIdx.x + n * NW * 64, x = i / (D / 8), c = i % (D / 8);
@@ -572,15 +635,15 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
                         v1[n] += *reinterpret_cast<const f32x4 *>(p + 4) * weight[n][y];
                     }
                 }
-                if (w0 + at_once < NW) __syncthreads();
+                if (w0 + at_once < NW) lds_barrier();
             }
 #pragma unroll
             for (int n = 0; n < EACH; ++n) {
                 const int i = threadIdx.x + n * NW * 64, x = i / (D / 8), c = i % (D / 8);
                 if (x >= rows_rb) continue;
                 if (whole_item) {
-                    const int row = row0 + rb * 16 + x;
-                    store_row<T>(a, (int64_t)(first + row / group) * a.q_heads + h * group + row % group, D, c, v0[n], v1[n], most[n], sum[n]);
+                    const int row = its_row0 + rb * 16 + x;
+                    store_row<T>(a, (int64_t)(its_first + row / group) * a.q_heads + h * group + row % group, D, c, v0[n], v1[n], most[n], sum[n]);
                 } else {
                     const int64_t at = (int64_t)slot * ROWS + rb * 16 + x;
                     float *p = a.part_o + at * D + c * 8;
@@ -590,13 +653,8 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
                 }
             }
         }
-        if (!whole_item && skip == 0) note = AttendNote{b, tile, parts, 0, now + cost - 1, all};
-        __syncthreads();                                          // the next item's sums go to the same place
-
-        left -= take;
-        now += cost;
-        skip = 0;
-        ++tile;
+        lds_barrier();                                            // the next item's sums go to the same place
+        if (!EARLY && more) open();
     }
     if (a.parts > 1 && threadIdx.x == 0) a.notes[me] = note;
 }

@@ -44,6 +44,7 @@ struct AttendArgs {
     float *lse;
     int parts;                         // workgroups a head at most
     int join_at, join_rows;            // LDS behind the tables: its place, and how many rows' sums fit there
+    int seq_at;                        // behind them SEQ_BYTES for a workgroup's range and 64 sequences' rows and lengths
     float *part_o;                     // (slots, rows of an item, D), against part_ml's maximum; two slots a workgroup
     float2 *part_ml;                   // (slots, rows of an item): maximum (base 2) and sum
     struct AttendNote *notes;          // one a workgroup
@@ -102,6 +103,7 @@ VQ_HIDDEN hipError_t vq_internal_attend_f16(const AttendArgs &a, const AttendPla
 constexpr int LDS_MOST = 160 * 1024;
 // The least that a workgroup is given: under two tiles a wave, staging and joining outweigh what is shared out.
 constexpr int LEAST_TILES = 16;
+constexpr int SEQ_BYTES = 64 * 12 + 48;
 constexpr int TILE = 32;              // tokens a wave takes at a time: two groups of 16, each inside one page
 
 constexpr int value_chunk(int D, int SUB) {
