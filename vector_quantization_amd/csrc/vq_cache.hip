@@ -290,7 +290,7 @@ Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int se
     // a head has at most so many items and tiles, by the caller's word
     const int64_t items = at_most(at_most((per_seq + rows - 1) / rows, 0x3fffffff) * seqs, 0x3fffffff);
     const int64_t tiles = items * ((at_most(max_kv, 0x7fffffff) + TILE - 1) / TILE);
-    const int64_t wanted = tiles / LEAST_TILES > items ? tiles / LEAST_TILES : items;
+    const int64_t wanted = parts_wanted(tiles, items);
     int64_t parts = (CUS + heads - 1) / heads;
     if (parts * heads > CUS && parts > 1) --parts;
     parts = parts < wanted ? parts : wanted;

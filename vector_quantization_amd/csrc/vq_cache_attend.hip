@@ -259,9 +259,8 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
             costs = costs_from(b0);
             all += of_last_lane(costs);
         }
-        // (a workgroup for every item at least, as far as they go: an item has costs of its own)
-        const int64_t most_parts = all / LEAST_TILES > items ? all / LEAST_TILES : items;
-        const int parts = most_parts < 1 ? 1 : most_parts > (int64_t)gridDim.y ? (int)gridDim.y : (int)most_parts;
+        const int64_t most_parts = parts_wanted(all, items);
+        const int parts = most_parts > (int64_t)gridDim.y ? (int)gridDim.y : (int)most_parts;
         const int64_t begin = uniform(part_begin(all, parts, blockIdx.y)), past = uniform(part_begin(all, parts, blockIdx.y + 1));
         const int64_t left = (int)blockIdx.y < parts && begin < past ? past - begin : 0;
         int64_t skip = begin;                                     // first: of the work before sequence b; then of item (b, tile)
