@@ -234,6 +234,22 @@ def test_large_vectors_keep_to_the_codewords_there_are(eng, K, dtype):
     assert dist.isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [1, 40, 100])
+def test_products_beyond_fp32(eng, K, dtype):
+    """Vectors and codewords of 1e20, whose products fp32 does not hold."""
+    T, H, D, sub = 70, 2, 32, 8
+    x, cb = data(7, (T, H, D), torch.float32).mul(1e20).to(dtype), data(8, (H, K, D), torch.float32) * 1e20
+    if dtype != torch.float32:
+        half = cb.to(dtype)
+        kc, vc = eng.cache_buffers(5, 16, H, D, sub)
+        eng.cache_write(x.to(DEV), x.to(DEV), torch.arange(T, device=DEV), half.to(DEV), half.to(DEV), kc, vc)
+        assert torch.equal(kc.cpu().transpose(1, 2).reshape(80, H, D // sub)[:T].long(), torch.from_numpy(codes64(x, half, sub)[0]))
+    sums, counts, dist = eng.cache_lbg_accum(x.to(DEV), cb.to(DEV), sub)
+    new, mean = eng.cache_lbg_finish(sums, counts, dist, cb.to(DEV))
+    check_training(x, cb, sub, sums, counts, dist, new, mean)
+
+
 def test_write_strides_and_shared_codebook(eng):
     """Keys and values inside one larger tensor, copies where their vectors do not start at multiples of 16 bytes, one codebook for all heads."""
     T, H, D, sub, K, page = 77, 4, 64, 4, 256, 16

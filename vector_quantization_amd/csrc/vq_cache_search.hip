@@ -257,7 +257,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
         const float best = upper ? h1 : l1, second = least(upper ? l1 : h1, least(l2, h2));
         const float bound = 0.5f * reach + __builtin_amdgcn_sqrtf(size) * far;
         bool open = !(second - best > bound * GAP + 1e-36f) || !(bound < BOUND_MOST) || !(size < SIZE_MOST);
-        const int group = __builtin_bit_cast(uint32_t, best) & 15;
+        const int group = __builtin_bit_cast(uint32_t, best) & (2 * NT - 1);      // (a score beyond fp32 names any)
 
         // step 2: rows k0 to k0 + 3 and k0 + 8 to k0 + 11
         const int k0 = group * 16 + 4 * (int)upper, at0 = row_at<SUB>(group * 16) + (upper ? 4 * SUB : 0);
