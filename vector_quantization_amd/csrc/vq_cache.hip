@@ -266,6 +266,7 @@ int64_t at_most(int64_t n, int64_t most) { return n < most ? n : most; }
 struct Attention {
     AttendPlan p;
     int parts, join_at, join_rows, seq_at;
+    bool split;
     size_t slots, ws;
 };
 Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int seqs, int64_t max_q, int64_t max_kv) {
@@ -296,9 +297,11 @@ Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int se
     const int64_t wanted = parts_wanted(tiles, items);
     int64_t parts = (CUS + heads - 1) / heads;
     if (parts * heads > CUS && parts > 1) --parts;
-    parts = parts < wanted ? parts : wanted;
+    const bool whole = items <= parts && tiles <= items * WHOLE_TILES;
+    parts = whole ? items : parts < wanted ? parts : wanted;
     r.parts = (int)(parts < 1 ? 1 : parts);
-    r.slots = r.parts > 1 ? (size_t)2 * heads * r.parts : 0;
+    r.split = !whole && r.parts > 1;
+    r.slots = r.split ? (size_t)2 * heads * r.parts : 0;
     r.ws = r.slots * (rows * ((size_t)dim * 4 + 8)) + r.slots / 2 * sizeof(AttendNote);
     return r;
 }
@@ -434,7 +437,7 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
     float2 *part_ml = reinterpret_cast<float2 *>(part_o + r.slots * r.p.rb * 16 * dim);
     AttendArgs a = {q, q_token_stride, q_head_stride, rows, q_heads, {k_cb, v_cb}, cb_heads, heads, K, rows_padded(K), {k_codes, v_codes}, pages,
                     page, table, seqs, width, kv_lens, starts, (float)fmax(fabs(scale) * 1.4426950408889634, 1e-37), scale < 0 ? 0x80008000u : 0u,
-                    out, lse, r.parts, r.join_at, r.join_rows, r.seq_at, part_o, part_ml,
+                    out, lse, r.split, r.join_at, r.join_rows, r.seq_at, part_o, part_ml,
                     reinterpret_cast<AttendNote *>(part_ml + r.slots * r.p.rb * 16)};
     const dim3 grid(heads, r.parts);
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -166,7 +166,8 @@ __device__ inline int64_t part_begin(int64_t all, int parts, int part) {
 // One head's work is all its items side by side, (sequence, tile of rows) after (sequence, tile of rows), cut into as many equal
 // ranges of tiles as there are workgroups: causal and ragged lengths are balanced by themselves, and a workgroup stages its tables once.
 // A range may begin and end inside an item.  Such an item's parts go to the workspace (`slots`, two a workgroup: the part that begins
-// an item and the part that does not), and the workgroup that holds its beginning notes it for k_cache_join.
+// an item and the part that does not), and the workgroup that holds its beginning notes it for k_cache_join.  Without `split` an item
+// counts as one, whatever its length, and is never cut.
 struct Range {
     int64_t left, skip, now, all;      // tiles to be done, of them already done by others in the first item, where that begins; all of the head's
     int seq, tile, held, parts;        // the first item; the first of the 64 sequences beside this
@@ -252,8 +253,9 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
             }
             const int tiles = (seq_q * group + ROWS - 1) / ROWS;
             items += of_last_lane(running(tiles));
-            if (tiles == 1) sum = cost_of<RB>(0, seq_q, seq_kv, group);
-            for (uint64_t todo = __ballot(tiles > 1); todo; todo &= todo - 1) {
+            if (!a.split) sum = tiles;
+            else if (tiles == 1) sum = cost_of<RB>(0, seq_q, seq_kv, group);
+            for (uint64_t todo = a.split ? __ballot(tiles > 1) : 0; todo; todo &= todo - 1) {
                 const int of = __builtin_ctzll(todo), x_q = __shfl(seq_q, of), x_kv = __shfl(seq_kv, of), x_tiles = __shfl(tiles, of);
                 int64_t part = 0;
                 for (int t = lane; t < x_tiles; t += 64) part += cost_of<RB>(t, x_q, x_kv, group);
@@ -267,7 +269,7 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
             costs = costs_from(b0);
             all += of_last_lane(costs);
         }
-        const int64_t most_parts = parts_wanted(all, items);
+        const int64_t most_parts = a.split ? parts_wanted(all, items) : items < 1 ? 1 : items;
         const int parts = most_parts > (int64_t)gridDim.y ? (int)gridDim.y : (int)most_parts;
         const int64_t begin = uniform(part_begin(all, parts, blockIdx.y)), past = uniform(part_begin(all, parts, blockIdx.y + 1));
         const int64_t left = (int)blockIdx.y < parts && begin < past ? past - begin : 0;
@@ -290,7 +292,7 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
         const int tiles = (n_q * group + ROWS - 1) / ROWS;
         for (int t0 = 0; tiles > 1 && t0 < tiles; t0 += 64) {
             const int t = t0 + lane;
-            const bool here = locate(running(t < tiles ? cost_of<RB>(t, n_q, n_kv, group) : 0));
+            const bool here = locate(running(t >= tiles ? 0 : a.split ? cost_of<RB>(t, n_q, n_kv, group) : 1));
             tile = t0 + at;
             if (here) break;
         }
@@ -367,9 +369,9 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
     // Sends off the loads of item (b, tile): queries, page numbers, the codes of a wave's first tiles.
     auto open = [&]() {
         const int tiles = tiles_of<RB>(tile, n_q, n_kv, group), n_rows = n_q * group, back = n_kv - n_q;     // row i sees tokens 0 .. back + i
-        cost = tiles < 1 ? 1 : tiles;
+        cost = !a.split || tiles < 1 ? 1 : tiles;
         take = (int)(left < cost - skip ? left : cost - skip);
-        lo = (int)skip < tiles ? (int)skip : tiles, hi = (int)skip + take < tiles ? (int)skip + take : tiles;
+        lo = (int)skip < tiles ? (int)skip : tiles, hi = a.split && (int)skip + take < tiles ? (int)skip + take : tiles;
         table = a.table + (int64_t)b * a.width;
         row0 = tile * ROWS, rows_here = n_rows - row0 < ROWS ? n_rows - row0 : ROWS;
         all_see = back + row0 / group;                            // every row of the item sees tokens up to here
@@ -663,7 +665,7 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
         lds_barrier();                                            // the next item's sums go to the same place
         if (!EARLY && more) open();
     }
-    if (a.parts > 1 && threadIdx.x == 0) a.notes[me] = note;
+    if (a.split && threadIdx.x == 0) a.notes[me] = note;
 }
 
 // Joins an item's parts: the one of the workgroup that noted it, then the others in order.  4 to 6 us, nearly all of it the launch and two
@@ -711,7 +713,7 @@ hipError_t launch(const AttendArgs &a, const AttendPlan &p, dim3 grid, hipStream
     const hipError_t e = vq_internal_allow_lds(reinterpret_cast<const void *>(kernel), allowed);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, grid, dim3(NW * 64), p.lds, stream, a);
-    if (a.parts > 1) hipLaunchKernelGGL((k_cache_join<T, D, RB>), grid, dim3(256), 0, stream, a);
+    if (a.split) hipLaunchKernelGGL((k_cache_join<T, D, RB>), grid, dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -42,7 +42,7 @@ struct AttendArgs {
     uint32_t flip;                     // the sign bits of two 16-bit numbers where scale < 0: q is negated instead
     void *out;
     float *lse;
-    int parts;                         // workgroups a head at most
+    bool split;                        // items may be cut between workgroups
     int join_at, join_rows;            // LDS behind the tables: its place, and how many rows' sums fit there
     int seq_at;                        // behind them SEQ_BYTES for a workgroup's range and 64 sequences' rows and lengths
     float *part_o;                     // (slots, rows of an item, D), against part_ml's maximum; two slots a workgroup
@@ -104,6 +104,10 @@ constexpr int LDS_MOST = 160 * 1024;
 // The least that a workgroup is given: under two tiles a wave, staging and joining outweigh what is shared out (one row of 500 tokens: 10.8 us
 // by 16 tiles, 12.8 by 8; of 2000: 14.7 by 16, 13.8 by 8, 16.4 by 32).
 constexpr int LEAST_TILES = 16;
+// Items that are no longer than this, and for each of which there is a workgroup, are not cut: nothing has to be joined then, and the call is one
+// launch.  (One row of 1000 tokens, 32 tiles: 12.5 us whole, 13.5 cut in two, 12.7 in four; of 2000: 16.4 whole, 14.7 in three.  From
+// Python a second launch and a workspace take another 4.)
+constexpr int WHOLE_TILES = 3 * LEAST_TILES;
 // The workgroups a head's work asks for: one for every item at least, since to change items costs as much as several tiles, and a
 // multiple of the items, so that those of equal length are cut alike and nobody has to change (4 sequences of 5 rows and 4000 tokens:
 // 30 us by 31 workgroups a head, 21 by 32).
