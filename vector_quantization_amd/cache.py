@@ -73,10 +73,19 @@ _F64 = (torch.float64,)
 
 def cache_shape(k_cb, v_cb, k_codes, v_codes, device):
     """Checks codebooks and code buffers against each other; returns (heads, dim, sub, K, pages, page)."""
-    _tensor("k_cb", k_cb, device, _HALVES, 3)
-    _tensor("v_cb", v_cb, device, (k_cb.dtype,), 3)
-    _whole("k_codes", _tensor("k_codes", k_codes, device, _BYTES, 4))
-    _whole("v_codes", _tensor("v_codes", v_codes, device, _BYTES, 4))
+    try:
+        dtype = k_cb.dtype
+        right = (dtype in _HALVES and v_cb.dtype is dtype and k_codes.dtype is torch.uint8 and v_codes.dtype is torch.uint8 and
+                 k_cb.device == device and v_cb.device == device and k_codes.device == device and v_codes.device == device and
+                 k_cb.dim() == 3 and k_codes.dim() == 4 and not (k_cb.requires_grad or v_cb.requires_grad) and
+                 k_codes.is_contiguous() and v_codes.is_contiguous() and not (k_codes.data_ptr() | v_codes.data_ptr()) % 16)
+    except AttributeError:
+        right = False
+    if not right:
+        _tensor("k_cb", k_cb, device, _HALVES, 3)
+        _tensor("v_cb", v_cb, device, (k_cb.dtype,), 3)
+        _whole("k_codes", _tensor("k_codes", k_codes, device, _BYTES, 4))
+        _whole("v_codes", _tensor("v_codes", v_codes, device, _BYTES, 4))
     pages, heads, page, parts = k_codes.shape
     books, K, dim = k_cb.shape
     if not (pages and heads and page and parts):
@@ -91,7 +100,8 @@ def cache_shape(k_cb, v_cb, k_codes, v_codes, device):
 
 
 def _ints(name, t, dtypes, dims, device):
-    _tensor(name, t, device, dtypes, dims)
+    if not (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dims and t.device == device):
+        _tensor(name, t, device, dtypes, dims)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -147,8 +157,8 @@ class CacheOps:
         slots = _ints("slots", slots, _INT64, 1, device)
         tokens = slots.shape[0]
         k_cb, v_cb = _books(k_cb), _books(v_cb)
-        k = torch.empty((tokens, heads, dim), dtype=k_cb.dtype, device=device)
-        v = torch.empty((tokens, heads, dim), dtype=k_cb.dtype, device=device)
+        k = torch.empty(tokens, heads, dim, dtype=k_cb.dtype, device=device)       # (sizes one by one: the shorter way through torch)
+        v = torch.empty_like(k)
         if tokens:
             self._launch("vq_cache_read", slots.data_ptr(), tokens, k_cb.data_ptr(), v_cb.data_ptr(), k_cb.shape[0], heads, dim, sub, K,
                          _DTYPES[k_cb.dtype], k_codes.data_ptr(), v_codes.data_ptr(), pages, page, k.data_ptr(), v.data_ptr())
@@ -181,10 +191,10 @@ class CacheOps:
         width = table.shape[1]
         _sized("table", table, (seqs, width))
         if out is None:
-            out = torch.empty((rows, q_heads, dim), dtype=dtype, device=device)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(rows, q_heads, dim, dtype=dtype, device=device)
         else:
             _sized("out", _whole("out", _tensor("out", out, device, (dtype,), 3)), (rows, q_heads, dim))
-        lse = torch.empty((rows, q_heads), dtype=torch.float32, device=device) if want_lse else None
+        lse = torch.empty(rows, q_heads, dtype=torch.float32, device=device) if want_lse else None
         if rows and seqs:
             q, k_cb, v_cb = _vectors(q), _books(k_cb), _books(v_cb)
             scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
@@ -258,9 +268,9 @@ class CacheOps:
             new, mean = self.cache_lbg_finish(sums, counts, dist, cb)
             return new, counts, mean
         x, cb = _vectors(x), _books(cb)
-        new = torch.empty((heads, K, dim), dtype=torch.float32, device=device)
-        counts = torch.empty((heads, parts, K), dtype=torch.int64, device=device)
-        mean = torch.empty((heads, parts), dtype=torch.float64, device=device)
+        new = torch.empty(heads, K, dim, dtype=torch.float32, device=device)
+        counts = torch.empty(heads, parts, K, dtype=torch.int64, device=device)
+        mean = torch.empty(heads, parts, dtype=torch.float64, device=device)
         need = lib.vq_cache_lbg_ws_bytes(tokens, heads, dim, sub, K)
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         self._launch("vq_cache_lbg_iterate", x.data_ptr(), x.stride(0), x.stride(1), tokens, cb.data_ptr(), heads, dim, sub, K, _DTYPES[x.dtype],
