@@ -399,6 +399,26 @@ def test_attention_hints_do_not_change_results(eng, max_q, max_kv):
     check_attention(out, lse, attention64(*case, 4, 1.0 / math.sqrt(128)), 900)
 
 
+@pytest.mark.parametrize("max_q,max_kv", [(5, 200), (5, 100000), (1, 1), (5, 1600)])
+@pytest.mark.parametrize("seqs,H", [(64, 8), (65, 2), (150, 1)])
+def test_attention_many_sequences(eng, seqs, H, max_q, max_kv):
+    """More sequences than a wave has lanes, some of no rows or no tokens, cut and uncut."""
+    gen = torch.Generator().manual_seed(seqs)
+    n_q, n_kv = (torch.randint(0, top, (seqs,), generator=gen).tolist() for top in (6, 201))
+    n_q[0], n_q[-1], n_kv[-1] = 5, 1, 200
+    case = attention_case(n_q, n_kv, 2 * H, H, 32, 8, 16, 16, torch.bfloat16, seed=seqs)
+    out, lse = eng.cache_attention(*[t.to(DEV) for t in case], max_q, max_kv=max_kv, want_lse=True)
+    check_attention(out, lse, attention64(*case, 8, 32 ** -0.5), max(n_kv))
+
+
+@pytest.mark.parametrize("dtype,D,sub", [(torch.bfloat16, 32, 8), (torch.float16, 64, 4)])
+def test_attention_many_row_tiles(eng, dtype, D, sub):
+    """A sequence of more tiles of rows than a wave has lanes, between short ones."""
+    case = attention_case([3, 1100, 0, 2], [90, 1250, 7, 400], 2, 1, D, sub, 64, 32, dtype, seed=77)
+    out, lse = eng.cache_attention(*[t.to(DEV) for t in case], 1100, want_lse=True)
+    check_attention(out, lse, attention64(*case, sub, D ** -0.5), 1250)
+
+
 def test_attention_strided_q_shared_codebook_repeatable(eng):
     args = ([1, 20], [200, 95], 8, 4, 64, 4, 256, 16, torch.float16)
     q, k_cb, v_cb, *rest = attention_case(*args, seed=60)

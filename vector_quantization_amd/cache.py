@@ -22,6 +22,7 @@ import torch
 
 from ._lib import lib, check, VQ_BF16, VQ_F16, VQ_F32
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)     # (the engine has set the runtime up)
 _DTYPES = {torch.float32: VQ_F32, torch.bfloat16: VQ_BF16, torch.float16: VQ_F16}
 
 
@@ -125,12 +126,11 @@ class CacheOps:
 
     def _launch(self, name, *args):
         """Calls the library on the engine's device and its current stream."""
-        stream = self._stream()
-        if torch.cuda.current_device() == self.device.index:
-            check(getattr(lib, name)(*args, stream), name)
+        if _current_device() == self.device.index:
+            check(getattr(lib, name)(*args, self._stream()), name)
         else:
             with torch.cuda.device(self.device):
-                check(getattr(lib, name)(*args, stream), name)
+                check(getattr(lib, name)(*args, self._stream()), name)
 
     def cache_write(self, k, v, slots, k_cb, v_cb, k_codes, v_codes):
         """Quantises k and v (tokens, heads, dim) and stores the codes at slots (tokens, int64); a slot outside the cache
