@@ -480,7 +480,7 @@ TRAIN = [
     # tokens, heads, dim, sub, K, dtype
     (1, 1, 32, 2, 256, torch.bfloat16), (31, 2, 64, 4, 16, torch.float32), (33, 1, 128, 8, 256, torch.bfloat16), (500, 3, 64, 4, 100, torch.float16),
     (700, 1, 96, 2, 33, torch.float32), (257, 2, 192, 8, 256, torch.float32), (2500, 1, 32, 4, 256, torch.bfloat16), (900, 2, 256, 8, 7, torch.float16),
-    (5000, 1, 32, 8, 256, torch.float32), (300, 2, 96, 8, 256, torch.bfloat16), (300, 1, 96, 4, 1, torch.bfloat16), (4097, 1, 64, 2, 200, torch.float16),
+    (5000, 1, 32, 8, 256, torch.float32), (300, 2, 96, 8, 256, torch.bfloat16), (30000, 1, 32, 8, 100, torch.float16), (20000, 1, 32, 2, 9, torch.float32), (300, 1, 96, 4, 1, torch.bfloat16), (4097, 1, 64, 2, 200, torch.float16),
 ]
 
 

@@ -323,7 +323,7 @@ int lbg(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens
     if (!ws || ws_bytes < need) return fail(VQ_E_WORKSPACE, "workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, need);
     if ((uintptr_t)ws & 15) return fail(VQ_E_INVALID, "the workspace must start at a multiple of 16 bytes");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    double *part_dist = static_cast<double *>(ws);
+    double2 *part_dist = static_cast<double2 *>(ws);
     float *part_sums = reinterpret_cast<float *>(part_dist + (int64_t)p.chunks * heads * (dim / sub));
     const SearchArgs a = {{x, x}, {token_stride, token_stride}, {head_stride, head_stride}, {cb, cb}, tokens, heads, heads, dim, K, p.pw, p.chunk,
                           nullptr, 0, 0, 0, nullptr, nullptr, part_sums, part_dist};
@@ -449,7 +449,7 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
 size_t vq_cache_lbg_ws_bytes(int64_t tokens, int heads, int dim, int sub, int K) {
     if (tokens <= 0 || tokens > 0x7fffffff || check_shape(heads, dim, sub, K)) return 0;
     const SearchPlan p = vq_internal_search_plan(tokens, heads, dim, sub, 1);
-    return (size_t)p.chunks * heads * (dim / sub) * ((sub + 1) * 256 * 4 + 8);
+    return (size_t)p.chunks * heads * (dim / sub) * ((sub + 1) * 256 * 4 + 16);
 }
 
 int vq_cache_lbg_accum(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens, const float *cb, int heads, int dim,

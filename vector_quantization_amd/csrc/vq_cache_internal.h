@@ -69,7 +69,7 @@ struct SearchArgs {
     int page, page_shift;              // page = 1 << page_shift, or page_shift < 0
     uint8_t *k_codes, *v_codes;
     float *part_sums;                  // training: (chunks, heads * parts, sub + 1, 256), the last plane the counts
-    double *part_dist;                 // (chunks, heads * parts)
+    double2 *part_dist;                // (chunks, heads * parts): squared distances and vectors that count
 };
 
 struct SearchPlan {

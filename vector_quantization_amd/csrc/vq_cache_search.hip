@@ -170,6 +170,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
 
     f32x4 sum[TRAIN ? SUB + 1 : 1];
     double away = 0.0;
+    int counted = 0;
     if constexpr (TRAIN)
 #pragma unroll
         for (int e = 0; e <= SUB; ++e) sum[e] = (f32x4){0, 0, 0, 0};
@@ -319,6 +320,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
             for (int e = 0; e < SUB; ++e) fine = fine && fabsf(x[e]) < COUNTED;
             // sums by products with the one-hot numbers of the codewords: number = 16 hi + lo, and
             // sum[hi][lo] = sum over vectors of (x where its hi is this row) * (1 where its lo is this column)
+            counted += __popcll(__ballot(fine));
             if (fine) {
                 double f = 0.0;
 #pragma unroll
@@ -372,57 +374,72 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
             for (int i = 0; i < 4; ++i) a.part_sums[(place * (SUB + 1) + e) * 256 + (4 * (lane >> 4) + i) * 16 + (lane & 15)] = sum[e][i];
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) away += __shfl_xor(away, o);
-        if (lane == 0) a.part_dist[place] = away;
+        if (lane == 0) a.part_dist[place] = make_double2(away, (double)counted);
     }
 }
 
-// Adds the chunks' sums, in fp64 and in a fixed order: a workgroup for each head and part, four threads for each codeword, each of
-// them a quarter of the chunks.  Reads (sub + 1) KB a chunk once; where a new codebook is asked for it also divides, and the sums are not
-// stored.  5 to 11 us (64 workgroups of 9 KB a chunk and 64 chunks: 11): launch and latency.
-constexpr int GATHER_SIDE = 4;
+// Adds the chunks' sums, in fp64 and in an order that follows from the sizes.  A workgroup takes C = 1 << shift codewords of a head and part;
+// its 1024 threads are C codewords by 1024 / C shares of the chunks.  Reads (sub + 1) KB a chunk once; where a new codebook is asked for it
+// also divides, and the sums are not stored.  Bound by latency and by the chunks' sums coming back (64 groups of 32 chunks, 19 MB: 8.4 us): C
+// falls, to a cache line's 32, until there are workgroups for all compute units or a thread has one chunk (parts of 4, 16 groups of 470
+// chunks: 39.7 us for the iteration with 256 codewords to a workgroup, 26.2 so; 12 groups, parts of 8, 146 chunks: 46.6, 32.2, and with
+// 16 codewords 37.3).
+constexpr int GATHER_THREADS = 1024;
+__device__ inline double wave_sum(double v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    return v;
+}
 template <int SUB>
-__global__ __launch_bounds__(256 * GATHER_SIDE) void k_lbg_gather(const float *__restrict__ part_sums, const double *__restrict__ part_dist, int chunks,
-                                                                  const LbgOut out) {
-    __shared__ double s_sum[GATHER_SIDE - 1][SUB + 1][256], s_away[256 * GATHER_SIDE], s_n[256 * GATHER_SIDE];
-    const int parts = out.dim / SUB, h = blockIdx.x / parts, m = blockIdx.x % parts;
-    const int k = threadIdx.x & 255, side = threadIdx.x >> 8;
+__global__ __launch_bounds__(GATHER_THREADS) void k_lbg_gather(const float *__restrict__ part_sums, const double2 *__restrict__ part_dist, int chunks,
+                                                               int shift, const LbgOut out) {
+    __shared__ double s_sum[SUB + 1][GATHER_THREADS], s_away[GATHER_THREADS / 64], s_n[GATHER_THREADS / 64];
+    const int tid = threadIdx.x, parts = out.dim / SUB, h = blockIdx.x / parts, m = blockIdx.x % parts;
+    const int k = (blockIdx.y << shift) + (tid & ((1 << shift) - 1)), side = tid >> shift, sides = GATHER_THREADS >> shift;
     const int64_t groups = (int64_t)out.heads * parts;
     double sum[SUB + 1];
 #pragma unroll
     for (int e = 0; e <= SUB; ++e) sum[e] = 0.0;
 #pragma unroll 4
-    for (int c = side; c < chunks; c += GATHER_SIDE) {
+    for (int c = side; c < chunks; c += sides) {
         const float *p = part_sums + (c * groups + blockIdx.x) * ((SUB + 1) * 256) + k;
 #pragma unroll
         for (int e = 0; e <= SUB; ++e) sum[e] += (double)p[e * 256];
     }
-    double away = 0.0;
-    for (int c = threadIdx.x; c < chunks; c += 256 * GATHER_SIDE) away += part_dist[c * groups + blockIdx.x];
-    s_away[threadIdx.x] = away;
-    s_n[threadIdx.x] = sum[SUB];                                          // every vector that counts is a member of one codeword
-    if (side > 0)
 #pragma unroll
-        for (int e = 0; e <= SUB; ++e) s_sum[side - 1][e][k] = sum[e];
+    for (int e = 0; e <= SUB; ++e) s_sum[e][tid] = sum[e];
+    if (blockIdx.y == 0) {
+        double away = 0.0, n = 0.0;
+        for (int c = tid; c < chunks; c += GATHER_THREADS) {
+            const double2 d = part_dist[c * groups + blockIdx.x];
+            away += d.x, n += d.y;
+        }
+        away = wave_sum(away), n = wave_sum(n);
+        if ((tid & 63) == 0) s_away[tid >> 6] = away, s_n[tid >> 6] = n;
+    }
     __syncthreads();
-    for (int o = 128 * GATHER_SIDE; o; o >>= 1) {
-        if ((int)threadIdx.x < o) s_away[threadIdx.x] += s_away[threadIdx.x + o], s_n[threadIdx.x] += s_n[threadIdx.x + o];
+    for (int o = sides / 2; o; o >>= 1) {
+        if (side < o)
+#pragma unroll
+            for (int e = 0; e <= SUB; ++e) s_sum[e][tid] += s_sum[e][tid + (o << shift)];
         __syncthreads();
     }
-    if (side > 0) return;
-#pragma unroll
-    for (int e = 0; e <= SUB; ++e)
-        for (int x = 0; x < GATHER_SIDE - 1; ++x) sum[e] += s_sum[x][e][k];
-    if (k < out.K) {
+    if (side == 0 && k < out.K) {
+        const double n = s_sum[SUB][tid];
         const int64_t at = ((int64_t)h * out.K + k) * out.dim + m * SUB;
-        out.counts[(int64_t)blockIdx.x * out.K + k] = (int64_t)sum[SUB];
+        out.counts[(int64_t)blockIdx.x * out.K + k] = (int64_t)n;
 #pragma unroll
         for (int e = 0; e < SUB; ++e) {
-            const double s = sum[e] * (1.0 / (double)SUM_SCALE);
-            if (out.cb_new) out.cb_new[at + e] = sum[SUB] > 0.0 ? (float)(s / sum[SUB]) : out.cb_old[at + e];
+            const double s = s_sum[e][tid] * (1.0 / (double)SUM_SCALE);
+            if (out.cb_new) out.cb_new[at + e] = n > 0.0 ? (float)(s / n) : out.cb_old[at + e];
             else out.sums[at + e] = s;
         }
     }
-    if (k == 0) out.dist[blockIdx.x] = out.cb_new ? (s_n[0] > 0.0 ? s_away[0] / s_n[0] : 0.0) : s_away[0];
+    if (blockIdx.y == 0 && tid == 0) {
+        double away = 0.0, n = 0.0;
+        for (int w = 0; w < GATHER_THREADS / 64; ++w) away += s_away[w], n += s_n[w];
+        out.dist[blockIdx.x] = out.cb_new ? (n > 0.0 ? away / n : 0.0) : away;
+    }
 }
 
 template <typename T, typename C, int SUB, bool TRAIN>
@@ -449,12 +466,13 @@ SearchPlan vq_internal_search_plan(int64_t tokens, int heads, int dim, int sub, 
     p.pw = parts % 8 ? 4 : 8;
     const int64_t side = SEARCH_WAVES / p.pw;                             // token ranges side by side in one workgroup
     const int64_t base = (int64_t)heads * (parts / p.pw) * both;
-    // A workgroup takes 8 parts, or 4 where they do not come by eights (dims of 96 by 8); two workgroups for each compute unit.  A write
-    // is spread as thinly as turns of 64 tokens allow (256 tokens: 7.8 us; turns of 128 9.4).  A training chunk of fewer than 128 costs
-    // more to gather than it saves (1000 vectors, 4 heads: 19.4 us; of 64 20.1, of 256 23.1), and none is longer than 4096: its sums are fp32.
+    // A workgroup takes 8 parts, or 4 where they do not come by eights (dims of 96 by 8); two workgroups for each compute unit, or one in
+    // training by parts of 8, whose registers leave no room for two (8192 vectors, 4 heads: 45 us; in two rounds 54).  A write is spread as
+    // thinly as turns of 64 tokens allow (256 tokens: 7.8 us; turns of 128 9.4).  A training chunk of fewer than 128 costs more to gather
+    // than it saves (1000 vectors, 4 heads: 19.4 us; of 64 20.1, of 256 23.1), and none is longer than 4096: its sums are fp32.
     const int fewest = both == 2 ? 64 : 128, longest = both == 2 ? 1 << 24 : 4096;
     const int64_t most = (tokens + fewest * side - 1) / (fewest * side), least = (tokens + longest * side - 1) / (longest * side);
-    int64_t n = (2 * CUS + base - 1) / base;
+    int64_t n = ((both == 2 || sub < 8 ? 2 : 1) * CUS + base - 1) / base;
     n = n < most ? n : most;
     n = n > least ? n : least;
     p.chunk = (int)(((tokens + n * side - 1) / (n * side) + 63) / 64 * 64);
@@ -477,9 +495,13 @@ hipError_t vq_internal_search(const SearchArgs &a, int sub, int dtype, bool trai
 }
 
 hipError_t vq_internal_lbg_gather(const SearchArgs &a, int sub, int chunks, const LbgOut &out, hipStream_t stream) {
-    const dim3 grid(a.heads * (a.dim / sub)), block(256 * GATHER_SIDE);
-    if (sub == 2) hipLaunchKernelGGL(k_lbg_gather<2>, grid, block, 0, stream, a.part_sums, a.part_dist, chunks, out);
-    else if (sub == 4) hipLaunchKernelGGL(k_lbg_gather<4>, grid, block, 0, stream, a.part_sums, a.part_dist, chunks, out);
-    else hipLaunchKernelGGL(k_lbg_gather<8>, grid, block, 0, stream, a.part_sums, a.part_dist, chunks, out);
+    const int groups = a.heads * (a.dim / sub);
+    int shift = 8;
+    auto across = [&]() { return (out.K + (1 << shift) - 1) >> shift; };
+    while (shift > 5 && (out.K <= 1 << (shift - 1) || (groups * across() < 256 && chunks > GATHER_THREADS >> shift))) --shift;
+    const dim3 grid(groups, across()), block(GATHER_THREADS);
+    if (sub == 2) hipLaunchKernelGGL(k_lbg_gather<2>, grid, block, 0, stream, a.part_sums, a.part_dist, chunks, shift, out);
+    else if (sub == 4) hipLaunchKernelGGL(k_lbg_gather<4>, grid, block, 0, stream, a.part_sums, a.part_dist, chunks, shift, out);
+    else hipLaunchKernelGGL(k_lbg_gather<8>, grid, block, 0, stream, a.part_sums, a.part_dist, chunks, shift, out);
     return hipGetLastError();
 }
