@@ -59,10 +59,11 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
  * grouped: head h reads cache head h / (q_heads / heads).  rows * q_heads / heads is below 2^30, width * page below 2^31,
  * q_heads at most 4096, seqs at most 65535.  out and lse overlap no other tensor of the call.
  *   out (rows, q_heads, dim) = softmax(scale * q k^T) v      lse (rows, q_heads, nullable) = log sum exp(scale * q k^T)
- * A row that sees no token, or whose scores are all minus infinity, gets zeros and minus infinity; rows of no sequence are left as they were.  Lengths past
- * the table's width are cut to it; the tokens of a page number outside [0, pages) are not seen.  Codewords have to be
- * finite; a code of K or more stands for some codeword or for zeros.  max_q and max_kv, the longest of the sequences' rows and lengths as the caller knows them, only shape
- * the launch: any value of 1 or more gives the same sums, up to the order of addition.
+ * A row that sees no token, or whose scores are all minus infinity, gets zeros and minus infinity; rows of no sequence
+ * are left as they were.  Lengths past the table's width are cut to it; the tokens of a page number outside [0, pages)
+ * are not seen.  Codewords have to be finite; a code of K or more stands for some codeword or for zeros.  max_q and
+ * max_kv, the longest of the sequences' rows and lengths as the caller knows them, only shape the launch: any value of
+ * 1 or more gives the same sums, up to the order of addition.
  * `starts` rises, from 0 or more to `rows` or less.  dtype: VQ_BF16 or VQ_F16. */
 size_t vq_cache_attention_ws_bytes(int64_t rows, int q_heads, int heads, int dim, int sub, int K, int seqs,
                                    int64_t max_q, int64_t max_kv);
@@ -75,10 +76,12 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
 
 /* The accumulating half of an LBG iteration of float codebooks: over `tokens` tokens' vectors x, for each head,
  * part and codeword, the sum and number of the vectors nearest to it (as in vq_cache_write), and for each head and part
- * the sum of the least squared distances.  A vector of which a number is 2^100 or more in size, or no number, is left out of all three.
- * sums (heads, K, dim) fp64, counts (heads, parts, K) int64, dist (heads, parts) fp64 are overwritten; the result
- * does not depend on timing.  cb is (heads, K, dim) fp32; x is of any of the three types; at most 65535 chunks
- * of 4096 tokens (268 million) a call; a codeword's sum over a chunk stays below 2^104 (of numbers below 2^92 it always does).  Adding several calls' sums, counts and dist gives those of their tokens together. */
+ * the sum of the least squared distances.  A vector of which a number is 2^100 or more
+ * in size, or no number, is left out of all three.  sums (heads, K, dim) fp64, counts (heads, parts, K) int64, dist
+ * (heads, parts) fp64 are overwritten; the result does not depend on timing.  cb is (heads, K, dim) fp32; x is of any
+ * of the three types.  A call takes 65535 chunks of 4096 tokens (268 million); a codeword's sum over a chunk has to stay
+ * below 2^104, as that of numbers below 2^92 always does.  Adding several calls' sums, counts and dist gives those of their
+ * tokens together. */
 size_t vq_cache_lbg_ws_bytes(int64_t tokens, int heads, int dim, int sub, int K);
 int vq_cache_lbg_accum(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens,
                        const float *cb, int heads, int dim, int sub, int K, int dtype,

@@ -39,7 +39,8 @@ struct ReadArgs {
 };
 
 // Codes -> vectors.  Bound by the writes: 65536 tokens of 8 heads and 128 dims, 268 MB of vectors out of 34 MB of codes, take 54 us, 5.6 TB/s;
-// a copy reaches 5.0.  A few tokens are 4 us of latency.  A thread writes 16 bytes, 8 numbers of 8 / SUB codewords; neighbouring threads write neighbouring ones.
+// a copy reaches 5.0.  A few tokens are 4 us of latency.  A thread writes 16 bytes, 8 numbers of 8 / SUB codewords; neighbouring threads
+// write neighbouring ones.
 
 // The 16 bytes that N codes stand for, at place c of a vector.
 template <int D, int SUB> __device__ inline u32x4 expand(const uint8_t *book, uint32_t codes, int K, int c) {
@@ -198,8 +199,9 @@ template <int D, int SUB> hipError_t launch_read(const ReadArgs &a, hipStream_t 
     // What the last cache (256 MB) can keep for whoever reads it next is left there; more is stored past it.  Read and then added up by another
     // kernel, 128 MiB of vectors took 56 us with the caches and 59 past them, 160 MiB 86 and 79, 192 MiB 108 and 90, 512 MiB 314 and
     // 303 (by itself the read of 256 MiB takes 80 and 54).
-    if ((a.tokens < a.chunk ? a.tokens : a.chunk) * (16 / SUB) >= a.K) return a.tokens * a.heads * D * 4 > (int64_t)144 << 20 ? launch_read_many<D, SUB, true>(a, grid, stream) :
-                                                                                 launch_read_many<D, SUB, false>(a, grid, stream);
+    const bool past = a.tokens * a.heads * D * 4 > (int64_t)144 << 20;
+    if ((a.tokens < a.chunk ? a.tokens : a.chunk) * (16 / SUB) >= a.K)
+        return past ? launch_read_many<D, SUB, true>(a, grid, stream) : launch_read_many<D, SUB, false>(a, grid, stream);
     hipLaunchKernelGGL((k_cache_read_few<D, SUB>), grid, dim3(512), 0, stream, a);
     return hipGetLastError();
 }
