@@ -22,7 +22,6 @@ import torch
 
 from ._lib import lib, check, VQ_BF16, VQ_F16, VQ_F32
 
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)     # (the engine has set the runtime up)
 _DTYPES = {torch.float32: VQ_F32, torch.bfloat16: VQ_BF16, torch.float16: VQ_F16}
 
 
@@ -126,7 +125,7 @@ class CacheOps:
 
     def _launch(self, name, *args):
         """Calls the library on the engine's device and its current stream."""
-        if _current_device() == self.device.index:
+        if torch.cuda.current_device() == self.device.index:
             check(getattr(lib, name)(*args, self._stream()), name)
         else:
             with torch.cuda.device(self.device):
