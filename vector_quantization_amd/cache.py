@@ -125,11 +125,12 @@ class CacheOps:
 
     def _launch(self, name, *args):
         """Calls the library on the engine's device and its current stream."""
+        stream = self._stream()
         if torch.cuda.current_device() == self.device.index:
-            check(getattr(lib, name)(*args, self._stream()), name)
+            check(getattr(lib, name)(*args, stream), name)
         else:
             with torch.cuda.device(self.device):
-                check(getattr(lib, name)(*args, self._stream()), name)
+                check(getattr(lib, name)(*args, stream), name)
 
     def cache_write(self, k, v, slots, k_cb, v_cb, k_codes, v_codes):
         """Quantises k and v (tokens, heads, dim) and stores the codes at slots (tokens, int64); a slot outside the cache
