@@ -400,7 +400,7 @@ def test_attention_hints_do_not_change_results(eng, max_q, max_kv):
 
 
 @pytest.mark.parametrize("max_q,max_kv", [(5, 200), (5, 100000), (1, 1), (5, 1600)])
-@pytest.mark.parametrize("seqs,H", [(64, 8), (65, 2), (150, 1)])
+@pytest.mark.parametrize("seqs,H", [(64, 8), (65, 2), (150, 1), (200, 8)])
 def test_attention_many_sequences(eng, seqs, H, max_q, max_kv):
     """More sequences than a wave has lanes, some of no rows or no tokens, cut and uncut."""
     gen = torch.Generator().manual_seed(seqs)

@@ -308,19 +308,25 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
 
     int64_t left = uniform(s_range->left), skip = uniform(s_range->skip), now = uniform(s_range->now);      // now: where item (b, tile) begins
     int b = __builtin_amdgcn_readfirstlane(s_range->seq), tile = __builtin_amdgcn_readfirstlane(s_range->tile);
-    const int held = __builtin_amdgcn_readfirstlane(s_range->held);
+    int held = __builtin_amdgcn_readfirstlane(s_range->held);
     int first = 0, n_q = 0, n_kv = 0;
+    // Rows and length of sequence b: out of LDS for all waves alike, so that they come to every barrier together whatever becomes of the
+    // tensors meanwhile; the next 64 are fetched by one wave.
     auto take_sequence = [&]() {
-        if (b - held < 64) {
-            first = __builtin_amdgcn_readfirstlane(s_seq[3 * (b - held)]);
-            n_q = __builtin_amdgcn_readfirstlane(s_seq[3 * (b - held) + 1]);
-            n_kv = __builtin_amdgcn_readfirstlane(s_seq[3 * (b - held) + 2]);
-        } else {
-            int64_t x;
-            int y, z;
-            sequence(a, b, x, y, z);
-            first = (int)x, n_q = y, n_kv = z;
+        if (b - held >= 64) {
+            lds_barrier();
+            if (wave == 0) {
+                int64_t x = 0;
+                int y = 0, z = 0;
+                if (b + lane < a.seqs) sequence(a, b + lane, x, y, z);
+                s_seq[3 * lane] = (int)x, s_seq[3 * lane + 1] = y, s_seq[3 * lane + 2] = z;
+            }
+            held = b;
+            lds_barrier();
         }
+        first = __builtin_amdgcn_readfirstlane(s_seq[3 * (b - held)]);
+        n_q = __builtin_amdgcn_readfirstlane(s_seq[3 * (b - held) + 1]);
+        n_kv = __builtin_amdgcn_readfirstlane(s_seq[3 * (b - held) + 2]);
     };
     AttendNote note = {-1, 0, 0, 0, 0, 0};
 
