@@ -1,0 +1,63 @@
+"""Values and shapes at which the cache operators (HipEngine.cache_*) could go astray, each for itself, against their definitions in 64 bits."""
+import pytest
+import torch
+
+from test_gpu_cache import DEV, HALF, attention64, attention_case, check_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def eng():
+    from vector_quantization_amd import HipEngine
+    return HipEngine(DEV)
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,hint", [(1, 1), (1, None), (20, 1)])
+@pytest.mark.parametrize("where", ["first", "last", "by turns"])
+@pytest.mark.parametrize("nats", [17.5, 19.0, 24.0, 26.0])
+def test_attention_where_one_token_takes_all_and_gives_nothing(eng, dtype, rows, hint, where, nats):
+    """Tokens whose values are zero hold all but e^-nats of the weight, so the result is what the others add: their weights may not vanish.
+    A hint of one token leaves all the work to one workgroup, in which one wave meets the heavy token and an eighth of the others."""
+    n, D, sub, K, page = 20000, 64, 4, 32, 64
+    q, k_cb, v_cb, kc, vc, table, kv_lens, starts = attention_case([rows], [n], 2, 1, D, sub, K, page, dtype, seed=80)
+    q[:] = 0.25
+    k_cb[:] = ((1 - nats / 16) + (torch.arange(K) - 16) / 512)[:, None].to(dtype)
+    k_cb[:, 0] = 1.0                                                     # its score is 16, the others' lie about `nats` below
+    v_cb[:] = (1e4 + 1e4 * torch.rand((1, K, D), generator=torch.Generator().manual_seed(81))).to(dtype)
+    v_cb[:, 0] = 0.0
+    kc.clamp_(min=1), vc.clamp_(min=1)
+    j = torch.arange(n)
+    heavy = {"first": j == 5, "last": j == n - 30, "by turns": j // 256 % 2 == 0}[where]      # (256: a tile for each of eight waves)
+    at, off = table[0].long()[j[heavy] // page], j[heavy] % page
+    kc[at, :, off], vc[at, :, :, off] = 0, 0
+    case = (q, k_cb, v_cb, kc, vc, table, kv_lens, starts)
+    out, lse = eng.cache_attention(*[t.to(DEV) for t in case], hint or rows, max_kv=hint, scale=1.0, want_lse=True)
+    ref, ref_lse, size, slip = attention64(*case, sub, 1.0)
+    half = HALF[dtype]
+    # as check_attention; results below fp16's normal numbers are off by half of 2^-24; and the 31 tokens beside the heavy one in its tile have weights
+    # that are off by 2^-33 of its own at most (half of 2^-24, where its own is 2^8 or more)
+    tol = half * (1 + half) * (ref.abs() + size) + (2 * slip + (n + 8) * 2.0 ** -23) * size + 2.0 ** -25 + 31 * 2.0 ** -33 * v_cb.max().double()
+    assert (tol <= 0.25 * ref).any() or where == "by turns"
+    off = (out.cpu().double() - ref).abs()
+    assert (off <= tol).all(), float((off / ref).max())
+    assert ((lse.cpu().double() - ref_lse).abs() <= slip[..., 0] + (n + 8) * 2.0 ** -23 + 2.0 ** -21 * ref_lse.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_levels_far_apart(eng, dtype):
+    """Tiles whose scores fall and rise by up to a thousand: maxima move both ways, nothing overflows, only what is too small to be seen is lost."""
+    n, D, sub, K, page = 3000, 64, 4, 64, 64
+    q, k_cb, v_cb, kc, vc, table, kv_lens, starts = attention_case([3], [n], 2, 1, D, sub, K, page, dtype, seed=85)
+    q[:] = 0.25
+    level = torch.randint(0, K, (n,), generator=torch.Generator().manual_seed(86))
+    level = level[torch.arange(n) // 32 * 32]                            # one level to a tile
+    k_cb[:] = (torch.arange(K) - K / 2)[:, None].to(dtype)
+    kc[table[0].long()[torch.arange(n) // page], :, torch.arange(n) % page] = level[:, None, None].to(torch.uint8)
+    for scale in (1.0, 0.25, 1 / 64):
+        case = (q, k_cb, v_cb, kc, vc, table, kv_lens, starts)
+        out, lse = eng.cache_attention(*[t.to(DEV) for t in case], 1, max_kv=1, scale=scale, want_lse=True)
+        check_attention(out, lse, attention64(*case, sub, scale), n)

@@ -23,9 +23,10 @@
 // Measured and not kept: 64 rows to a workgroup (863 us for that chunk, where 32 took 690), 16 waves (75 us where 8 took 62 for
 // the 16 sequences).
 //
-// Softmax in base 2 with a running maximum per row that is only moved once a score exceeds it by 8 (weights stay
-// below 2^8, sums are fp32), so that most tiles need neither a reduction across lanes nor a rescaling.  Weights are rounded to the cache's type
-// for the second product (half a step, as the values themselves are of that type); the sum of weights takes them unrounded.
+// Softmax in base 2.  A row's weights are taken against a running reference: for bf16 the largest score so far, moved only once a score
+// exceeds it by 8 (weights stay below 2^8, sums are fp32), so that most tiles need neither a reduction across lanes nor a rescaling.  Weights are
+// rounded to the cache's type for the second product (half a step, as the values themselves are of that type); the sum of weights takes them
+// unrounded.  fp16 has 2^-14 to 2^16 for that, so there the reference follows the scores both ways: see Reference.
 
 #include "vq_cache_internal.h"
 
@@ -106,9 +107,15 @@ __device__ inline void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-__device__ inline float wave_any_max(float v) {          // the maximum over the four lanes of one row
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+// The maximum over the four lanes of one row, to each of them, by the VALU alone: a shuffle through LDS would wait for the look-ups under way.
+__device__ inline float wave_any_max(float v) {
+    uint32_t bits = __builtin_bit_cast(uint32_t, v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);       // rows 0, 0, 2, 2 and 1, 1, 3, 3 of 16 lanes
+    const uint32_t even = rows[0], odd = rows[1];
+    bits = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, even), __builtin_bit_cast(float, odd)));
+    const auto halves = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+    const uint32_t low = halves[0], high = halves[1];
+    return fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
 }
 
 // A value that every lane holds, in scalar registers: what follows from it stays there.
@@ -136,15 +143,35 @@ __device__ inline int64_t of_last_lane(int64_t v) {
     return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, 63) | (int64_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32;
 }
 
-// 8 numbers of a finished row, place = row * q_heads + head: v against the maximum `most` (base 2) and the sum of weights.
+// 8 numbers of a finished row, place = row * q_heads + head: v against the reference `most` (base 2) and the sum of weights.
 template <typename T>
 __device__ inline void store_row(const AttendArgs &a, int64_t place, int D, int c, f32x4 v0, f32x4 v1, float most, float sum) {
     const float over = sum == 0.0f ? 0.0f : 1.0f / sum;              // 0: the row sees no token (of any other the largest weight is 1 or more)
     *reinterpret_cast<u32x4 *>(static_cast<T *>(a.out) + place * D + c * 8) =
         (u32x4){pack2<T>(v0[0] * over, v0[1] * over), pack2<T>(v0[2] * over, v0[3] * over),
                 pack2<T>(v1[0] * over, v1[1] * over), pack2<T>(v1[2] * over, v1[3] * over)};
-    if (c == 0 && a.lse) a.lse[place] = sum == 0.0f ? -INFINITY : most * 0.69314718055994531f + logf(sum);
+    // (the sum's power of two goes to `most` first: where the reference came down far, the two are large and nearly cancel)
+    if (c == 0 && a.lse)
+        a.lse[place] = sum == 0.0f ? -INFINITY : ((most + (float)__builtin_amdgcn_frexp_expf(sum)) + log2f(__builtin_amdgcn_frexp_mantf(sum))) * 0.69314718055994531f;
 }
+
+// How a row's reference follows its scores.  It is moved where a tile's largest weight leaves 2^LEAST .. 2^MOST, to where that is 2^AIM or a
+// little more; for bf16, whose weights have fp32's range, to the maximum itself and never down.  In fp16 a weight below 2^-14 loses bits and one
+// below 2^-25 is nothing, and a reference that only rose would do that to all tokens of a wave behind one heavy token: with a heavy token whose
+// value is zero and 20000 others 17 to 26 nats below it, an eighth of the result was lost.  With one that comes down again a weight is
+// off by half a step, or by 2^-19 of the largest in its own tile (2^-33 where that has just moved the reference).  References of
+// fp16 are whole numbers, so moving is exact, and come down only as far as the row's sum stays below 2^92 (the products' sums, up
+// to 2^16 times that, then stay inside fp32).  Scores of a few nats move it no oftener than before (512 rows on 8192 tokens, 128 dims by 4: 129 us);
+// with a deviation of 4 nats it takes 136 us where 126 were, of 8 nats 145.
+template <typename T> struct Reference {
+    static constexpr bool BOTH_WAYS = false;
+    static constexpr float MOST = 8.0f;
+};
+template <> struct Reference<_Float16> {
+    static constexpr bool BOTH_WAYS = true;
+    static constexpr float MOST = 15.0f, AIM = 8.0f, LEAST = -6.0f;
+    static constexpr int SUM_MOST = 90;
+};
 
 // The tiles that the rows of one item see: rows tile * RB * 16 on of a sequence, whose row i sees tokens 0 .. n_kv - n_q + i.
 template <int RB> __device__ inline int tiles_of(int tile, int n_q, int n_kv, int group) {
@@ -527,15 +554,31 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) best = fmaxf(best, z[rb][s][i]);
                 best *= a.scale2;
-                if (__any(best > top[rb] + 8.0f)) {
-                    const float now = fmaxf(top[rb], wave_any_max(best));
-                    const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[rb] - now);
-                    top[rb] = now;
-                    total[rb] *= keep;
+                using Ref = Reference<T>;
+                bool leaves = best > top[rb] + Ref::MOST;
+                if constexpr (Ref::BOTH_WAYS) leaves = leaves || best < top[rb] + Ref::LEAST;
+                if (__any(leaves)) {
+                    const float most = wave_any_max(best);
+                    float now = fmaxf(top[rb], most);
+                    if constexpr (Ref::BOTH_WAYS) {               // (most tiles that come here have a lane's 8 tokens below the row's 32, no more)
+                        const bool falls = most < top[rb] + Ref::LEAST && most > -INFINITY;
+                        const float aim = floorf(most) - Ref::AIM;
+                        now = most > top[rb] + Ref::MOST ? aim : top[rb];
+                        if (__any(falls)) {
+                            // (a lane has a quarter of its row's sum, and its exponent leaves out up to a bit more)
+                            const float room = (float)(Ref::SUM_MOST + 127 - (int)(__builtin_bit_cast(uint32_t, wave_any_max(total[rb])) >> 23));
+                            if (falls) now = fmaxf(aim, top[rb] - fmaxf(room, 0.0f));
+                        }
+                    }
+                    if (!Ref::BOTH_WAYS || __any(now != top[rb])) {
+                        const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[rb] - now);
+                        top[rb] = now;
+                        total[rb] *= keep;
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
+                        for (int u = 0; u < U; ++u)
 #pragma unroll
-                        for (int e = 0; e < E; ++e) o[rb][u][e] *= keep;
+                            for (int e = 0; e < E; ++e) o[rb][u][e] *= keep;
+                    }
                 }
                 const float base = top[rb] == -INFINITY ? 0.0f : -top[rb];
 #pragma unroll
