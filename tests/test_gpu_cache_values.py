@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_cache import DEV, HALF, attention64, attention_case, check_attention
+from test_gpu_cache import DEV, HALF, attention64, attention_case, check_attention, vectors64
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,31 @@ def test_attention_levels_far_apart(eng, dtype):
         case = (q, k_cb, v_cb, kc, vc, table, kv_lens, starts)
         out, lse = eng.cache_attention(*[t.to(DEV) for t in case], 1, max_kv=1, scale=scale, want_lse=True)
         check_attention(out, lse, attention64(*case, sub, scale), n)
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 2e4), (torch.bfloat16, 2e4), (torch.bfloat16, 1e8), (torch.bfloat16, 1e15)])
+@pytest.mark.parametrize("n_q,n_kv", [([1, 1], [700, 90]), ([20, 40], [300, 64])])
+def test_attention_scores_whose_steps_are_large(eng, dtype, size, n_q, n_kv):
+    """Scores of 10^10 and more, where neighbouring fp32 numbers are far apart: the largest takes all, and its value comes back as it is."""
+    D, sub, K = 64, 4, 256
+    case = list(attention_case(n_q, n_kv, 4, 2, D, sub, K, 16, dtype, seed=90))
+    case[0], case[1] = (case[0].float().clamp(-3, 3) * size).to(dtype), (case[1].float().clamp(-3, 3) * size).to(dtype)
+    ref, ref_lse, _, slip = attention64(*case, sub, 1.0)
+    # rows whose two largest scores could change places are left out: their weights are 0 and 1 to the last bit everywhere else
+    out, lse = eng.cache_attention(*[t.to(DEV) for t in case], max(n_q), scale=1.0, want_lse=True)
+    out, lse = out.cpu().double(), lse.cpu().double()
+    assert out.isfinite().all() and lse.isfinite().all()
+    assert ((lse - ref_lse).abs() <= slip[..., 0] + 2.0 ** -21 * ref_lse.abs()).all()
+    q, k_cb, _, kc, _, table, kv_lens, starts = case
+    sure = torch.zeros(out.shape[:2], dtype=torch.bool)
+    for b in range(len(n_q)):
+        j = torch.arange(n_kv[b])
+        for h in range(2):
+            kd = vectors64(kc[table[b].long()[j // 16], h, j % 16], k_cb[h], sub)
+            for r in range(int(starts[b]), int(starts[b + 1])):
+                see = j <= n_kv[b] - int(starts[b + 1]) + r
+                for g in (2 * h, 2 * h + 1):
+                    z = (kd[see] @ q[r, g].double()).sort(descending=True)[0]
+                    sure[r, g] = len(z) == 1 or z[0] - z[1] > 2 * slip[r, g, 0] + 200
+    assert sure.float().mean() > 0.9
+    assert torch.equal(out[sure], ref[sure])

@@ -155,6 +155,11 @@ __device__ inline void store_row(const AttendArgs &a, int64_t place, int D, int 
         a.lse[place] = sum == 0.0f ? -INFINITY : ((most + (float)__builtin_amdgcn_frexp_expf(sum)) + log2f(__builtin_amdgcn_frexp_mantf(sum))) * 0.69314718055994531f;
 }
 
+// From here on a score's rounding is no longer small against 1: scores are then rounded as their maximum was before it is taken off, so that the
+// largest weight is what the reference says.  (Multiplied and subtracted at once, a score of 10^10 missed its own maximum by up to
+// 2^9, and its weight was infinite or nothing.)
+constexpr float LARGE = 0x1p20f;
+
 // How a row's reference follows its scores.  It is moved where a tile's largest weight leaves 2^LEAST .. 2^MOST, to where that is 2^AIM or a
 // little more; for bf16, whose weights have fp32's range, to the maximum itself and never down.  In fp16 a weight below 2^-14 loses bits and one
 // below 2^-25 is nothing, and a reference that only rose would do that to all tokens of a wave behind one heavy token: with a heavy token whose
@@ -444,6 +449,7 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
     while (more) {
         f32x4 o[RB][U][E];
         float top[RB], total[RB];
+        bool large = false;                                       // some row's reference is LARGE
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             top[rb] = -INFINITY;
@@ -541,29 +547,31 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
             const bool whole = have == 3 && t * TILE + TILE - 1 <= all_see;
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                if (!whole) {
+                float by = large ? 1.0f : a.scale2;               // what is still to be multiplied by
+                if (!whole || large) {
+                    const float times = large ? a.scale2 : 1.0f;
 #pragma unroll
                     for (int s = 0; s < 2; ++s)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (!(have >> s & 1) || t * TILE + 16 * s + 4 * g + i > sees[rb]) z[rb][s][i] = -INFINITY;
+                            z[rb][s][i] = !(have >> s & 1) || t * TILE + 16 * s + 4 * g + i > sees[rb] ? -INFINITY : z[rb][s][i] * times;
                 }
                 float best = -INFINITY;
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) best = fmaxf(best, z[rb][s][i]);
-                best *= a.scale2;
+                best *= by;
                 using Ref = Reference<T>;
-                bool leaves = best > top[rb] + Ref::MOST;
-                if constexpr (Ref::BOTH_WAYS) leaves = leaves || best < top[rb] + Ref::LEAST;
+                bool leaves = best - top[rb] > Ref::MOST;         // (not best > top + MOST: large scores would round it away)
+                if constexpr (Ref::BOTH_WAYS) leaves = leaves || best - top[rb] < Ref::LEAST;
                 if (__any(leaves)) {
                     const float most = wave_any_max(best);
                     float now = fmaxf(top[rb], most);
                     if constexpr (Ref::BOTH_WAYS) {               // (most tiles that come here have a lane's 8 tokens below the row's 32, no more)
-                        const bool falls = most < top[rb] + Ref::LEAST && most > -INFINITY;
-                        const float aim = floorf(most) - Ref::AIM;
-                        now = most > top[rb] + Ref::MOST ? aim : top[rb];
+                        const bool falls = most - top[rb] < Ref::LEAST && most > -INFINITY;
+                        const float aim = fabsf(most) < LARGE ? floorf(most) - Ref::AIM : most;
+                        now = most - top[rb] > Ref::MOST ? aim : top[rb];
                         if (__any(falls)) {
                             // (a lane has a quarter of its row's sum, and its exponent leaves out up to a bit more)
                             const float room = (float)(Ref::SUM_MOST + 127 - (int)(__builtin_bit_cast(uint32_t, wave_any_max(total[rb])) >> 23));
@@ -578,13 +586,20 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
                         for (int u = 0; u < U; ++u)
 #pragma unroll
                             for (int e = 0; e < E; ++e) o[rb][u][e] *= keep;
+                        if (!large && __any(fabsf(now) >= LARGE && now > -INFINITY)) {
+                            large = true, by = 1.0f;
+#pragma unroll
+                            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) z[rb][s][i] *= a.scale2;
+                        }
                     }
                 }
                 const float base = top[rb] == -INFINITY ? 0.0f : -top[rb];
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) z[rb][s][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[rb][s][i], a.scale2, base));
+                    for (int i = 0; i < 4; ++i) z[rb][s][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[rb][s][i], by, base));
                 total[rb] += ((z[rb][0][0] + z[rb][0][1]) + (z[rb][0][2] + z[rb][0][3])) + ((z[rb][1][0] + z[rb][1][1]) + (z[rb][1][2] + z[rb][1][3]));
                 w[rb] = (u32x4){pack2<T>(z[rb][0][0], z[rb][0][1]), pack2<T>(z[rb][0][2], z[rb][0][3]),
                                 pack2<T>(z[rb][1][0], z[rb][1][1]), pack2<T>(z[rb][1][2], z[rb][1][3])};
