@@ -89,3 +89,12 @@ def test_attention_scores_whose_steps_are_large(eng, dtype, size, n_q, n_kv):
                     sure[r, g] = len(z) == 1 or z[0] - z[1] > 2 * slip[r, g, 0] + 200
     assert sure.float().mean() > 0.9
     assert torch.equal(out[sure], ref[sure])
+
+
+@pytest.mark.parametrize("scale", [3e-38, -2e-39, 1e-44])
+def test_attention_tiny_scale(eng, scale):
+    """A scale near or below fp32's smallest normal number is taken as it is."""
+    case = list(attention_case([1, 20], [300, 95], 4, 2, 64, 4, 256, 16, torch.bfloat16, seed=95))
+    case[0], case[1] = (case[0].float() * 1e18).to(torch.bfloat16), (case[1].float() * 1e18).to(torch.bfloat16)
+    out, lse = eng.cache_attention(*[t.to(DEV) for t in case], 20, scale=scale, want_lse=True)
+    check_attention(out, lse, attention64(*case, 4, scale), 300)

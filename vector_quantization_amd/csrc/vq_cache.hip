@@ -438,7 +438,7 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
     float *part_o = static_cast<float *>(ws);
     float2 *part_ml = reinterpret_cast<float2 *>(part_o + r.slots * r.p.rb * 16 * dim);
     AttendArgs a = {q, q_token_stride, q_head_stride, rows, q_heads, {k_cb, v_cb}, cb_heads, heads, K, rows_padded(K), {k_codes, v_codes}, pages,
-                    page, table, seqs, width, kv_lens, starts, (float)fmax(fabs(scale) * 1.4426950408889634, 1e-37), scale < 0 ? 0x80008000u : 0u,
+                    page, table, seqs, width, kv_lens, starts, (float)fmax(fabs(scale) * 1.4426950408889634, 1e-45), scale < 0 ? 0x80008000u : 0u,
                     out, lse, r.split, r.join_at, r.join_rows, r.seq_at, part_o, part_ml,
                     reinterpret_cast<AttendNote *>(part_ml + r.slots * r.p.rb * 16)};
     const dim3 grid(heads, r.parts);

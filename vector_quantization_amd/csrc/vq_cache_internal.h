@@ -38,7 +38,7 @@ struct AttendArgs {
     const int32_t *table;
     int seqs, width;
     const int32_t *kv_lens, *starts;
-    float scale2;                      // |scale| * log2(e), above 0: maxima can be taken before it
+    float scale2;                      // |scale| * log2(e), or fp32's least number: above 0, so that maxima can be taken before it
     uint32_t flip;                     // the sign bits of two 16-bit numbers where scale < 0: q is negated instead
     void *out;
     float *lse;
