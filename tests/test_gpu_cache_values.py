@@ -1,8 +1,9 @@
 """Values and shapes at which the cache operators (HipEngine.cache_*) could go astray, each for itself, against their definitions in 64 bits."""
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_cache import DEV, HALF, attention64, attention_case, check_attention, vectors64
+from test_gpu_cache import DEV, HALF, attention64, attention_case, check_attention, codes64, data, vectors64
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +99,24 @@ def test_attention_tiny_scale(eng, scale):
     case[0], case[1] = (case[0].float() * 1e18).to(torch.bfloat16), (case[1].float() * 1e18).to(torch.bfloat16)
     out, lse = eng.cache_attention(*[t.to(DEV) for t in case], 20, scale=scale, want_lse=True)
     check_attention(out, lse, attention64(*case, 4, scale), 300)
+
+
+# ---- search and training ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("sub", [2, 4, 8])
+@pytest.mark.parametrize("K", [2, 5, 17, 20, 21, 33, 37, 256])
+def test_codewords_too_small_to_tell_apart(eng, K, sub):
+    """Codewords of 10^-19 to 10^-12 of the vectors' size: where the sums of 64 bits are equal, the lowest number wins."""
+    T, H, D = 600, 1, 64
+    x = data(7, (T, H, D), torch.bfloat16)
+    x = (x.float() * 10.0 ** (torch.arange(T) % 8).float().reshape(T, 1, 1)).to(torch.bfloat16)
+    cb = (data(8, (H, K, D), torch.float32) * 1e-12).to(torch.bfloat16)
+    code, _ = codes64(x, cb, sub)
+    assert len(np.unique(code)) > 1
+    kc, vc = eng.cache_buffers(38, 16, H, D, sub)
+    eng.cache_write(x.to(DEV), x.to(DEV), torch.arange(T, device=DEV), cb.to(DEV), cb.to(DEV), kc, vc)
+    assert torch.equal(kc.cpu().transpose(1, 2).reshape(608, H, D // sub)[:T].long(), torch.from_numpy(code))
+    assert torch.equal(vc.cpu().permute(0, 3, 1, 2).reshape(608, H, D // sub)[:T].long(), torch.from_numpy(code))
+    _, counts, _ = eng.cache_lbg_accum(x.to(DEV), cb.float().to(DEV), sub)
+    for m in range(D // sub):
+        assert torch.equal(counts[0, m].cpu(), torch.bincount(torch.from_numpy(code[:, 0, m]), minlength=K))

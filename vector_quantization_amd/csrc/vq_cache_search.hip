@@ -167,6 +167,10 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) reach = fmaxf(reach, __shfl_xor(reach, o));
     const float far = __builtin_amdgcn_sqrtf(reach);
+    // A vector longer than this is left to step 3: 2^19 times as long as any codeword, its distances may be equal in fp64 where step 1 can tell them
+    // apart, and then the lowest number is asked for.  (Up to there, what step 1 tells apart differs by 2^-36 |x|^2 or more, fp64 sums
+    // by 2^-47 at most.  Step 2 leaves nearly all of those open by itself, but not in a group of one codeword.)
+    const float size_most = a.K > 1 ? fminf(SIZE_MOST, reach * 0x1p38f) : SIZE_MOST;
 
     f32x4 sum[TRAIN ? SUB + 1 : 1];
     double away = 0.0;
@@ -257,7 +261,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
         const bool upper = h1 < l1;
         const float best = upper ? h1 : l1, second = least(upper ? l1 : h1, least(l2, h2));
         const float bound = 0.5f * reach + __builtin_amdgcn_sqrtf(size) * far;
-        bool open = !(second - best > bound * GAP + 1e-36f) || !(bound < BOUND_MOST) || !(size < SIZE_MOST);
+        bool open = !(second - best > bound * GAP + 1e-36f) || !(bound < BOUND_MOST) || !(size < size_most);
         const int group = __builtin_bit_cast(uint32_t, best) & (2 * NT - 1);      // (a score beyond fp32 names any)
 
         // step 2: rows k0 to k0 + 3 and k0 + 8 to k0 + 11
