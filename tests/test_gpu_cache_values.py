@@ -1,4 +1,6 @@
 """Values and shapes at which the cache operators (HipEngine.cache_*) could go astray, each for itself, against their definitions in 64 bits."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -120,3 +122,24 @@ def test_codewords_too_small_to_tell_apart(eng, K, sub):
     _, counts, _ = eng.cache_lbg_accum(x.to(DEV), cb.float().to(DEV), sub)
     for m in range(D // sub):
         assert torch.equal(counts[0, m].cpu(), torch.bincount(torch.from_numpy(code[:, 0, m]), minlength=K))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,D,sub", [(8, 256, 2), (8, 256, 4), (8, 256, 8)])
+@pytest.mark.parametrize("value", [math.pi, 0.1, -1234.567])
+def test_training_mean_of_equal_vectors(eng, dtype, H, D, sub, value):
+    """Whole chunks of 4096 equal vectors: their mean is that vector within the roundings of 256 of them."""
+    T = 4096 * {2: 4, 4: 8, 8: 8}[sub] + 40
+    x = torch.full((1, 1, 1), value, dtype=dtype, device=DEV).expand(T, H, D).contiguous()
+    x[:, 1] *= 1.5
+    cb = torch.full((H, 3, D), 1e4, device=DEV)
+    cb[:, 1] = value
+    sums, counts, _ = eng.cache_lbg_accum(x, cb, sub)
+    assert (counts[:, :, 1] == T).all()
+    want = x[0].double()
+    # Products of three pieces add up 256 numbers in 8 steps of 32: 24 additions, each off by 2^-23 of a partial sum at most (half of all, on average),
+    # all the same way.  What they add up to is added exactly, rounded once to fp32 and joined in fp64.
+    off = float(((sums[:, 1] / T - want).abs() / want.abs()).max())
+    assert off <= (2 * 3 * 4.5 + 1) * 2.0 ** -24, off * 2 ** 24
+    new, _, _ = eng.cache_lbg_iterate(x, cb, sub)
+    assert float(((new[:, 1].double() - want).abs() / want.abs()).max()) <= (2 * 3 * 4.5 + 2) * 2.0 ** -24

@@ -43,6 +43,12 @@ constexpr float FAR_SCORE = 1e38f, FAR_NUMBER = 1e18f, BOUND_MOST = 1e30f, SIZE_
 // Rows past K lie at FAR_NUMBER: a vector within SIZE_MOST (1e17 long) and codewords within BOUND_MOST (1.5e15) are nearer to each other.
 constexpr float SUM_SCALE = 16777216.0f;       // lifts fp32's smallest numbers into bf16's normal range
 constexpr float COUNTED = 0x1p100f;            // training leaves out what is larger: times SUM_SCALE it would leave fp32
+// Training's sums.  Products add up FOLD vectors at a time in fp32, in FOLD / 32 steps for each piece, each off by half a step or a whole one; what
+// they give goes into LDS by an addition whose error is kept and goes on with the next products.  Equal numbers err the same way in every
+// step, so a sum is off by up to 27 * 2^-24 of its numbers' sizes (3 pieces * (FOLD / 32 + 1) / 2 steps, twice 2^-24 each); added
+// over the whole chunk in one go, 4096 fp32 copies of a number gave a mean up to 162 * 2^-24 off, now 6.  Costs 2 to 3% of an iteration, by
+// parts of 8 up to 6.
+constexpr int FOLD = 256;
 
 __device__ inline uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 
@@ -106,6 +112,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
     __shared__ __align__(16) float s_tab[SEARCH_WAVES][row_at<SUB>(NT * 32)];
     __shared__ __align__(16) uint16_t s_hi[TRAIN ? SEARCH_WAVES : 1][64], s_lo[TRAIN ? SEARCH_WAVES : 1][64];
     __shared__ __align__(16) uint16_t s_x[TRAIN ? SEARCH_WAVES : 1][XP][SUB][64];
+    __shared__ f32x4 s_sum[TRAIN ? SEARCH_WAVES : 1][SUB][64];            // a lane's own sums, see FOLD
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int which = blockIdx.z, parts = a.dim / SUB, per = parts / a.pw;
@@ -177,7 +184,17 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
     int counted = 0;
     if constexpr (TRAIN)
 #pragma unroll
-        for (int e = 0; e <= SUB; ++e) sum[e] = (f32x4){0, 0, 0, 0};
+        for (int e = 0; e <= SUB; ++e) {
+            sum[e] = (f32x4){0, 0, 0, 0};
+            if (e < SUB) s_sum[wave][e][lane] = sum[e];
+        }
+    // v into sum[e], exactly: the rounded sum to LDS, what is missing stays behind
+    auto put = [&](int e, f32x4 v) {
+        const f32x4 had = s_sum[wave][e][lane], now = had + v, added = now - had;
+        s_sum[wave][e][lane] = now;
+        __builtin_amdgcn_sched_barrier(0);                        // (one after the other: few registers)
+        return (had - (now - added)) + (v - added);
+    };
 
     auto fetch = [&](int64_t t) -> Numbers<T, SUB> {                      // past the end: the last token again
         t = t < end ? t : end - 1;
@@ -357,7 +374,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
                 }
                 const bf16x8 lo8 = __builtin_bit_cast(bf16x8, lows);
 #pragma unroll
-                for (int p = 0; p < XP; ++p)
+                for (int p = XP - 1; p >= 0; --p)                         // (the smallest pieces first)
 #pragma unroll
                     for (int e = 0; e < SUB; ++e) {
                         const u32x4 of = *reinterpret_cast<const u32x4 *>(&s_x[wave][p][e][first]) & member;
@@ -368,6 +385,9 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
+            if ((t0 - begin) % FOLD == FOLD - 64)
+#pragma unroll
+                for (int e = 0; e < SUB; ++e) sum[e] = put(e, sum[e] * (1.0f / SUM_SCALE)) * SUM_SCALE;
         }
     }
     if constexpr (TRAIN) {
@@ -375,7 +395,9 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
 #pragma unroll
         for (int e = 0; e <= SUB; ++e)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a.part_sums[(place * (SUB + 1) + e) * 256 + (4 * (lane >> 4) + i) * 16 + (lane & 15)] = sum[e][i];
+            for (int i = 0; i < 4; ++i)
+                a.part_sums[(place * (SUB + 1) + e) * 256 + (4 * (lane >> 4) + i) * 16 + (lane & 15)] =
+                    e < SUB ? s_sum[wave][e < SUB ? e : 0][lane][i] + sum[e][i] * (1.0f / SUM_SCALE) : sum[e][i];
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) away += __shfl_xor(away, o);
         if (lane == 0) a.part_dist[place] = make_double2(away, (double)counted);
@@ -434,7 +456,7 @@ __global__ __launch_bounds__(GATHER_THREADS) void k_lbg_gather(const float *__re
         out.counts[(int64_t)blockIdx.x * out.K + k] = (int64_t)n;
 #pragma unroll
         for (int e = 0; e < SUB; ++e) {
-            const double s = s_sum[e][tid] * (1.0 / (double)SUM_SCALE);
+            const double s = s_sum[e][tid];
             if (out.cb_new) out.cb_new[at + e] = n > 0.0 ? (float)(s / n) : out.cb_old[at + e];
             else out.sums[at + e] = s;
         }
