@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_cache import DEV, HALF, attention64, attention_case, check_attention, codes64, data, vectors64
+from test_gpu_cache import DEV, HALF, attention64, attention_case, check_attention, check_training, codes64, data, vectors64
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +143,20 @@ def test_training_mean_of_equal_vectors(eng, dtype, H, D, sub, value):
     assert off <= (2 * 3 * 4.5 + 1) * 2.0 ** -24, off * 2 ** 24
     new, _, _ = eng.cache_lbg_iterate(x, cb, sub)
     assert float(((new[:, 1].double() - want).abs() / want.abs()).max()) <= (2 * 3 * 4.5 + 2) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("sub", [2, 4, 8])
+def test_training_sums_of_the_largest_numbers(eng, dtype, sub):
+    """Numbers just below 2^100: hundreds of them in one cluster add up to more than 2^106."""
+    T, H, D, K = 1500, 1, 64, 7
+    x = data(7, (T, H, D), torch.float32)
+    x = x.sign() * (0.5 + 0.49 * x.abs().clamp(max=1.0))
+    big = torch.arange(T) % 3 == 0
+    x = torch.where(big[:, None, None], x * 2.0 ** 100, x).to(dtype)
+    cb = data(8, (H, K, D), torch.float32)
+    cb[:, 3], cb[:, 5] = 2.0 ** 99, -2.0 ** 99
+    sums, counts, dist = eng.cache_lbg_accum(x.to(DEV), cb.to(DEV), sub)
+    assert sums.isfinite().all() and float(sums.abs().max()) > 2.0 ** 104
+    new, mean = eng.cache_lbg_finish(sums, counts, dist, cb.to(DEV))
+    check_training(x, cb, sub, sums, counts, dist, new, mean)

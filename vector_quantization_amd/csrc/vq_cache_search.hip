@@ -42,7 +42,8 @@ constexpr int SEARCH_WAVES = 8;
 constexpr float FAR_SCORE = 1e38f, FAR_NUMBER = 1e18f, BOUND_MOST = 1e30f, SIZE_MOST = 1e34f;
 // Rows past K lie at FAR_NUMBER: a vector within SIZE_MOST (1e17 long) and codewords within BOUND_MOST (1.5e15) are nearer to each other.
 constexpr float SUM_SCALE = 16777216.0f;       // lifts fp32's smallest numbers into bf16's normal range
-constexpr float COUNTED = 0x1p100f;            // training leaves out what is larger: times SUM_SCALE it would leave fp32
+constexpr float COUNTED = 0x1p100f;            // training leaves out what is larger
+constexpr float NEAR = 0x1p126f;               // vectors shorter than 2^63 are added by products: FOLD of them, times SUM_SCALE, stay inside fp32
 // Training's sums.  Products add up FOLD vectors at a time in fp32, in FOLD / 32 steps for each piece, each off by half a step or a whole one; what
 // they give goes into LDS by an addition whose error is kept and goes on with the next products.  Equal numbers err the same way in every
 // step, so a sum is off by up to 27 * 2^-24 of its numbers' sizes (3 pieces * (FOLD / 32 + 1) / 2 steps, twice 2^-24 each); added
@@ -341,6 +342,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
             for (int e = 0; e < SUB; ++e) fine = fine && fabsf(x[e]) < COUNTED;
             // sums by products with the one-hot numbers of the codewords: number = 16 hi + lo, and
             // sum[hi][lo] = sum over vectors of (x where its hi is this row) * (1 where its lo is this column)
+            const bool near = size < NEAR;
             counted += __popcll(__ballot(fine));
             if (fine) {
                 double f = 0.0;
@@ -351,7 +353,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
                 }
                 away += f <= INFINITY ? f : INFINITY;
             }
-            s_hi[wave][lane] = fine ? (uint16_t)(code >> 4) : (uint16_t)0xffff;
+            s_hi[wave][lane] = fine && near ? (uint16_t)(code >> 4) : (uint16_t)0xffff;
             s_lo[wave][lane] = (uint16_t)(code & 15);
 #pragma unroll
             for (int e = 0; e < SUB; ++e) {
@@ -388,6 +390,17 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
             if ((t0 - begin) % FOLD == FOLD - 64)
 #pragma unroll
                 for (int e = 0; e < SUB; ++e) sum[e] = put(e, sum[e] * (1.0f / SUM_SCALE)) * SUM_SCALE;
+            // longer vectors one by one, by the lane that holds their codeword
+            for (uint64_t todo = __ballot(fine && !near); todo; todo &= todo - 1) {
+                const int v = __builtin_ctzll(todo), c = __builtin_amdgcn_readlane(code, v);
+                f32x4 one = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) one[i] = lane == (c >> 6 << 4 | (c & 15)) && (c >> 4 & 3) == i ? 1.0f : 0.0f;
+#pragma unroll
+                for (int e = 0; e < SUB; ++e)
+                    sum[e] += put(e, one * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x[e]), v))) * SUM_SCALE;
+                sum[SUB] += one;
+            }
         }
     }
     if constexpr (TRAIN) {
