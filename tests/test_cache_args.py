@@ -241,3 +241,25 @@ def test_training_log_and_stop_rule():
     assert short.iters_per_stage == [1, 1] and short.converged_iter == [-1, -1]
     flat = train_cache_codebooks(HostEngine(), torch.ones(9, 1, 16), 4, 4, log=None)      # no spread: nothing to part, nothing diverges
     assert torch.equal(flat.codebook, torch.ones(1, 4, 16)) and flat.distortions[-1] == 0.0
+
+
+def test_training_by_whole_iterations():
+    """An engine that runs an iteration in one call is trained by it, and by the halves where a group's results are added."""
+    class Whole(HostEngine):
+        calls = 0
+
+        def cache_lbg_iterate(self, x, cb, sub):
+            self.calls += 1
+            part = HostEngine.cache_lbg_accum(self, x, cb, sub)
+            new, mean = HostEngine.cache_lbg_finish(self, *part, cb)
+            return new, part[1], mean
+
+        def cache_lbg_accum(self, *_a):
+            raise AssertionError("the halves were called")
+
+    eng = Whole()
+    one, halves = (train_cache_codebooks(e, clouds(), 8, 4, log=None) for e in (eng, HostEngine()))
+    assert torch.equal(one.codebook, halves.codebook) and one.distortions == halves.distortions
+    assert eng.calls == 2 + sum(one.iters_per_stage)
+    with pytest.raises(ValueError, match="cannot exceed"):
+        train_cache_codebooks(eng, clouds()[:4], 8, 4, log=None)

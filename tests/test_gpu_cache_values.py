@@ -160,3 +160,21 @@ def test_training_sums_of_the_largest_numbers(eng, dtype, sub):
     assert sums.isfinite().all() and float(sums.abs().max()) > 2.0 ** 104
     new, mean = eng.cache_lbg_finish(sums, counts, dist, cb.to(DEV))
     check_training(x, cb, sub, sums, counts, dist, new, mean)
+
+
+class HalvesOnly:
+    """An engine of the two halves alone."""
+
+    def __init__(self, eng):
+        self.device, self.cache_lbg_accum, self.cache_lbg_finish = eng.device, eng.cache_lbg_accum, eng.cache_lbg_finish
+
+
+def test_whole_training_by_one_call_an_iteration(eng, monkeypatch):
+    """A process by itself trains by cache_lbg_iterate, bit for bit as by the two halves."""
+    from vector_quantization_amd import train_cache_codebooks
+    x = data(5, (3000, 3, 64), torch.bfloat16).to(DEV)
+    halves = train_cache_codebooks(HalvesOnly(eng), x, 32, 4, log=None, max_iterations=20)
+    monkeypatch.setattr(eng, "cache_lbg_accum", lambda *a: pytest.fail("the halves were called"), raising=False)
+    one = train_cache_codebooks(eng, x, 32, 4, log=None, max_iterations=20)
+    assert torch.equal(one.codebook, halves.codebook)
+    assert one.distortions == halves.distortions and one.iters_per_stage == halves.iters_per_stage

@@ -298,7 +298,8 @@ def train_cache_codebooks(engine, x, k, sub, epsilon=0.01, threshold=0.001, max_
     head and part side by side, in squared distance.
 
     x (tokens, heads, dim): sample vectors on the engine's device, of any of the three float types; this rank's share where
-    `group` names a process group.  A split replaces every codeword c by c + e and c - e, e being epsilon times the root
+    `group` names a process group, whose results are added between the two halves of an iteration; a process by itself runs
+    both in one (cache_lbg_iterate), with the same bits.  A split replaces every codeword c by c + e and c - e, e being epsilon times the root
     of its part's mean squared distance per number (the reference scales c, which cannot part codewords near
     zero).  A stage ends once the total distortion changes by less than `threshold` of itself.
     Returns an LBGResult whose codebook is (heads, K, dim) float32, K the next power of two from k; the cache takes it
@@ -312,7 +313,11 @@ def train_cache_codebooks(engine, x, k, sub, epsilon=0.01, threshold=0.001, max_
     if sub < 1 or dim % sub:
         raise ValueError(f"vectors of {dim} numbers cannot be cut into sub-vectors of {sub}")
 
+    whole = getattr(engine, "cache_lbg_iterate", None) if group is None else None     # (an engine may have the halves alone)
+
     def iterate(cb):
+        if whole is not None:
+            return whole(x, cb, sub)
         part = engine.cache_lbg_accum(x, cb, sub)
         if group is not None:
             part = _added_over_ranks(*part, group)
