@@ -263,3 +263,30 @@ def test_training_by_whole_iterations():
     assert eng.calls == 2 + sum(one.iters_per_stage)
     with pytest.raises(ValueError, match="cannot exceed"):
         train_cache_codebooks(eng, clouds()[:4], 8, 4, log=None)
+
+
+def test_tangents_are_refused(eng):
+    """Forward-mode derivatives would be lost without a word; tensors without one pass also where others may carry one."""
+    from torch.autograd import forward_ad
+    k_cb, v_cb, kc, vc = parts()
+    x, slots = torch.zeros((5, 2, 64), dtype=torch.bfloat16), torch.zeros(5, dtype=torch.int64)
+    table, lens, starts = torch.zeros((2, 3), dtype=torch.int32), torch.ones(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    f, cb = torch.zeros((9, 2, 64)), torch.zeros((2, 16, 64))
+    sums, counts, dist = eng.cache_lbg_accum(f[:0], cb, 4)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: eng.cache_write(dual(x), x, slots, k_cb, v_cb, kc, vc), lambda: eng.cache_write(x, dual(x), slots, k_cb, v_cb, kc, vc),
+                     lambda: eng.cache_write(x, x, slots, dual(k_cb), v_cb, kc, vc), lambda: eng.cache_read(slots, k_cb, dual(v_cb), kc, vc),
+                     lambda: eng.cache_attention(dual(x), k_cb, v_cb, kc, vc, table, lens, starts, 3),
+                     lambda: eng.cache_attention(x, k_cb, v_cb, kc, vc, table, lens, starts, 3, out=dual(x)),
+                     lambda: eng.cache_lbg_accum(dual(f), cb, 4), lambda: eng.cache_lbg_iterate(f, dual(cb), 4),
+                     lambda: eng.cache_lbg_finish(dual(sums), counts, dist, cb), lambda: eng.cache_lbg_finish(sums, counts, dual(dist), cb)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                call()
+        with pytest.raises(AssertionError, match="reached the launch"):
+            eng.cache_write(x, x, slots, k_cb, v_cb, kc, vc)
+        with torch.no_grad(), pytest.raises(AssertionError, match="reached the launch"):
+            eng.cache_write(x.clone().requires_grad_(), x, slots, k_cb, v_cb, kc, vc)

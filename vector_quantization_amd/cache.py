@@ -14,11 +14,12 @@ takes 32 bytes a head for its key and 32 for its value, an eighth of bfloat16.
 
 The methods launch on the engine's device and its current stream, allocate what they return (and their workspace)
 from torch's allocator and wait for nothing, so they may be captured into a graph.  None of them is differentiable:
-they refuse tensors that require a gradient.
+they refuse tensors that require a gradient or carry a tangent.
 """
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import lib, check, VQ_BF16, VQ_F16, VQ_F32
 
@@ -28,8 +29,13 @@ _DTYPES = {torch.float32: VQ_F32, torch.bfloat16: VQ_BF16, torch.float16: VQ_F16
 # ---- checks of arguments: shapes, types and devices only, nothing is read from the GPU.  They run on every call, so what
 # is right passes in one expression and only what is not is looked at again for its message. ------------------------------
 
+def _forward_mode():
+    """Whether tensors may carry tangents now: inside forward_ad.dual_level (which torch counts from -1, where it counts)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def _tensor(name, t, device, dtypes, dims):
-    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dims and t.device == device and not t.requires_grad:
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dims and t.device == device and not t.requires_grad and not _forward_mode():
         return t
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
@@ -39,8 +45,10 @@ def _tensor(name, t, device, dtypes, dims):
         raise ValueError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
     if t.dim() != dims:
         raise ValueError(f"{name} must have {dims} dimensions, got shape {tuple(t.shape)}")
-    if torch.is_grad_enabled():
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the cache operators are not differentiable")
+    if t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a tangent: the cache operators are not differentiable")
     return t
 
 
@@ -77,7 +85,7 @@ def cache_shape(k_cb, v_cb, k_codes, v_codes, device):
         dtype = k_cb.dtype
         right = (dtype in _HALVES and v_cb.dtype is dtype and k_codes.dtype is torch.uint8 and v_codes.dtype is torch.uint8 and
                  k_cb.device == device and v_cb.device == device and k_codes.device == device and v_codes.device == device and
-                 k_cb.dim() == 3 and k_codes.dim() == 4 and not (k_cb.requires_grad or v_cb.requires_grad) and
+                 k_cb.dim() == 3 and k_codes.dim() == 4 and not (k_cb.requires_grad or v_cb.requires_grad or _forward_mode()) and
                  k_codes.is_contiguous() and v_codes.is_contiguous() and not (k_codes.data_ptr() | v_codes.data_ptr()) % 16)
     except AttributeError:
         right = False
