@@ -103,6 +103,20 @@ def test_attention_tiny_scale(eng, scale):
     check_attention(out, lse, attention64(*case, 4, scale), 300)
 
 
+def test_attention_longest_context(eng):
+    """The longest length there is, 2^31 - 16 tokens, by a table that names one page again and again."""
+    D, sub, K, page, width = 32, 8, 16, 16, (1 << 27) - 1
+    q, k_cb, v_cb, kc, vc, table, kv_lens, starts = attention_case([1], [16], 1, 1, D, sub, K, page, torch.bfloat16, seed=99)
+    ref, ref_lse, size, slip = attention64(q, k_cb, v_cb, kc, vc, table, kv_lens, starts, sub, D ** -0.5)
+    long = torch.full((1, width), int(table[0, 0]), dtype=torch.int32, device=DEV)
+    lens = torch.tensor([2 ** 31 - 1], dtype=torch.int32, device=DEV)
+    out, lse = eng.cache_attention(*[t.to(DEV) for t in (q, k_cb, v_cb, kc, vc)], long, lens, starts.to(DEV), 1, want_lse=True)
+    # a lane adds 2^31 / (256 workgroups * 8 waves * 32) = 2^15 times; all those additions may err the same way
+    adds = 2.0 ** 15 * 1.1 * 2.0 ** -23
+    assert ((out.cpu().double() - ref).abs() <= 2.0 ** -8 * 1.01 * (ref.abs() + size) + (2 * slip + 2 * adds) * size).all()
+    assert ((lse.cpu().double() - ref_lse - math.log(width)).abs() <= slip[..., 0] + adds + 2.0 ** -21 * 30).all()
+
+
 # ---- search and training ------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("sub", [2, 4, 8])

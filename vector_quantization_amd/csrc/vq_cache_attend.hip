@@ -182,7 +182,7 @@ template <> struct Reference<_Float16> {
 template <int RB> __device__ inline int tiles_of(int tile, int n_q, int n_kv, int group) {
     const int n_rows = n_q * group, past = (tile + 1) * RB * 16;
     const int end = n_kv - n_q + ((past < n_rows ? past : n_rows) - 1) / group + 1;
-    return end < 0 ? 0 : (end + TILE - 1) / TILE;
+    return end <= 0 ? 0 : (end - 1) / TILE + 1;                      // (end may be near 2^31)
 }
 // What an item counts in the division of the work: its tiles, and one where it has none but zeros to be written.
 template <int RB> __device__ inline int cost_of(int tile, int n_q, int n_kv, int group) {
