@@ -290,3 +290,15 @@ def test_tangents_are_refused(eng):
             eng.cache_write(x, x, slots, k_cb, v_cb, kc, vc)
         with torch.no_grad(), pytest.raises(AssertionError, match="reached the launch"):
             eng.cache_write(x.clone().requires_grad_(), x, slots, k_cb, v_cb, kc, vc)
+
+
+@pytest.mark.parametrize("seqs,max_q,max_kv,dim,sub,K", [(1, 1, 1 << 16, 128, 4, 256), (16, 1, 20000, 64, 8, 200), (1, 2048, 16384, 256, 2, 256), (3, 40, 5000, 192, 4, 64)])
+def test_attention_workspace_is_asked_for_and_checked(seqs, max_q, max_kv, dim, sub, K):
+    """Where a head's work is cut there has to be a workspace, of the size that is named and in its place."""
+    kw = dict(rows=seqs * max_q, seqs=seqs, max_q=max_q, max_kv=max_kv, dim=dim, sub=sub, K=K, qt=32 * dim, qh=dim)
+    need = _lib.lib.vq_cache_attention_ws_bytes(seqs * max_q, 32, 8, dim, sub, K, seqs, max_q, max_kv)
+    assert need > 0
+    assert attend(**kw, ws_bytes=need - 1) == _lib.VQ_E_WORKSPACE and str(need) in _lib.last_error()
+    assert attend(**kw, ws=None) == _lib.VQ_E_WORKSPACE
+    assert attend(**kw, ws=ctypes.c_void_p(4100), ws_bytes=need) == _lib.VQ_E_INVALID and "16 bytes" in _lib.last_error()
+    assert _lib.lib.vq_cache_attention_ws_bytes(1, 32, 8, dim, sub, K, 1, 1, 64) == 0      # a short sequence is not cut

@@ -103,6 +103,51 @@ def test_attention_tiny_scale(eng, scale):
     check_attention(out, lse, attention64(*case, 4, scale), 300)
 
 
+WIDE = [
+    # new tokens, lengths, q_heads, heads, dim, sub, K, page, dtype: single tokens, sixteen rows a head at most; 192 and 256 dims
+    ([1, 1], [700, 90], 4, 2, 192, 2, 40, 64, torch.float16), ([1, 1], [2500, 90], 4, 2, 192, 4, 128, 16, torch.bfloat16),
+    ([1, 1], [333, 1], 8, 2, 192, 8, 100, 16, torch.bfloat16), ([1, 2], [1700, 64], 8, 1, 192, 8, 128, 48, torch.float16),
+    ([1, 1], [700, 90], 4, 2, 192, 2, 256, 64, torch.bfloat16), ([1, 1], [2500, 90], 4, 2, 192, 4, 256, 16, torch.float16),
+    ([1, 1], [333, 1], 8, 2, 192, 8, 255, 16, torch.float16), ([1, 1], [3000, 3000], 8, 2, 192, 8, 129, 32, torch.bfloat16),
+    ([1, 1], [700, 90], 4, 2, 256, 2, 40, 64, torch.float16), ([1, 1], [2500, 90], 4, 2, 256, 4, 128, 16, torch.bfloat16),
+    ([1, 1], [333, 1], 8, 2, 256, 8, 100, 16, torch.bfloat16), ([1, 2], [1700, 64], 8, 1, 256, 8, 128, 48, torch.float16),
+    ([1, 1], [700, 90], 4, 2, 256, 2, 256, 64, torch.bfloat16), ([1, 1], [2500, 90], 4, 2, 256, 4, 256, 16, torch.float16),
+    ([1, 1], [333, 1], 8, 2, 256, 8, 255, 16, torch.float16), ([1, 1], [3000, 3000], 8, 2, 256, 8, 129, 32, torch.bfloat16),
+    ([1, 1], [700, 90], 4, 2, 192, 2, 64, 64, torch.bfloat16), ([1, 1], [1700, 90], 4, 2, 192, 2, 200, 64, torch.float16),
+    ([1, 1], [700, 90], 4, 2, 192, 4, 64, 64, torch.float16), ([1, 1], [1700, 90], 4, 2, 192, 4, 200, 64, torch.bfloat16),
+    ([1, 1], [700, 90], 4, 2, 256, 2, 64, 64, torch.bfloat16), ([1, 1], [1700, 90], 4, 2, 256, 2, 200, 64, torch.float16),
+    ([1, 1], [700, 90], 4, 2, 256, 4, 64, 64, torch.float16), ([1, 1], [1700, 90], 4, 2, 256, 4, 200, 64, torch.bfloat16),
+    # many rows: what is looked up in the caches and what is not, by the pairs of dims and parts that no other test has
+    ([40, 3], [300, 64], 4, 2, 192, 8, 256, 16, torch.bfloat16), ([40, 3], [300, 64], 4, 2, 192, 8, 16, 16, torch.float16),
+    ([40, 3], [300, 64], 4, 2, 256, 2, 256, 16, torch.float16), ([40, 3], [300, 64], 4, 2, 256, 2, 33, 16, torch.bfloat16),
+    ([1, 40], [300, 64], 4, 2, 32, 4, 256, 16, torch.bfloat16), ([1, 1], [300, 2000], 4, 2, 32, 4, 100, 16, torch.float16),
+    ([1, 40], [300, 64], 4, 2, 96, 2, 256, 16, torch.float16), ([1, 1], [300, 2000], 4, 2, 96, 2, 100, 16, torch.bfloat16),
+]
+
+
+@pytest.mark.parametrize("hint", [None, 1])
+@pytest.mark.parametrize("n_q,n_kv,Hq,H,D,sub,K,page,dtype", WIDE)
+def test_attention_wide(eng, n_q, n_kv, Hq, H, D, sub, K, page, dtype, hint):
+    """(hint: with what the table holds the longer sequences are cut between workgroups; with one token none is.)"""
+    case = attention_case(n_q, n_kv, Hq, H, D, sub, K, page, dtype, seed=D + sub)
+    out, lse = eng.cache_attention(*[t.to(DEV) for t in case], max(n_q), max_kv=hint, want_lse=True)
+    check_attention(out, lse, attention64(*case, sub, 1.0 / math.sqrt(D)), max(n_kv))
+
+
+@pytest.mark.parametrize("n_q,n_kv,Hq,H,D,sub,K,dtype", [
+    ([1], [501], 32, 8, 128, 4, 256, torch.bfloat16), ([1] * 16, [2000 + 700 * i for i in range(16)], 32, 8, 128, 4, 256, torch.bfloat16),
+    ([61, 1, 30, 2, 7], [3001, 900, 1400, 0, 2000], 6, 2, 64, 8, 200, torch.float16), ([600], [4000], 32, 8, 128, 4, 256, torch.bfloat16)])
+def test_attention_repeats_itself(eng, n_q, n_kv, Hq, H, D, sub, K, dtype):
+    """The same call gives the same bits, other calls between."""
+    case = [t.to(DEV) for t in attention_case(n_q, n_kv, Hq, H, D, sub, K, 16, dtype, seed=97)]
+    first = eng.cache_attention(*case, max(n_q), want_lse=True)
+    for i in range(4):
+        other = torch.empty(1 << (16 + 2 * i), device=DEV).fill_(math.nan)          # what the allocator hands out next holds something else
+        del other
+        again = eng.cache_attention(*case, max(n_q), want_lse=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
 def test_attention_longest_context(eng):
     """The longest length there is, 2^31 - 16 tokens, by a table that names one page again and again."""
     D, sub, K, page, width = 32, 8, 16, 16, (1 << 27) - 1
@@ -174,6 +219,35 @@ def test_training_sums_of_the_largest_numbers(eng, dtype, sub):
     assert sums.isfinite().all() and float(sums.abs().max()) > 2.0 ** 104
     new, mean = eng.cache_lbg_finish(sums, counts, dist, cb.to(DEV))
     check_training(x, cb, sub, sums, counts, dist, new, mean)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_training_beside_what_is_not_finite(eng, dtype):
+    """Vectors and codewords that are not finite, everything that an iteration gives: they are left out, or stay as they were."""
+    T, H, D, sub, K = 200, 1, 64, 4, 64
+    x, cb = data(7, (T, H, D), dtype), data(8, (H, K, D), torch.float32)
+    x[3, 0, 5], x[4, 0, 7], x[5, 0, 0] = math.nan, math.inf, -math.inf
+    cb[:, 9], cb[:, 3, 2] = math.inf, math.nan
+    code, least = codes64(x, cb, sub)
+    fine = x.double().reshape(T, H, D // sub, sub).isfinite().all(-1)
+    sums, counts, dist = (t.cpu() for t in eng.cache_lbg_accum(x.to(DEV), cb.to(DEV), sub))
+    new, mean = (t.cpu() for t in eng.cache_lbg_finish(sums.to(DEV), counts.to(DEV), dist.to(DEV), cb.to(DEV)))
+    new2, counts2, mean2 = (t.cpu() for t in eng.cache_lbg_iterate(x.to(DEV), cb.to(DEV), sub))
+    assert torch.equal(counts, counts2) and torch.equal(mean, mean2) and torch.equal(new.nan_to_num(7.0), new2.nan_to_num(7.0))
+    for m in range(D // sub):
+        ok, part = fine[:, 0, m], slice(m * sub, (m + 1) * sub)
+        xs, c = x[ok, 0, part].double(), torch.from_numpy(code[:, 0, m])[ok]
+        n = torch.bincount(c, minlength=K)
+        assert torch.equal(counts[0, m], n)
+        want, size = (torch.zeros((K, sub), dtype=torch.float64).index_add_(0, c, t) for t in (xs, xs.abs()))
+        tol = 32 * 2.0 ** -23 * size
+        assert ((sums[0, :, part] - want).abs() <= tol).all()
+        far = torch.from_numpy(least[:, 0, m])[ok].sum()
+        assert abs(float(dist[0, m] - far)) <= 1e-12 * float(far) and abs(float(mean[0, m] - far / int(ok.sum()))) <= 2e-12 * float(far) / int(ok.sum())
+        has = n > 0
+        centre = want[has] / n[has, None]
+        assert ((new[0, has, part].double() - centre).abs() <= tol[has] / n[has, None] + 2.0 ** -24 * 1.001 * centre.abs()).all()
+        assert torch.equal(new[0, ~has, part].nan_to_num(7.0), cb[0, ~has, part].nan_to_num(7.0))
 
 
 class HalvesOnly:
