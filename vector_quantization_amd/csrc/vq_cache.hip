@@ -277,13 +277,13 @@ Attention plan_attention(int q_heads, int heads, int dim, int sub, int K, int se
     const int Kp = dim <= 128 ? 256 : rows_padded(K), group = q_heads / heads;      // (as k_cache_attend lays out its tables)
     const int64_t per_seq = at_most(max_q, 0x3fffffff) * group;
     // Behind the tables lie the waves' maxima and sums, 16 rows of at least one wave, and the workgroup's range.  More than 16 rows a sequence
-    // go 32 at a time, so that a look-up serves twice the products, unless the value table then no longer fits but would beside 16.
+    // go 32 at a time, so that a look-up serves twice the products; the value table fits beside them wherever it does beside 16.
     // (16 sequences of 20000 tokens, 4 rows: 53 us by 16 rows, 62 by 32; of 4000 tokens, 32 rows: 34 and 31; a chunk of 8192 rows on 16384
     // tokens: 1081 and 673.)
     const size_t keys = key_bytes(Kp, dim, sub), values = (size_t)Kp * dim * 2, row = (size_t)(dim + 4) * 4;
     auto waves = [&](int rb) { return rb == 2 && dim >= 192 ? 4 : 8; };
     auto fits = [&](int rb, size_t tables) { return tables + (size_t)waves(rb) * rb * 16 * 8 + 16 * row + SEQ_BYTES <= LDS_MOST; };
-    r.p.rb = per_seq <= 16 ? 1 : fits(2, keys + values) || !fits(1, keys + values) ? 2 : 1;
+    r.p.rb = per_seq <= 16 ? 1 : 2;
     r.p.nw = waves(r.p.rb);
     r.p.values_in_lds = fits(r.p.rb, keys + values);
     const int rows = r.p.rb * 16;
