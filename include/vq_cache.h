@@ -59,11 +59,13 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
  * grouped: head h reads cache head h / (q_heads / heads).  rows * q_heads / heads is below 2^30, width * page below 2^31,
  * q_heads at most 4096, seqs at most 65535.  out and lse overlap no other tensor of the call.
  *   out (rows, q_heads, dim) = softmax(scale * q k^T) v      lse (rows, q_heads, nullable) = log sum exp(scale * q k^T)
- * A row that sees no token, or whose scores are all minus infinity, gets zeros and minus infinity; rows of no sequence
- * are left as they were.  Lengths past the table's width are cut to it; the tokens of a page number outside [0, pages)
+ * A row that sees no token, or whose scores are all minus infinity, gets zeros and minus infinity; one with a score that is NaN or plus
+ * infinity (in fp32) gets NaN; rows of no sequence are left as they were.  Lengths past the table's width are cut to it; the tokens of a page number outside [0, pages)
  * are not seen.  Codewords have to be finite; a code of K or more stands for some codeword or for zeros.  max_q and
  * max_kv, the longest of the sequences' rows and lengths as the caller knows them, only shape the launch: any value of
  * 1 or more gives the same sums, up to the order of addition.
+ * Scores, weights and sums are fp32; weights are rounded to `dtype` before they meet the values, their sum takes them unrounded.  Of fp16 a
+ * weight is off by half a step, or by 2^-19 of the largest that its row has among the 32 tokens it is taken with.
  * `starts` rises, from 0 or more to `rows` or less.  dtype: VQ_BF16 or VQ_F16. */
 size_t vq_cache_attention_ws_bytes(int64_t rows, int q_heads, int heads, int dim, int sub, int K, int seqs,
                                    int64_t max_q, int64_t max_kv);

@@ -94,6 +94,28 @@ def test_attention_scores_whose_steps_are_large(eng, dtype, size, n_q, n_kv):
     assert torch.equal(out[sure], ref[sure])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n_q,n_kv", [([1, 1], [40, 700]), ([30, 3], [300, 60])])
+def test_attention_infinite_scores(eng, dtype, n_q, n_kv):
+    """A row with scores of plus infinity is none, with scores of minus infinity alone sees nothing;
+    the rows beside it stay as they are."""
+    case = list(attention_case(n_q, n_kv, 4, 2, 64, 4, 256, 16, dtype, seed=87))
+    q, k_cb = case[:2]
+    k_cb[:, :, 5] = k_cb[:, :, 5].abs() + 0.5
+    clean = [t.cpu() for t in eng.cache_attention(*[t.to(DEV) for t in case], max(n_q), want_lse=True)]
+    q[1, 0, 5], q[1, 3, 5] = math.inf, -math.inf
+    out, lse = (t.cpu() for t in eng.cache_attention(*[t.to(DEV) for t in case], max(n_q), want_lse=True))
+    assert out[1, 0].isnan().all() and lse[1, 0].isnan()
+    assert not out[1, 3].any() and lse[1, 3] == -math.inf
+    rest = torch.ones(out.shape[:2], dtype=torch.bool)
+    rest[1, 0] = rest[1, 3] = False
+    half = HALF[dtype]
+    assert out[rest].isfinite().all() and lse[rest].isfinite().all()
+    # the same sums, against references that may have moved at other tiles
+    assert ((out.double() - clean[0].double())[rest].abs() <= 4 * half * case[2].abs().max().double()).all()
+    assert ((lse.double() - clean[1].double())[rest].abs() <= 2.0 ** -18 * (1 + clean[1].double().abs())[rest]).all()
+
+
 @pytest.mark.parametrize("scale", [3e-38, -2e-39, 1e-44])
 def test_attention_tiny_scale(eng, scale):
     """A scale near or below fp32's smallest normal number is taken as it is."""
