@@ -42,6 +42,15 @@ PEAK_SAD_TOPS = 256 * 4 * 64 * 2.4e9 / 4 * 4 / 1e12
 PEAK_HBM_GBS = 8000.0
 
 
+def image_sources_sha256():
+    """Hash of what the image path's kernels are built from: their source, its header and the build's flags."""
+    h = hashlib.sha256()
+    for name in ("vector_quantization_amd/csrc/vq_hip.hip", "include/vq_hip.h", "vector_quantization_amd/csrc/build.sh"):
+        with open(os.path.join(ROOT, name), "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()
+
+
 # ---------------------------------------------------------------------------------------------------
 # CPU baseline (runs in a child process that never touches the GPU)
 # ---------------------------------------------------------------------------------------------------
@@ -390,21 +399,23 @@ def main():
     dec_ms = event_ms(lambda: eng.decode(labels.view(nr, nc), cb, BH, BW, 1), reps, device)
     enc_ms = event_ms(lambda: eng.encode_image(img, BH, BW, cb, scratch=scratch, labels=labels), reps, device)
 
-    # HBM bytes per launch from separate rocprofv3 --pmc passes of this library build, when a summary made
-    # from the same libvqhip.so is committed under profiles/ (FETCH_SIZE doubled per the gfx950 correction)
+    # HBM bytes per launch from separate rocprofv3 --pmc passes, when a summary made from the same sources of the image path is
+    # committed under profiles/ (FETCH_SIZE doubled per the gfx950 correction).  By sources, not by the library, which holds
+    # the cache operators too; a library given by $VQ_HIP_LIB may be of any.
     traffic, pmc_note = None, "no PMC summary for this library build under profiles/"
     lib_sha = hashlib.sha256(open(_lib.library_path(), "rb").read()).hexdigest()[:16]
-    pmc_path = os.path.join(ROOT, "profiles", "r03_pmc_summary.json")
+    src_sha = image_sources_sha256()[:16]
+    pmc_path = os.path.join(ROOT, "profiles", "image_pmc_summary.json")
     pmc = None
     if os.path.isfile(pmc_path):
         with open(pmc_path) as f:
             pmc = json.load(f)
-        if pmc.get("library_sha256_16") != lib_sha:
-            pmc_note = (f"profiles/r03_pmc_summary.json was made from library {pmc.get('library_sha256_16')}, this run "
-                        f"uses {lib_sha}: not reported")
+        if pmc.get("image_sources_sha256_16") != src_sha or "VQ_HIP_LIB" in os.environ:
+            pmc_note = (f"profiles/image_pmc_summary.json was made from sources {pmc.get('image_sources_sha256_16')}, this tree "
+                        f"has {src_sha}, or the library is another tree's: not reported")
             pmc = None
         else:
-            pmc_note = "HBM traffic per launch from profiles/r03_pmc_*.csv (rocprofv3 --pmc passes of this library build)"
+            pmc_note = "HBM traffic per launch from profiles/image_pmc_*.csv (rocprofv3 --pmc passes of these sources' library)"
 
     def pmc_bytes(role):
         r = (pmc or {}).get("roles", {}).get(role)

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Copies the rocprofv3 outputs of tools/gpu_round.sh from gpurun_out/ into profiles/ (filtered to this
 library's kernels) and derives the per-kernel PMC table and the summary bench.py reads.
-Usage: python3 tools/make_profiles.py r03"""
+Usage: python3 tools/make_profiles.py image"""
 import collections
 import csv
 import glob
@@ -12,7 +12,7 @@ import shutil
 import statistics
 import sys
 
-tag = sys.argv[1] if len(sys.argv) > 1 else "r03"
+tag = sys.argv[1] if len(sys.argv) > 1 else "image"
 root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 out = os.path.join(root, "profiles")
 src = os.path.join(root, "gpurun_out")
@@ -26,6 +26,9 @@ def short(name):
 def is_ours(name):
     return short(name).startswith("k_")
 
+
+sys.path.insert(0, root)
+from bench import image_sources_sha256  # noqa: E402
 
 lib_sha = hashlib.sha256(open(os.path.join(root, "vector_quantization_amd", "lib", "libvqhip.so"), "rb").read()).hexdigest()[:16]
 
@@ -111,6 +114,7 @@ roles = dict(
 summary = dict(
     roles=roles,
     library_sha256_16=lib_sha,
+    image_sources_sha256_16=image_sources_sha256()[:16],
     workload="tools/prof_encode.py: 8192x8192 gray, 4x4 blocks, K=256 (N = 4194304 block vectors)",
     hbm_bytes_by_kernel={e["kernel"]: e["hbm_read_bytes"] + e["hbm_write_bytes"] for e in big
                          if full_size(e["kernel"])},
