@@ -17,6 +17,7 @@ from torch's allocator and wait for nothing, so they may be captured into a grap
 they refuse tensors that require a gradient or carry a tangent.
 """
 import math
+from types import SimpleNamespace
 
 import torch
 from torch.autograd import forward_ad
@@ -26,16 +27,16 @@ from ._lib import lib, check, VQ_BF16, VQ_F16, VQ_F32
 _DTYPES = {torch.float32: VQ_F32, torch.bfloat16: VQ_BF16, torch.float16: VQ_F16}
 
 
+# where torch counts its levels of forward-mode derivatives: -1 outside of them all, where no tensor carries a tangent
+_levels = forward_ad if hasattr(forward_ad, "_current_level") else SimpleNamespace(_current_level=0)
+
+
 # ---- checks of arguments: shapes, types and devices only, nothing is read from the GPU.  They run on every call, so what
 # is right passes in one expression and only what is not is looked at again for its message. ------------------------------
 
-def _forward_mode():
-    """Whether tensors may carry tangents now: inside forward_ad.dual_level (which torch counts from -1, where it counts)."""
-    return getattr(forward_ad, "_current_level", 0) >= 0
-
-
 def _tensor(name, t, device, dtypes, dims):
-    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dims and t.device == device and not t.requires_grad and not _forward_mode():
+    if (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dims and t.device == device and not t.requires_grad and
+            _levels._current_level < 0):
         return t
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
@@ -85,7 +86,7 @@ def cache_shape(k_cb, v_cb, k_codes, v_codes, device):
         dtype = k_cb.dtype
         right = (dtype in _HALVES and v_cb.dtype is dtype and k_codes.dtype is torch.uint8 and v_codes.dtype is torch.uint8 and
                  k_cb.device == device and v_cb.device == device and k_codes.device == device and v_codes.device == device and
-                 k_cb.dim() == 3 and k_codes.dim() == 4 and not (k_cb.requires_grad or v_cb.requires_grad or _forward_mode()) and
+                 k_cb.dim() == 3 and k_codes.dim() == 4 and not (k_cb.requires_grad or v_cb.requires_grad or _levels._current_level >= 0) and
                  k_codes.is_contiguous() and v_codes.is_contiguous() and not (k_codes.data_ptr() | v_codes.data_ptr()) % 16)
     except AttributeError:
         right = False
