@@ -80,8 +80,8 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
  * part and codeword, the sum and number of the vectors nearest to it (as in vq_cache_write), and for each head and part
  * the sum of the least squared distances.  A vector of which a number is 2^100 or more
  * in size, or no number, is left out of all three.  sums (heads, K, dim) fp64, counts (heads, parts, K) int64, dist
- * (heads, parts) fp64 are overwritten; the result does not depend on timing.  A sum is off by 2^-19 of its numbers' sizes added up at
- * most (products in fp32, 256 vectors at a time, are added up exactly and rounded to fp32 once a chunk).  cb is (heads, K, dim) fp32; x is of any
+ * (heads, parts) fp64 are overwritten; the result does not depend on timing.  A sum is off by 2^-18 of its numbers' sizes added up at
+ * most (products in fp32, 256 to 1024 vectors at a time, are added up exactly and rounded to fp32 once a chunk).  cb is (heads, K, dim) fp32; x is of any
  * of the three types.  A call takes 65535 chunks of 4096 tokens (268 million).  Adding several calls' sums, counts and dist gives
  * those of their tokens together. */
 size_t vq_cache_lbg_ws_bytes(int64_t tokens, int heads, int dim, int sub, int K);

@@ -43,13 +43,13 @@ constexpr float FAR_SCORE = 1e38f, FAR_NUMBER = 1e18f, BOUND_MOST = 1e30f, SIZE_
 // Rows past K lie at FAR_NUMBER: a vector within SIZE_MOST (1e17 long) and codewords within BOUND_MOST (1.5e15) are nearer to each other.
 constexpr float SUM_SCALE = 16777216.0f;       // lifts fp32's smallest numbers into bf16's normal range
 constexpr float COUNTED = 0x1p100f;            // training leaves out what is larger
-constexpr float NEAR = 0x1p126f;               // vectors shorter than 2^63 are added by products: FOLD of them, times SUM_SCALE, stay inside fp32
-// Training's sums.  Products add up FOLD vectors at a time in fp32, in FOLD / 32 steps for each piece, each off by half a step or a whole one; what
-// they give goes into LDS by an addition whose error is kept and goes on with the next products.  Equal numbers err the same way in every
-// step, so a sum is off by up to 27 * 2^-24 of its numbers' sizes (3 pieces * (FOLD / 32 + 1) / 2 steps, twice 2^-24 each); added
-// over the whole chunk in one go, 4096 fp32 copies of a number gave a mean up to 162 * 2^-24 off, now 6.  Costs 2 to 3% of an iteration, by
-// parts of 8 up to 6.
-constexpr int FOLD = 256;
+constexpr float NEAR = 0x1p126f;               // vectors shorter than 2^63 are added by products: 1024 of them, times SUM_SCALE, stay inside fp32
+// Training's sums.  Products add up so many vectors at a time in fp32, in a step of 32 vectors for each piece of their numbers, each off by half a
+// step or a whole one; what they give goes into LDS by an addition whose error is kept and goes on with the next products.  Equal numbers err
+// the same way in every step, so a sum is off by up to 34 * 2^-24 of its numbers' sizes (pieces * (vectors / 32 + 1) / 2 steps, twice
+// 2^-24 each, and 2^-24 where it is stored); added over the whole chunk in one go, 4096 fp32 copies of a number gave a mean up to 162 * 2^-24 off,
+// now 6.  Costs 1 to 3% of an iteration.
+constexpr int fold_after(int pieces) { return pieces == 1 ? 1024 : pieces == 2 ? 512 : 256; }
 
 __device__ inline uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
     __shared__ __align__(16) float s_tab[SEARCH_WAVES][row_at<SUB>(NT * 32)];
     __shared__ __align__(16) uint16_t s_hi[TRAIN ? SEARCH_WAVES : 1][64], s_lo[TRAIN ? SEARCH_WAVES : 1][64];
     __shared__ __align__(16) uint16_t s_x[TRAIN ? SEARCH_WAVES : 1][XP][SUB][64];
-    __shared__ f32x4 s_sum[TRAIN ? SEARCH_WAVES : 1][SUB][64];            // a lane's own sums, see FOLD
+    __shared__ f32x4 s_sum[TRAIN ? SEARCH_WAVES : 1][SUB][64];            // a lane's own sums: see fold_after
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int which = blockIdx.z, parts = a.dim / SUB, per = parts / a.pw;
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            if ((t0 - begin) % FOLD == FOLD - 64)
+            if ((t0 - begin) % fold_after(XP) == fold_after(XP) - 64)
 #pragma unroll
                 for (int e = 0; e < SUB; ++e) sum[e] = put(e, sum[e] * (1.0f / SUM_SCALE)) * SUM_SCALE;
             // longer vectors one by one, by the lane that holds their codeword
