@@ -60,8 +60,8 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
  * q_heads at most 4096, seqs at most 65535.  out and lse overlap no other tensor of the call.
  *   out (rows, q_heads, dim) = softmax(scale * q k^T) v      lse (rows, q_heads, nullable) = log sum exp(scale * q k^T)
  * A row that sees no token, or whose scores are all minus infinity, gets zeros and minus infinity; one with a score that is NaN or plus
- * infinity (in fp32) gets NaN; rows of no sequence are left as they were.  Lengths past the table's width are cut to it; the tokens of a page number outside [0, pages)
- * are not seen.  Codewords have to be finite; a code of K or more stands for some codeword or for zeros.  max_q and
+ * infinity (in fp32) gets NaN; rows of no sequence are left as they were.  Lengths past the table's width are cut to it; the tokens of a
+ * page number outside [0, pages) are not seen.  Codewords have to be finite; a code of K or more stands for some codeword or for zeros.  max_q and
  * max_kv, the longest of the sequences' rows and lengths as the caller knows them, only shape the launch: any value of
  * 1 or more gives the same sums, up to the order of addition.
  * Scores, weights and sums are fp32; weights are rounded to `dtype` before they meet the values, their sum takes them unrounded.  Of fp16 a
@@ -80,9 +80,9 @@ int vq_cache_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
  * part and codeword, the sum and number of the vectors nearest to it (as in vq_cache_write), and for each head and part
  * the sum of the least squared distances.  A vector of which a number is 2^100 or more
  * in size, or no number, is left out of all three.  sums (heads, K, dim) fp64, counts (heads, parts, K) int64, dist
- * (heads, parts) fp64 are overwritten; the result does not depend on timing.  A sum is off by 2^-18 of its numbers' sizes added up at
- * most (products in fp32, 256 to 1024 vectors at a time, are added up exactly and rounded to fp32 once a chunk).  cb is (heads, K, dim) fp32; x is of any
- * of the three types.  A call takes 65535 chunks of 4096 tokens (268 million).  Adding several calls' sums, counts and dist gives
+ * (heads, parts) fp64 are overwritten; the result does not depend on timing.  A sum is off by 2^-17 of its numbers' sizes added up at
+ * most (products in fp32, 256 to 1024 vectors at a time, are added up exactly and rounded to fp32 once a chunk).  cb is (heads, K, dim)
+ * fp32; x is of any of the three types.  A call takes 65535 chunks of 4096 tokens (268 million).  Adding several calls' sums, counts and dist gives
  * those of their tokens together. */
 size_t vq_cache_lbg_ws_bytes(int64_t tokens, int heads, int dim, int sub, int K);
 int vq_cache_lbg_accum(const void *x, int64_t token_stride, int64_t head_stride, int64_t tokens,

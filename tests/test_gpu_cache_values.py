@@ -116,6 +116,28 @@ def test_attention_infinite_scores(eng, dtype, n_q, n_kv):
     assert ((lse.double() - clean[1].double())[rest].abs() <= 2.0 ** -18 * (1 + clean[1].double().abs())[rest]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,rows", [(64, 1), (128, 40), (192, 1), (256, 20)])
+def test_attention_of_one_token_is_its_value(eng, dtype, D, rows):
+    """A row that sees one token, or one 80 nats above the others, gives that token's value as it is, whatever the score."""
+    sub, K = 4, 64
+    case = list(attention_case([1, rows], [1, rows], 4, 2, D, sub, K, 16, dtype, seed=88))
+    q, k_cb, v_cb, kc, vc, table, kv_lens, starts = case
+    ref = attention64(*case, sub, 0.37)[0]
+    out = eng.cache_attention(*[t.to(DEV) for t in case], rows, scale=0.37).cpu().double()
+    assert torch.equal(out[:2], ref[:2])                                 # each sequence's first row
+    k_cb[:, 0], q[:] = 2.0, 1.0 + torch.rand(q.shape, generator=torch.Generator().manual_seed(89)).to(dtype)
+    k_cb[:, 1:] = -k_cb[:, 1:].abs()
+    kc.clamp_(min=1)
+    page, at = int(table[1, 0]), 0
+    kc[page, :, at] = 0                                                  # every row of the second sequence sees its first token
+    ref, _, size, _ = attention64(*case, sub, 1.0)
+    out = eng.cache_attention(*[t.to(DEV) for t in case], rows, scale=1.0).cpu().double()
+    value = torch.stack([vectors64(vc[page, g // 2, :, at][None], v_cb[g // 2], sub)[0] for g in range(4)])
+    assert (ref[1:] - value).abs().max() < 1e-20
+    assert torch.equal(out[1:], value.expand(rows, 4, D))
+
+
 @pytest.mark.parametrize("scale", [3e-38, -2e-39, 1e-44])
 def test_attention_tiny_scale(eng, scale):
     """A scale near or below fp32's smallest normal number is taken as it is."""

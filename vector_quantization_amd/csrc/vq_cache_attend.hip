@@ -160,14 +160,14 @@ __device__ inline void store_row(const AttendArgs &a, int64_t place, int D, int 
 // 2^9, and its weight was infinite or nothing.)
 constexpr float LARGE = 0x1p20f;
 
-// How a row's reference follows its scores.  It is moved where a tile's largest weight leaves 2^LEAST .. 2^MOST, to where that is 2^AIM or a
-// little more; for bf16, whose weights have fp32's range, to the maximum itself and never down.  In fp16 a weight below 2^-14 loses bits and one
-// below 2^-25 is nothing, and a reference that only rose would do that to all tokens of a wave behind one heavy token: with a heavy token whose
-// value is zero and 20000 others 17 to 26 nats below it, an eighth of the result was lost.  With one that comes down again a weight is
-// off by half a step, or by 2^-19 of the largest in its own tile (2^-33 where that has just moved the reference).  References of
-// fp16 are whole numbers, so moving is exact, and come down only as far as the row's sum stays below 2^92 (the products' sums, up
-// to 2^16 times that, then stay inside fp32).  Scores of a few nats move it no oftener than before (512 rows on 8192 tokens, 128 dims by 4: 129 us);
-// with a deviation of 4 nats it takes 136 us where 126 were, of 8 nats 145.
+// How a row's reference follows its scores.  It is moved where a tile's largest weight leaves 2^LEAST .. 2^MOST, to where that is 2^AIM; for bf16,
+// whose weights have fp32's range, to the maximum itself and never down.  In fp16 a weight below 2^-14 loses bits and one below 2^-25 is
+// nothing, and a reference that only rose would do that to all tokens of a wave behind one heavy token: with a heavy token whose value is zero
+// and 20000 others 17 to 26 nats below it, an eighth of the result was lost.  With one that comes down again a weight is off by half a
+// step, or by 2^-19 of the largest in its own tile (2^-33 where that has just moved the reference).  The reference lies a whole number below
+// the score that moved it, so that this one's weight is exact, as that of a row's only token.  It comes down only as far as
+// the row's sum stays below 2^93 (the products' sums, up to 2^16 times that, then stay inside fp32).  Scores of a few nats move it no oftener
+// than before (512 rows on 8192 tokens, 128 dims by 4: 128 us); with a deviation of 4 nats it takes 140 us where 125 were, of 8 nats 151.
 template <typename T> struct Reference {
     static constexpr bool BOTH_WAYS = false;
     static constexpr float MOST = 8.0f;
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(NW * 64) void k_cache_attend(const AttendArgs a) {
                     float now = fmaxf(top[rb], most);
                     if constexpr (Ref::BOTH_WAYS) {               // (most tiles that come here have a lane's 8 tokens below the row's 32, no more)
                         const bool falls = most - top[rb] < Ref::LEAST && most > -INFINITY;
-                        const float aim = fabsf(most) < LARGE ? floorf(most) - Ref::AIM : most;
+                        const float aim = fabsf(most) < LARGE ? most - Ref::AIM : most;
                         now = most - top[rb] > Ref::MOST ? aim : top[rb];
                         if (__any(falls)) {
                             // (a lane has a quarter of its row's sum, and its exponent leaves out up to a bit more)

@@ -44,12 +44,11 @@ constexpr float FAR_SCORE = 1e38f, FAR_NUMBER = 1e18f, BOUND_MOST = 1e30f, SIZE_
 constexpr float SUM_SCALE = 16777216.0f;       // lifts fp32's smallest numbers into bf16's normal range
 constexpr float COUNTED = 0x1p100f;            // training leaves out what is larger
 constexpr float NEAR = 0x1p126f;               // vectors shorter than 2^63 are added by products: 1024 of them, times SUM_SCALE, stay inside fp32
-// Training's sums.  Products add up so many vectors at a time in fp32, in a step of 32 vectors for each piece of their numbers, each off by half a
-// step or a whole one; what they give goes into LDS by an addition whose error is kept and goes on with the next products.  Equal numbers err
-// the same way in every step, so a sum is off by up to 34 * 2^-24 of its numbers' sizes (pieces * (vectors / 32 + 1) / 2 steps, twice
-// 2^-24 each, and 2^-24 where it is stored); added over the whole chunk in one go, 4096 fp32 copies of a number gave a mean up to 162 * 2^-24 off,
-// now 6.  Costs 1 to 3% of an iteration.
-constexpr int fold_after(int pieces) { return pieces == 1 ? 1024 : pieces == 2 ? 512 : 256; }
+// Training's sums.  Products add up so many vectors at a time in fp32, in a step of 32 vectors for each piece of their numbers, each off by a step
+// (2^-23 of the sum so far) at most; what they give goes into LDS by an addition whose error is kept and goes on with the next products.  Equal
+// numbers err the same way in every step, so a sum is off by up to 2^-17 of its numbers' sizes (32 steps by 1 or 2 pieces, or 8 by 3);
+// added over the whole chunk in one go, 4096 fp32 copies of a number gave a mean up to 162 * 2^-24 off, now 6.  Costs 1 to 3% of an iteration.
+constexpr int fold_after(int pieces) { return pieces == 1 ? 1024 : pieces == 2 ? 512 : 256; }      // vectors
 
 __device__ inline uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 
