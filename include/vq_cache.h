@@ -64,8 +64,9 @@ int vq_cache_read(const int64_t *slots, int64_t tokens, const void *k_cb, const 
  * page number outside [0, pages) are not seen.  Codewords have to be finite; a code of K or more stands for some codeword or for zeros.  max_q and
  * max_kv, the longest of the sequences' rows and lengths as the caller knows them, only shape the launch: any value of
  * 1 or more gives the same sums, up to the order of addition.
- * Scores, weights and sums are fp32; weights are rounded to `dtype` before they meet the values, their sum takes them unrounded.  Of fp16 a
- * weight is off by half a step, or by 2^-19 of the largest that its row has among the 32 tokens it is taken with.
+ * Scores, weights and sums are fp32, which holds the sums of bf16 values up to 2^120 divided by the number of tokens.  Weights are rounded to
+ * `dtype` before they meet the values; their sum takes them unrounded.  Of fp16 a weight is off by half a step, or by 2^-19 of the
+ * largest that its row has among the 32 tokens it is taken with.
  * `starts` rises, from 0 or more to `rows` or less.  dtype: VQ_BF16 or VQ_F16. */
 size_t vq_cache_attention_ws_bytes(int64_t rows, int q_heads, int heads, int dim, int sub, int K, int seqs,
                                    int64_t max_q, int64_t max_kv);

@@ -138,6 +138,25 @@ def test_attention_of_one_token_is_its_value(eng, dtype, D, rows):
     assert torch.equal(out[1:], value.expand(rows, 4, D))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 12])
+def test_attention_of_the_largest_values(eng, dtype, rows):
+    """A mean of the type's largest numbers is none larger, though weights whose rounding is all upwards make it one by a step."""
+    n, D, sub, K = 32, 64, 4, 64
+    q, k_cb, v_cb, kc, vc, table, kv_lens, starts = attention_case([rows], [n], 4, 2, D, sub, K, 16, dtype, seed=91)
+    q[:], k_cb[:], kc[:] = 0.25, 0.0, 1
+    k_cb[:, 0] = 1.0                                                     # one token's score is 16, the others' 0; one wave takes them all
+    kc[int(table[0, 0]), :, 3] = 0
+    v_cb[:] = torch.finfo(dtype).max * (1 if dtype == torch.float16 else 2.0 ** -20)     # (fp32's sums hold 2^20 of the latter)
+    v_cb[:, :, ::2] *= -1
+    weight = 0.5 + 1.05 * HALF[dtype] / 2                                # of the others: a little above the middle of two neighbours
+    case = (q, k_cb, v_cb, kc, vc, table, kv_lens, starts)
+    scale = -math.log(weight) / 16
+    out, lse = eng.cache_attention(*[t.to(DEV) for t in case], rows, scale=scale, want_lse=True)
+    assert out.isfinite().all()
+    check_attention(out, lse, attention64(*case, sub, scale), n)
+
+
 @pytest.mark.parametrize("scale", [3e-38, -2e-39, 1e-44])
 def test_attention_tiny_scale(eng, scale):
     """A scale near or below fp32's smallest normal number is taken as it is."""

@@ -48,6 +48,9 @@ template <> __device__ inline uint32_t pack2<_Float16>(float lo, float hi) {
     const f16x2 v = {(_Float16)lo, (_Float16)hi};
     return __builtin_bit_cast(uint32_t, v);
 }
+// The mean of finite values is none larger than the largest; where the weights' rounding makes it so, it may not become fp16's infinity.
+template <typename T> __device__ inline float bounded(float v) { return v; }
+template <> __device__ inline float bounded<_Float16>(float v) { return v > 65504.0f ? 65504.0f : v < -65504.0f ? -65504.0f : v; }
 
 // The rows and the length of sequence b, kept inside the tensors whatever the device arrays hold.
 __device__ inline void sequence(const AttendArgs &a, int b, int64_t &first, int &n_q, int &n_kv) {
@@ -148,8 +151,8 @@ template <typename T>
 __device__ inline void store_row(const AttendArgs &a, int64_t place, int D, int c, f32x4 v0, f32x4 v1, float most, float sum) {
     const float over = sum == 0.0f ? 0.0f : 1.0f / sum;              // 0: the row sees no token (of any other the largest weight is 1 or more)
     *reinterpret_cast<u32x4 *>(static_cast<T *>(a.out) + place * D + c * 8) =
-        (u32x4){pack2<T>(v0[0] * over, v0[1] * over), pack2<T>(v0[2] * over, v0[3] * over),
-                pack2<T>(v1[0] * over, v1[1] * over), pack2<T>(v1[2] * over, v1[3] * over)};
+        (u32x4){pack2<T>(bounded<T>(v0[0] * over), bounded<T>(v0[1] * over)), pack2<T>(bounded<T>(v0[2] * over), bounded<T>(v0[3] * over)),
+                pack2<T>(bounded<T>(v1[0] * over), bounded<T>(v1[1] * over)), pack2<T>(bounded<T>(v1[2] * over), bounded<T>(v1[3] * over))};
     // (the sum's power of two goes to `most` first: where the reference came down far, the two are large and nearly cancel)
     if (c == 0 && a.lse)
         a.lse[place] = sum == 0.0f ? -INFINITY : ((most + (float)__builtin_amdgcn_frexp_expf(sum)) + log2f(__builtin_amdgcn_frexp_mantf(sum))) * 0.69314718055994531f;
