@@ -336,12 +336,15 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
                 codes[p * page_bytes + (which == 0 ? o * parts : o)] = (uint8_t)code;
             }
         } else {
-            bool fine = token < end;
+            const bool near = token < end && size < NEAR;
+            bool fine = near;                                             // it counts; of longer ones (and of NaN) those do whose numbers all are small enough
+            if (__builtin_expect(__any(token < end && !near), 0)) {
+                fine = token < end;
 #pragma unroll
-            for (int e = 0; e < SUB; ++e) fine = fine && fabsf(x[e]) < COUNTED;
+                for (int e = 0; e < SUB; ++e) fine = fine && fabsf(x[e]) < COUNTED;
+            }
             // sums by products with the one-hot numbers of the codewords: number = 16 hi + lo, and
             // sum[hi][lo] = sum over vectors of (x where its hi is this row) * (1 where its lo is this column)
-            const bool near = size < NEAR;
             counted += __popcll(__ballot(fine));
             if (fine) {
                 double f = 0.0;
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(SEARCH_WAVES * 64) void k_cache_search(const Search
                 }
                 away += f <= INFINITY ? f : INFINITY;
             }
-            s_hi[wave][lane] = fine && near ? (uint16_t)(code >> 4) : (uint16_t)0xffff;
+            s_hi[wave][lane] = near ? (uint16_t)(code >> 4) : (uint16_t)0xffff;
             s_lo[wave][lane] = (uint16_t)(code & 15);
 #pragma unroll
             for (int e = 0; e < SUB; ++e) {
