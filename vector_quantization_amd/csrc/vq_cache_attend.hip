@@ -16,10 +16,12 @@
 //   key table is part-major: 16 lanes read 16 codes of one part, which clash as random numbers do.
 //
 // What it reaches (8 cache heads, 32 query heads, 128 dims, 256 codewords, parts of 4; bf16) and what bounds it:
-//   16 sequences of 20000 tokens on average, a token each: 58 us; 10 to 14 of them to the first tile and to the end, then 4.4 TB/s of codes.
-//     One wave's chain (codes, look-ups, products, softmax) is the limit: two waves a SIMD are all that the registers leave.  LDS
-//     is busy for two thirds of the cycles (a third of them clashes of key look-ups), VALU half, the matrix unit a sixth.
-//   2048 new tokens on 16384: 670 us, 770 TFLOP/s, 56% of what the library's plain product reaches.  VALU 59%, LDS 59%, matrix unit 32%.
+//   16 sequences of 20000 tokens on average, a token each: 58 us, 54 here and 5 in the join.  A call on 501 tokens takes 10, nearly all of it tables,
+//     range and one chain to the first tile; what is left for the 161 MB of codes is 44 us, 3.7 TB/s.  There one wave's chain (codes, look-ups,
+//     products, softmax) is the limit: two waves a SIMD are all that the registers leave.  Of the busy cycles LDS has 49% and clashes of
+//     key look-ups 30%, VALU 52%, the matrix unit 17%.
+//   2048 new tokens on 16384: 665 us, 775 TFLOP/s, 57% of what the library's plain product reaches.  VALU 64%, LDS 45% and clashes 27%, matrix unit
+//     33%: all eight waves hold the same 32 rows, so every tile of tokens is looked up and transposed for each 32 rows anew.
 // Measured and not kept: 64 rows to a workgroup (863 us for that chunk, where 32 took 690), 16 waves (75 us where 8 took 62 for
 // the 16 sequences).
 //

@@ -9,14 +9,16 @@
 //      A second-best group more than twice that behind (GAP) holds no nearest codeword.
 //   2. The 8 codewords of the best group by direct differences in fp32, each sum off by less than 2^-19 of itself.
 //   3. Vectors that either step leaves open (close calls, ties, values beyond fp32's range, what is not finite) are searched by the whole wave
-//      in fp64, by the definition: about one in a hundred.
+//      in fp64, by the definition: one in 600 to 900 where vectors and codewords are of one size (counted with these bounds on the CPU).
 //
 // A wave keeps its part's 256 codewords in registers as the operand of step 1 and streams its tokens past them.
 //
 // What it reaches (8 heads, 128 dims in parts of 4, 256 codewords, bf16): 16384 tokens' keys and values written in 113 us, an iteration
-// on 32768 vectors a head in 168 us: 75 and 50 G sub-vectors/s, 19 and 13 T distances/s.  Bound by the VALU, busy for 89% of the cycles; of
+// on 32768 vectors a head in 172 us: 75 and 49 G sub-vectors/s, 19 and 12 T distances/s.  Bound by the VALU, busy for 90% of the cycles; of
 // 436 operations on 64 sub-vectors, 224 take the least of the scores (7 for 8 of them; the matrix unit is busy a quarter of the time), 88
 // are step 2's, 20 step 3's.  A write of a few tokens is 7 us of latency: codewords, operand, one turn.
+// The same by parts of 2 and 8: written in 324 and 74 us, trained in 326 and 137; in fp16, whose numbers are two pieces a side, four terms and an
+// operand that has to be moved, written in 345, 151 and 108 and trained in 340, 222 and 172; trained on fp32 in 366, 264 and 215.
 // Groups of 16 in step 1 would save 48 operations there and cost 88 in step 2; vectors 32 at a time took 155 and 211 us.
 #include "vq_cache_internal.h"
 
@@ -508,7 +510,7 @@ SearchPlan vq_internal_search_plan(int64_t tokens, int heads, int dim, int sub, 
     const int64_t side = SEARCH_WAVES / p.pw;                             // token ranges side by side in one workgroup
     const int64_t base = (int64_t)heads * (parts / p.pw) * both;
     // A workgroup takes 8 parts, or 4 where they do not come by eights (dims of 96 by 8); two workgroups for each compute unit, or one in
-    // training by parts of 8, whose registers leave no room for two (8192 vectors, 4 heads: 45 us; in two rounds 54).  A write is spread as
+    // training by parts of 8, whose registers and LDS leave no room for two (8192 vectors, 4 heads: 46 us; in two rounds 54).  A write is spread as
     // thinly as turns of 64 tokens allow (256 tokens: 7.8 us; turns of 128 9.4).  A training chunk of fewer than 128 costs more to gather
     // than it saves (1000 vectors, 4 heads: 19.4 us; of 64 20.1, of 256 23.1), and none is longer than 4096: its sums are fp32.
     const int fewest = both == 2 ? 64 : 128, longest = both == 2 ? 1 << 24 : 4096;
